@@ -86,9 +86,31 @@ SIGNATURES = {
     "cdx_sum_reduce_rows_f64": (_int, [_vp, _vp, _i64, _i64, _vp, _sz, _vp]),
     "cdx_activation_forward_f64": (_int, [_vp, _vp, _i64, _int, _f32, _vp]),
     "cdx_activation_backward_f64": (_int, [_vp, _vp, _vp, _i64, _int, _f32, _vp]),
+    "cdx_layer_norm_forward": (_int, [_vp, _i64, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64,
+                                      ctypes.c_double, _int, _int, _vp]),
+    "cdx_layer_norm_backward_workspace_size": (_sz, [_i64, _i64, _int]),
+    "cdx_layer_norm_backward": (_int, [_vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp,
+                                       _i64, _i64, _int, _int, _vp, _sz, _vp]),
+    "cdx_quantize_e4m3": (_int, [_vp, _i64, _i64, _i64, _int, _int, _vp, _i64, _vp, _i64, _int,
+                                 _vp]),
+    "cdx_dequantize_e4m3": (_int, [_vp, _i64, _vp, _i64, _int, _int, _vp, _i64, _i64, _i64, _int,
+                                   _vp]),
+    "cdx_gemm_e4m3_workspace_size": (_sz, [_i64] * 3),
+    "cdx_gemm_e4m3": (_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _int, _vp, _i64, _vp, _i64,
+                             _int, _vp, _i64, _int, _vp, _int, _vp, _sz, _vp]),
+    "cdx_linear_e4m3_workspace_size": (_sz, [_i64] * 3),
+    "cdx_linear_e4m3": (_int, [_i64, _i64, _i64, _vp, _i64, _int, _vp, _i64, _vp, _i64, _int,
+                               _vp, _i64, _int, _vp, _int, _vp, _sz, _vp]),
+    "cdx_activation_forward_e4m3": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _int,
+                                           _i64, _i64, _int, _int, _f32, _vp]),
+    "cdx_activation_backward_e4m3": (_int, [_vp, _i64, _vp, _i64, _vp, _i64, _int, _vp, _i64,
+                                            _i64, _i64, _int, _int, _f32, _vp]),
+    "cdx_linear_weight_grad_e4m3_workspace_size": (_sz, [_i64, _i64, _i64, _int]),
+    "cdx_linear_weight_grad_e4m3": (_int, [_vp, _i64, _int, _vp, _i64, _vp, _i64, _vp, _vp, _i64,
+                                           _i64, _i64, _vp, _sz, _vp]),
 }
 
-DTYPE_F32, DTYPE_F64, DTYPE_F16, DTYPE_BF16 = 0, 1, 2, 3
+DTYPE_F32, DTYPE_F64, DTYPE_F16, DTYPE_BF16, DTYPE_E8M0 = 0, 1, 2, 3, 4
 BINARY_ADD, BINARY_SUB, BINARY_MUL = 0, 1, 2
 
 _lib = None

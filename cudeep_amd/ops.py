@@ -6,9 +6,10 @@ host before any launch, so a bad call raises instead of faulting.
 """
 from __future__ import annotations
 
-import torch
-
 import ctypes
+from typing import NamedTuple
+
+import torch
 
 from . import _lib as L
 
@@ -590,3 +591,351 @@ def total_sum(x):
     out = torch.empty((1,), device=x.device, dtype=x.dtype)
     L.call("cdx_sum", x.data_ptr(), out.data_ptr(), x.numel(), _dtype_code(x), None, 0, _stream())
     return out
+
+
+# ---- layer norm and the 8-bit block-scaled format ------------------------------------------
+
+_FLOATS = {torch.float32: L.DTYPE_F32, torch.float16: L.DTYPE_F16, torch.bfloat16: L.DTYPE_BF16}
+_SCALES = {torch.float8_e8m0fnu: L.DTYPE_E8M0, torch.float32: L.DTYPE_F32}
+_E4M3 = torch.float8_e4m3fn
+_BLOCK = 128
+
+
+def _float_code(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    code = _FLOATS.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}")
+    return code
+
+
+def _rows(t, name):
+    """(rows, columns, leading dimension) of a tensor seen as a matrix of its last
+    dimension: any strides for two dimensions but a unit one in the last, dense beyond."""
+    shape = t.shape
+    if len(shape) == 2:
+        rows, cols = shape
+        ld, step = t.stride()
+        if step != 1 and cols > 1:
+            raise ValueError(f"{name} must have unit column stride")
+        if rows > 1 and ld < cols:
+            raise ValueError(f"{name}: rows overlap")
+        return rows, cols, ld if ld >= cols and rows > 1 else cols
+    if not shape:
+        raise ValueError(f"{name} must have a last dimension")
+    if not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous (or 2-D with unit column stride)")
+    cols = shape[-1]
+    rows = 1
+    for d in shape[:-1]:
+        rows *= d
+    return rows, cols, cols
+
+
+def _workspace(workspace, nbytes, device):
+    """_scratch with the caller's workspace checked."""
+    if workspace is not None:
+        if not isinstance(workspace, torch.Tensor) or not workspace.is_cuda \
+                or not workspace.is_contiguous():
+            raise ValueError("workspace must be a contiguous device tensor")
+    return _scratch(workspace, nbytes, device)
+
+
+def _like(out, name, shape, dtype, device):
+    if out is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _need(out, name, dtype)
+    if out.shape != shape:
+        raise ValueError(f"{name} has the wrong shape")
+    return out
+
+
+def _param(p, name, dim, dtype):
+    if not isinstance(p, torch.Tensor) or not p.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    if p.dtype != dtype and p.dtype != torch.float32:
+        raise TypeError(f"{name} must be {dtype} or float32, got {p.dtype}")
+    if p.dim() != 1 or p.shape[0] != dim or not p.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [{dim}] tensor")
+    return p.data_ptr()
+
+
+def layer_norm(x, weight=None, bias=None, eps=1e-5, *, stats=False, out=None):
+    """Layer norm over the last dimension of a float32, float16 or bfloat16 tensor (2-D: any
+    row stride); sums in float32.  weight and bias are of x's type or float32 (both the
+    same).  With stats, (y, mean, rstd), float32 [rows], as layer_norm_backward takes them."""
+    code = _float_code(x, "input")
+    rows, dim, ldx = _rows(x, "input")
+    if dim < 1:
+        raise ValueError("layer_norm: the last dimension is empty")
+    y = _like(out, "out", x.shape, x.dtype, x.device)
+    wptr = bptr = None
+    pcode = code
+    if weight is not None:
+        wptr = _param(weight, "weight", dim, x.dtype)
+        pcode = _FLOATS[weight.dtype]
+    if bias is not None:
+        bptr = _param(bias, "bias", dim, x.dtype)
+        if weight is not None and bias.dtype != weight.dtype:
+            raise TypeError("weight and bias must have the same type")
+        pcode = _FLOATS[bias.dtype]
+    mean = rstd = None
+    mptr = rptr = None
+    if stats:
+        both = torch.empty((2, rows), dtype=torch.float32, device=x.device)
+        mean, rstd = both[0], both[1]
+        mptr = both.data_ptr()
+        rptr = mptr + 4 * rows
+    L.call("cdx_layer_norm_forward", x.data_ptr(), ldx, wptr, bptr, y.data_ptr(),
+           _rows(y, "out")[2], mptr, rptr, rows, dim, eps, code, pcode, _stream())
+    return (y, mean, rstd) if stats else y
+
+
+def layer_norm_backward(grad_out, x, mean, rstd, weight=None, *, params=True, param_dtype=None,
+                        out=None, workspace=None):
+    """(grad of x, of weight, of bias) of layer_norm, from the statistics it returned.  The
+    parameters' gradients are of `param_dtype` (weight's type, else x's), None each without
+    `params`.  `workspace` (layer_norm_backward_workspace_bytes) makes the call
+    allocation-free."""
+    code = _float_code(x, "input")
+    _need(grad_out, "grad_out", x.dtype)
+    if grad_out.shape != x.shape:
+        raise ValueError("layer_norm_backward: grad_out and input differ in shape")
+    rows, dim, ldx = _rows(x, "input")
+    ldg = _rows(grad_out, "grad_out")[2]
+    if dim < 1:
+        raise ValueError("layer_norm_backward: the last dimension is empty")
+    for t, name in ((mean, "mean"), (rstd, "rstd")):
+        _need(t, name)
+        if t.numel() != rows or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous tensor of {rows} elements")
+    wptr = None
+    pdtype = param_dtype or x.dtype
+    if weight is not None:
+        wptr = _param(weight, "weight", dim, x.dtype)
+        if param_dtype is not None and param_dtype != weight.dtype:
+            raise TypeError("param_dtype must be weight's type")
+        pdtype = weight.dtype
+    if pdtype != x.dtype and pdtype != torch.float32:
+        raise TypeError(f"param_dtype must be {x.dtype} or float32")
+    dx = _like(out, "out", x.shape, x.dtype, x.device)
+    dw = db = None
+    wsp, wsb, _keep = None, 0, None
+    dwp = dbp = None
+    if params:
+        both = torch.empty((2, dim), dtype=pdtype, device=x.device)
+        dw, db = both[0], both[1]
+        dwp = both.data_ptr()
+        dbp = dwp + dim * both.element_size()
+        wsp, wsb, _keep = _workspace(
+            workspace, lambda: layer_norm_backward_workspace_bytes(rows, dim, x.dtype), x.device)
+    L.call("cdx_layer_norm_backward", grad_out.data_ptr(), ldg, x.data_ptr(), ldx, wptr,
+           mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _rows(dx, "out")[2], dwp, dbp,
+           rows, dim, code, _FLOATS[pdtype], wsp, wsb, _stream())
+    return dx, dw, db
+
+
+def layer_norm_backward_workspace_bytes(rows: int, dim: int, dtype=torch.float32) -> int:
+    return int(L.lib().cdx_layer_norm_backward_workspace_size(rows, dim, _FLOATS[dtype]))
+
+
+class Block8(NamedTuple):
+    """A matrix in 8 bits: `q`, float8_e4m3fn [rows, cols], and `scale`, one for each 128
+    columns of a row ([rows, ceil(cols / 128)], tile_rows 1) or each 128 x 128 tile
+    ([ceil(rows / 128), ceil(cols / 128)], tile_rows 128), as float8_e8m0fnu (a power of two) or
+    float32.  A value is q * scale."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    tile_rows: int = 1
+
+    @property
+    def shape(self):
+        return self.q.shape
+
+
+def _block8(b, name, tile_rows=None):
+    """(rows, cols, q pointer, ld, scale pointer, ld, scale code) of a checked Block8."""
+    if not isinstance(b, Block8):
+        raise TypeError(f"{name} must be a Block8")
+    q, s = b.q, b.scale
+    if q.dtype != _E4M3:
+        raise TypeError(f"{name}.q must be float8_e4m3fn, got {q.dtype}")
+    code = _SCALES.get(s.dtype)
+    if code is None:
+        raise TypeError(f"{name}.scale must be float8_e8m0fnu or float32, got {s.dtype}")
+    if not (q.is_cuda and s.is_cuda):
+        raise ValueError(f"{name} must be on the device")
+    if q.dim() != 2 or s.dim() != 2:
+        raise ValueError(f"{name}: q and scale must be 2-D")
+    if b.tile_rows not in (1, _BLOCK) or (tile_rows is not None and b.tile_rows != tile_rows):
+        raise ValueError(f"{name}: tile_rows must be "
+                         f"{tile_rows if tile_rows is not None else '1 or 128'}, got {b.tile_rows}")
+    rows, cols, ldq = _rows(q, f"{name}.q")
+    want = (rows if b.tile_rows == 1 else -(-rows // _BLOCK), -(-cols // _BLOCK))
+    if tuple(s.shape) != want:
+        raise ValueError(f"{name}.scale must be {list(want)}, got {list(s.shape)}")
+    return rows, cols, q.data_ptr(), ldq, s.data_ptr(), _rows(s, f"{name}.scale")[2], code
+
+
+def _empty8(rows, cols, tile_rows, scale_dtype, device):
+    """An uninitialised Block8 whose rows begin on 16-byte boundaries (what the products'
+    wide loads want)."""
+    ld = -(-cols // 16) * 16
+    q = torch.empty((rows, ld), dtype=_E4M3, device=device)
+    if ld != cols:
+        q = q[:, :cols]
+    tiles = rows if tile_rows == 1 else -(-rows // _BLOCK)
+    return Block8(q, torch.empty((tiles, -(-cols // _BLOCK)), dtype=scale_dtype, device=device),
+                  tile_rows), ld
+
+
+def quantize8(x, tile_rows=1, *, scale_dtype=torch.float8_e8m0fnu):
+    """x [rows, cols] (float32, float16, bfloat16) as a Block8: activations with a scale for
+    each 128 columns of a row (tile_rows 1), weights with one for each 128 x 128 tile
+    (tile_rows 128).  A scale is the least power of two under which the block's largest finite
+    magnitude is at most 448 (1 for a block of zeros); infinities and NaN become NaN."""
+    code = _float_code(x, "input")
+    if x.dim() != 2:
+        raise ValueError("quantize8: input must be 2-D")
+    if tile_rows not in (1, _BLOCK):
+        raise ValueError("quantize8: tile_rows must be 1 or 128")
+    scode = _SCALES.get(scale_dtype)
+    if scode is None:
+        raise TypeError("quantize8: scale_dtype must be float8_e8m0fnu or float32")
+    rows, cols, ldx = _rows(x, "input")
+    b, ld = _empty8(rows, cols, tile_rows, scale_dtype, x.device)
+    L.call("cdx_quantize_e4m3", x.data_ptr(), ldx, rows, cols, code, tile_rows, b.q.data_ptr(), ld,
+           b.scale.data_ptr(), b.scale.shape[1], scode, _stream())
+    return b
+
+
+def dequantize8(b, dtype=torch.float32, out=None):
+    """The values of a Block8, rounded to `dtype`."""
+    rows, cols, q, ldq, s, lds, scode = _block8(b, "input")
+    code = _FLOATS.get(dtype)
+    if code is None:
+        raise TypeError("dequantize8: dtype must be float32, float16 or bfloat16")
+    out = _like(out, "out", b.q.shape, dtype, b.q.device)
+    L.call("cdx_dequantize_e4m3", q, ldq, s, lds, scode, b.tile_rows, out.data_ptr(),
+           _rows(out, "out")[2], rows, cols, code, _stream())
+    return out
+
+
+def _vector(bias, n, name="bias"):
+    if bias is None:
+        return None
+    _need(bias, name)
+    if bias.numel() != n or not bias.is_contiguous():
+        raise ValueError(f"{name} has the wrong size or is not contiguous")
+    return bias.data_ptr()
+
+
+def gemm8(a, b, *, bias=None, epilogue=L.EPI_NONE, dtype=torch.bfloat16, out=None,
+          workspace=None):
+    """C = epi(A B^T + bias) of two Block8 matrices, A [M, K] with tile_rows 1 and B [N, K] (a
+    Linear layer's weight) with tile_rows 128; float32 sums, C of `dtype`, bias float32."""
+    M, K, aq, lda, asc, ldsa, acode = _block8(a, "A", 1)
+    N, K2, bq, ldb, bsc, ldsb, bcode = _block8(b, "B", _BLOCK)
+    if K != K2:
+        raise ValueError(f"inner dimensions differ: {K} vs {K2}")
+    code = _FLOATS.get(dtype)
+    if code is None:
+        raise TypeError("gemm8: dtype must be float32, float16 or bfloat16")
+    out = _like(out, "out", (M, N), dtype, a.q.device)
+    ws_ptr, ws_bytes, _keep = _workspace(
+        workspace, lambda: L.lib().cdx_gemm_e4m3_workspace_size(M, N, K), a.q.device)
+    L.call("cdx_gemm_e4m3", M, N, K, aq, lda, asc, ldsa, acode, bq, ldb, bsc, ldsb, bcode,
+           out.data_ptr(), _rows(out, "out")[2], code, _vector(bias, N), epilogue, ws_ptr,
+           ws_bytes, _stream())
+    return out
+
+
+def gemm8_workspace_bytes(M: int, N: int, K: int) -> int:
+    return int(L.lib().cdx_gemm_e4m3_workspace_size(M, N, K))
+
+
+def linear8(x, weight, bias=None, *, epilogue=L.EPI_NONE, dtype=None, out=None, workspace=None):
+    """epi(x W^T + bias) with W a Block8 [N, K] (tile_rows 128) and x [M, K] quantised on the way
+    in as quantize8(x) does; the result is of `dtype` (x's own by default)."""
+    xcode = _float_code(x, "input")
+    if x.dim() != 2:
+        raise ValueError("linear8: input must be 2-D")
+    M, K, ldx = _rows(x, "input")
+    N, K2, bq, ldb, bsc, ldsb, bcode = _block8(weight, "weight", _BLOCK)
+    if K != K2:
+        raise ValueError(f"inner dimensions differ: {K} vs {K2}")
+    dtype = dtype or x.dtype
+    code = _FLOATS.get(dtype)
+    if code is None:
+        raise TypeError("linear8: dtype must be float32, float16 or bfloat16")
+    out = _like(out, "out", (M, N), dtype, x.device)
+    ws_ptr, ws_bytes, _keep = _workspace(
+        workspace, lambda: L.lib().cdx_linear_e4m3_workspace_size(M, N, K), x.device)
+    L.call("cdx_linear_e4m3", M, N, K, x.data_ptr(), ldx, xcode, bq, ldb, bsc, ldsb, bcode,
+           out.data_ptr(), _rows(out, "out")[2], code, _vector(bias, N), epilogue, ws_ptr,
+           ws_bytes, _stream())
+    return out
+
+
+def linear8_workspace_bytes(M: int, N: int, K: int) -> int:
+    return int(L.lib().cdx_linear_e4m3_workspace_size(M, N, K))
+
+
+def activation8(z, act, *, alpha=0.01, scale_dtype=torch.float8_e8m0fnu, out=None):
+    """(act(z), z as a Block8) in one pass over z [rows, cols]: what the backward pass keeps of
+    an activation's input.  act as for `activation`."""
+    code = _float_code(z, "input")
+    if z.dim() != 2:
+        raise ValueError("activation8: input must be 2-D")
+    scode = _SCALES.get(scale_dtype)
+    if scode is None:
+        raise TypeError("activation8: scale_dtype must be float8_e8m0fnu or float32")
+    rows, cols, ldz = _rows(z, "input")
+    y = _like(out, "out", z.shape, z.dtype, z.device)
+    b, ld = _empty8(rows, cols, 1, scale_dtype, z.device)
+    L.call("cdx_activation_forward_e4m3", z.data_ptr(), ldz, y.data_ptr(), _rows(y, "out")[2],
+           b.q.data_ptr(), ld, b.scale.data_ptr(), b.scale.shape[1], scode, rows, cols, code, act,
+           alpha, _stream())
+    return y, b
+
+
+def activation_backward8(grad_out, z, act, *, alpha=0.01, out=None):
+    """grad_out * act'(z) with z a Block8 (tile_rows 1)."""
+    code = _float_code(grad_out, "grad_out")
+    rows, cols, q, ldq, s, lds, scode = _block8(z, "input", 1)
+    if tuple(grad_out.shape) != (rows, cols):
+        raise ValueError("activation_backward8: grad_out and input differ in shape")
+    ldg = _rows(grad_out, "grad_out")[2]
+    out = _like(out, "out", grad_out.shape, grad_out.dtype, grad_out.device)
+    L.call("cdx_activation_backward_e4m3", grad_out.data_ptr(), ldg, q, ldq, s, lds, scode,
+           out.data_ptr(), _rows(out, "out")[2], rows, cols, code, act, alpha, _stream())
+    return out
+
+
+def linear_weight_grad8(grad_out, x, *, bias=True, workspace=None):
+    """(weight gradient [N, K], bias gradient [N] or None) of a Linear layer from its output's
+    gradient [M, N] (float32, float16, bfloat16) and its input kept as a Block8 [M, K] (tile_rows
+    1, float8_e8m0fnu scales); both float32, exact products, float32 sums."""
+    code = _float_code(grad_out, "grad_out")
+    M, K, q, ldq, s, lds, scode = _block8(x, "input", 1)
+    if scode != L.DTYPE_E8M0:
+        raise TypeError("linear_weight_grad8: the input's scales must be float8_e8m0fnu")
+    if grad_out.dim() != 2 or grad_out.shape[0] != M:
+        raise ValueError(f"linear_weight_grad8: grad_out must be [{M}, out_features]")
+    N = grad_out.shape[1]
+    ldg = _rows(grad_out, "grad_out")[2]
+    dw = torch.empty((N, K), dtype=torch.float32, device=grad_out.device)
+    db = torch.empty((N,), dtype=torch.float32, device=grad_out.device) if bias else None
+    ws_ptr, ws_bytes, _keep = _workspace(
+        workspace, lambda: L.lib().cdx_linear_weight_grad_e4m3_workspace_size(M, N, K, code),
+        grad_out.device)
+    L.call("cdx_linear_weight_grad_e4m3", grad_out.data_ptr(), ldg, code, q, ldq, s, lds,
+           dw.data_ptr(), db.data_ptr() if bias else None, M, N, K, ws_ptr, ws_bytes, _stream())
+    return dw, db
+
+
+def linear_weight_grad8_workspace_bytes(M: int, N: int, K: int, dtype=torch.float32) -> int:
+    return int(L.lib().cdx_linear_weight_grad_e4m3_workspace_size(M, N, K, _FLOATS[dtype]))

@@ -83,6 +83,8 @@ extern "C" {
 #define CDX_DTYPE_F64  1
 #define CDX_DTYPE_F16  2           /* IEEE binary16 (GEMM operands only) */
 #define CDX_DTYPE_BF16 3           /* bfloat16 (GEMM operands only)      */
+#define CDX_DTYPE_E8M0 4           /* a power of two as one byte, 2^(b - 127), 255 = NaN
+                                      (scales of 8-bit operands only)   */
 
 #define CDX_BINARY_ADD 0
 #define CDX_BINARY_SUB 1
@@ -490,6 +492,104 @@ int cdx_activation_forward_f64(const double* input, double* output, int64_t n,
 int cdx_activation_backward_f64(const double* grad_output, const double* input,
                                 double* grad_input, int64_t n, int act, float alpha,
                                 hipStream_t stream);
+
+/* ---- layer norm -------------------------------------------------------- */
+
+/* y = (x - mu) r w + b over the last dimension of a row-major [rows, dim]
+ * matrix, mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps); sums in fp32.
+ * dtype (x, y): CDX_DTYPE_F32, _F16 or _BF16; param_dtype (weight, bias): dtype
+ * or CDX_DTYPE_F32.  weight and bias may be NULL (1 and 0); mean and rstd (fp32,
+ * one per row, what the backward pass reads) may be NULL.  No counterpart in
+ * the reference's dense path. */
+int cdx_layer_norm_forward(const void* x, int64_t ldx, const void* weight, const void* bias,
+                           void* y, int64_t ldy, float* mean, float* rstd,
+                           int64_t rows, int64_t dim, double eps, int dtype, int param_dtype,
+                           hipStream_t stream);
+
+/* Gradients: with xh = (x - mu) r and g = grad_out w,
+ *   grad_in = r (g - mean(g) - xh mean(g xh)),
+ *   grad_weight = sum over rows of grad_out xh, grad_bias = sum of grad_out.
+ * grad_weight and grad_bias (param_dtype, dense [dim]; overwritten) may be NULL;
+ * weight may be NULL.  The row sums go through per-workgroup partials added in a
+ * fixed order: the same bits every time.  workspace: the query's bytes (0 where
+ * neither is wanted); NULL allocates stream-ordered. */
+size_t cdx_layer_norm_backward_workspace_size(int64_t rows, int64_t dim, int dtype);
+int cdx_layer_norm_backward(const void* grad_out, int64_t ldg, const void* x, int64_t ldx,
+                            const void* weight, const float* mean, const float* rstd,
+                            void* grad_in, int64_t ldgi, void* grad_weight, void* grad_bias,
+                            int64_t rows, int64_t dim, int dtype, int param_dtype,
+                            void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---- 8-bit block-scaled operands ------------------------------------------ */
+
+/* A matrix in 8 bits: e4m3 codes (OCP: largest 448, no infinities) [rows, cols]
+ * with leading dimension ldq, and scales [rows][ceil(cols / 128)] (tile_rows 1: one
+ * for each 128 columns of a row) or [ceil(rows / 128)][ceil(cols / 128)]
+ * (tile_rows 128: one for each 128 x 128 tile) with leading dimension lds, as
+ * bytes (CDX_DTYPE_E8M0) or floats (CDX_DTYPE_F32).  A value is code * scale.
+ *
+ * cdx_quantize_e4m3: the scale is 2^e with the least e in [-117, 120] for which
+ * the block's largest finite magnitude is at most 448 * 2^e (1 for a block
+ * without a finite nonzero), a code is x / scale rounded to nearest even;
+ * infinities and NaN become the NaN code.  dtype: CDX_DTYPE_F32, _F16 or _BF16.
+ * No counterpart in the reference. */
+int cdx_quantize_e4m3(const void* x, int64_t ldx, int64_t rows, int64_t cols, int dtype,
+                      int tile_rows, void* q, int64_t ldq, void* scale, int64_t lds,
+                      int scale_dtype, hipStream_t stream);
+
+/* out[r][c] = code * scale, rounded to dtype. */
+int cdx_dequantize_e4m3(const void* q, int64_t ldq, const void* scale, int64_t lds,
+                        int scale_dtype, int tile_rows, void* out, int64_t ldo,
+                        int64_t rows, int64_t cols, int dtype, hipStream_t stream);
+
+/* C[M,N] = epi(A B^T + bias): A [M,K] with scales by row, B [N,K] (a Linear
+ * layer's weight) with scales by 128 x 128 tile; fp32 sums, C in c_dtype
+ * (CDX_DTYPE_F32, _F16 or _BF16), bias fp32 [N] or NULL, epilogue CDX_EPI_NONE to
+ * _SIGMOID.  The two scale types may differ.  workspace: the query's bytes (scale
+ * types and alignments make no difference); NULL allocates stream-ordered. */
+size_t cdx_gemm_e4m3_workspace_size(int64_t M, int64_t N, int64_t K);
+int cdx_gemm_e4m3(int64_t M, int64_t N, int64_t K,
+                  const void* A, int64_t lda, const void* a_scale, int64_t ldsa, int a_scale_dtype,
+                  const void* B, int64_t ldb, const void* b_scale, int64_t ldsb, int b_scale_dtype,
+                  void* C, int64_t ldc, int c_dtype, const float* bias, int epilogue,
+                  void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* The same with A given as x [M,K] in x_dtype: quantised by row as
+ * cdx_quantize_e4m3 does, then multiplied. */
+size_t cdx_linear_e4m3_workspace_size(int64_t M, int64_t N, int64_t K);
+int cdx_linear_e4m3(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, int x_dtype,
+                    const void* B, int64_t ldb, const void* b_scale, int64_t ldsb,
+                    int b_scale_dtype, void* C, int64_t ldc, int c_dtype, const float* bias,
+                    int epilogue, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* ---- 8-bit activation checkpoints ------------------------------------------- */
+
+/* y = act(z), and z in 8 bits (tile_rows 1) for the backward pass, in one pass over
+ * z.  act: CDX_EPI_RELU to _SIGMOID, CDX_ACT_TANH or CDX_ACT_LEAKY_RELU (alpha: its
+ * slope).  16-bit results use the hardware's exponential and reciprocal. */
+int cdx_activation_forward_e4m3(const void* z, int64_t ldz, void* y, int64_t ldy,
+                                void* q, int64_t ldq, void* scale, int64_t lds, int scale_dtype,
+                                int64_t rows, int64_t cols, int dtype, int act, float alpha,
+                                hipStream_t stream);
+/* grad_in = grad_out * act'(z), z restored from its 8 bits. */
+int cdx_activation_backward_e4m3(const void* grad_out, int64_t ldg, const void* q, int64_t ldq,
+                                 const void* scale, int64_t lds, int scale_dtype,
+                                 void* grad_in, int64_t ldgi, int64_t rows, int64_t cols,
+                                 int dtype, int act, float alpha, hipStream_t stream);
+
+/* A Linear layer's weight gradient from its input kept in 8 bits (tile_rows 1,
+ * scales CDX_DTYPE_E8M0):
+ *   grad_weight[n][k] = sum over the batch of dz[m][n] x[m][k]   (fp32, dense),
+ *   grad_bias[n] = sum over the batch of dz[m][n]                (fp32; may be NULL).
+ * dz [batch, out_features] in dtype enters exactly (as one to three bf16 parts) and
+ * so does x; sums fp32, the same bits every time.  workspace as above. */
+size_t cdx_linear_weight_grad_e4m3_workspace_size(int64_t batch, int64_t out_features,
+                                                  int64_t in_features, int dtype);
+int cdx_linear_weight_grad_e4m3(const void* dz, int64_t lddz, int dtype,
+                                const void* q, int64_t ldq, const void* scale, int64_t lds,
+                                float* grad_weight, float* grad_bias, int64_t batch,
+                                int64_t out_features, int64_t in_features,
+                                void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* ---- tensor runtime ----------------------------------------------------- */
 

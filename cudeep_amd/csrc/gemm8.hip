@@ -39,9 +39,14 @@ struct Params {
 __device__ __forceinline__ u32x4 load_codes(const uint8_t* p, int64_t k, int64_t K) {
     if (k + 16 <= K) return load16(p + k);
     u32x4 v = {0u, 0u, 0u, 0u};
-#pragma unroll
-    for (int j = 0; j < 16; ++j)
-        if (k + j < K) v[j >> 2] |= (uint32_t)p[k + j] << (8 * (j & 3));
+    const int n = (int)(K - k);
+#pragma unroll 1
+    for (int j = n < 0 ? -1 : n - 1; j >= 0; --j) {   // the last code first
+        v[3] = v[3] << 8 | v[2] >> 24;
+        v[2] = v[2] << 8 | v[1] >> 24;
+        v[1] = v[1] << 8 | v[0] >> 24;
+        v[0] = v[0] << 8 | p[k + j];
+    }
     return v;
 }
 
@@ -100,19 +105,39 @@ __device__ __forceinline__ floatx4 block_product(const Frag<MODE>& w, const Frag
     }
 }
 
-// Four consecutive n (from n0) of row m: bias, activation, rounding, store.
-template <class T>
-__device__ __forceinline__ void store_four(const Params& p, int64_t m, int64_t n0, floatx4 v) {
-    if (m >= p.M || n0 >= p.N) return;
-    T* c = static_cast<T*>(p.C) + m * p.ldc + n0;
-    const int n = p.N - n0 < 4 ? (int)(p.N - n0) : 4;
-    float o[4];
+// A wave's FN x FM accumulators (first n and m: n0, m0) through bias and
+// activation into C: a lane stores four consecutive n of a row at once.
+template <class T, int ACT, int FN, int FM>
+__device__ __forceinline__ void store_act(const Params& p, int64_t m0, int64_t n0,
+                                          const floatx4 (&acc)[FN][FM]) {
+    const int l16 = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const float b = p.bias && r < n ? p.bias[n0 + r] : 0.0f;
-        o[r] = apply_act(v[r] + b, p.epilogue);
+    for (int i = 0; i < FN; ++i) {
+        const int64_t nn = n0 + 16 * i + 4 * g;
+        const int n = p.N - nn < 0 ? 0 : p.N - nn < 4 ? (int)(p.N - nn) : 4;
+        float b[4] = {};
+        if (p.bias) load_n<4>(p.bias + nn, n, b);
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            const int64_t m = m0 + 16 * j + l16;
+            float o[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = act_fixed<ACT>(acc[i][j][r] + b[r]);
+            if (m < p.M) store_n<4>(static_cast<T*>(p.C) + m * p.ldc + nn, n, o);
+        }
     }
-    store_n<4>(c, n, o);
+}
+
+template <class T, int FN, int FM>
+__device__ __forceinline__ void store_tile(const Params& p, int64_t m0, int64_t n0,
+                                           const floatx4 (&acc)[FN][FM]) {
+    switch (p.epilogue) {
+        case CDX_EPI_RELU: store_act<T, CDX_EPI_RELU>(p, m0, n0, acc); break;
+        case CDX_EPI_GELU: store_act<T, CDX_EPI_GELU>(p, m0, n0, acc); break;
+        case CDX_EPI_SILU: store_act<T, CDX_EPI_SILU>(p, m0, n0, acc); break;
+        case CDX_EPI_SIGMOID: store_act<T, CDX_EPI_SIGMOID>(p, m0, n0, acc); break;
+        default: store_act<T, CDX_EPI_NONE>(p, m0, n0, acc); break;
+    }
 }
 
 // Operands of any alignment and any K, 64 x 64 tiles: four waves of 32 x 32,
@@ -180,20 +205,177 @@ void gemm8_any_kernel(Params p) {
             for (int j = 0; j < 2; ++j)
                 acc[i][j] = block_product<MODE>(wq[i], xq[j], acc[i][j], sa[j], sb, s[j]);
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j)
-            store_four<T>(p, m0 + 32 * wm + 16 * j + l16, n0 + 32 * wn + 16 * i + 4 * g, acc[i][j]);
+    store_tile<T>(p, m0 + 32 * wm, n0 + 32 * wn, acc);
 }
 
-// K = 0: act(bias).
+// The workgroup's tile number as its XCD's share (workgroup b runs on XCD b % 8):
+// each XCD takes a run of neighbouring tiles, which share operands in its L2.
+__device__ __forceinline__ int64_t xcd_tile(int64_t b, int64_t count) {
+    const int64_t each = count / 8, more = count % 8, x = b % 8;
+    return x * each + (x < more ? x : more) + b / 8;
+}
+
+// Aligned operands (16-byte rows) of at least one whole block, BM x BN tiles (BM rows
+// of A, BN of B), WM x WN waves.  A block of 128 columns is one step: its rows go
+// from global memory straight into LDS, one step ahead of the products, two
+// buffers, one barrier a step.  LDS is filled in the order of the lanes, so that
+// the exchange of 16-byte pieces (piece ^ (row & 7)) is made on the side of the
+// global addresses.  The scales of kPanel steps are laid out in LDS at once, the
+// ones that a lane wants in a step side by side: as bytes they are the
+// instruction's scale operand, which picks one byte of a register per 16 rows.
+constexpr int64_t kMaxLd = 1 << 23;   // 256 rows within 32-bit offsets
+template <int MODE> constexpr int kPanel = MODE == kBytes ? 32 : 16;
+
+template <class T, int MODE, int BM, int BN, int WM, int WN>
+__global__ __launch_bounds__(64 * WM * WN)
+void gemm8_tile_kernel(Params p) {
+    constexpr int NT = 64 * WM * WN, ROWS = BM + BN, LOADS = ROWS * 8 / NT;
+    constexpr int FM = BM / WM / 16, FN = BN / WN / 16, P = kPanel<MODE>;
+    static_assert(ROWS * 8 % NT == 0 && BM * 8 % NT == 0, "whole rounds of loads");
+    static_assert(FM % 4 == 0, "whole registers of scale bytes");
+    using S = std::conditional_t<MODE == kBytes, uint8_t, float>;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2][ROWS * 128];
+    __shared__ __attribute__((aligned(16))) S panel[P][WM][16][FM];
+    const int tid = threadIdx.x, lane = tid & 63, l16 = tid & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave % WM, wn = wave / WM;
+    const int64_t tiles_m = ceil_div(p.M, (int64_t)BM), tiles_n = ceil_div(p.N, (int64_t)BN);
+    // eight tiles of A's rows at a time, all of B's
+    int64_t id = xcd_tile(blockIdx.x, tiles_m * tiles_n);
+    const int64_t first = id / (8 * tiles_n) * 8;
+    const int64_t high = tiles_m - first < 8 ? tiles_m - first : 8;
+    id -= first * tiles_n;
+    const int64_t m0 = (first + id % high) * BM, n0 = id / high * BN;
+
+    // offsets from the tile's first row; rows past the last one read it again, and
+    // what they give is not stored
+    const uint8_t* base_a = p.a + m0 * p.lda;
+    const uint8_t* base_b = p.b + n0 * p.ldb;
+    const int rows_a = p.M - m0 < BM ? (int)(p.M - m0) : BM, rows_b = p.N - n0 < BN ? (int)(p.N - n0) : BN;
+    const int c16 = 16 * ((tid & 7) ^ ((tid >> 3) & 7));
+    uint32_t off[LOADS];
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const bool is_b = i * NT >= BM * 8;
+        const int row = (i * NT + tid) / 8 - (is_b ? BM : 0), rows = is_b ? rows_b : rows_a;
+        off[i] = (uint32_t)(row < rows ? row : rows - 1) * (uint32_t)(is_b ? p.ldb : p.lda) + c16;
+    }
+    const int64_t whole = p.K / kBlock;   // blocks without a ragged end
+    auto fetch = [&](int64_t kb, int buf) {
+        typedef const __attribute__((address_space(1))) uint32_t* G;
+        typedef const __attribute__((address_space(1))) uint8_t* G8;
+        typedef __attribute__((address_space(3))) uint32_t* L;
+        // (kept apart from the offsets: scalar base + 32-bit offset, one VGPR a load)
+        uint64_t a = (uint64_t)(base_a + kb * kBlock), b = (uint64_t)(base_b + kb * kBlock);
+        asm("" : "+s"(a), "+s"(b));
+#pragma unroll
+        for (int i = 0; i < LOADS; ++i) {
+            uint32_t o = off[i];
+            asm("" : "+v"(o));
+            __builtin_amdgcn_global_load_lds((G)((G8)(i * NT >= BM * 8 ? b : a) + o),
+                                             (L)(&lds[buf][(i * NT + wave * 64) * 16]), 16, 0, 0);
+        }
+    };
+    auto fetch_end = [&](int64_t kb, int buf) {   // the last, ragged block: zeros past K
+#pragma unroll 1
+        for (int i = 0; i < LOADS; ++i) {
+            const bool is_b = i * NT >= BM * 8;
+            const int row = (i * NT + tid) / 8 - (is_b ? BM : 0), rows = is_b ? rows_b : rows_a;
+            const uint8_t* s = (is_b ? base_b : base_a) +
+                               (int64_t)(row < rows ? row : rows - 1) * (is_b ? p.ldb : p.lda);
+            *reinterpret_cast<u32x4*>(&lds[buf][(i * NT + tid) * 16]) = load_codes(s, kb * kBlock + c16, p.K);
+        }
+    };
+    auto fetch_panel = [&](int64_t kb) {   // A's scales of steps kb .. kb + P - 1
+        for (int i = tid; i < BM * P; i += NT) {
+            const int row = i / P, k = i % P;   // a row's scales lie side by side
+            const int64_t m = m0 + (row < rows_a ? row : rows_a - 1);
+            S v = 0;
+            if (kb + k < p.blocks) {
+                if constexpr (MODE == kBytes) v = static_cast<const uint8_t*>(p.sa)[m * p.ldsa + kb + k];
+                else v = load_scale(p.sa, m * p.ldsa + kb + k, p.a_e8m0);
+            }
+            panel[k][row / (16 * FM)][row % 16][row % (16 * FM) / 16] = v;
+        }
+    };
+    // the wave's rows of B lie in one tile of 128
+    const int64_t tile_b = (n0 + wn * (BN / WN)) / kBlock, last_tile = (p.N - 1) / kBlock;
+    const int64_t sb_row = (tile_b < last_tile ? tile_b : last_tile) * p.ldsb;
+    auto scale_b = [&](int64_t kb) {
+        if constexpr (MODE == kBytes) return (int)static_cast<const uint8_t*>(p.sb)[sb_row + kb];
+        else return load_scale(p.sb, sb_row + kb, p.b_e8m0);
+    };
+    floatx4 acc[FN][FM] = {};
+    fetch(0, 0);
+    fetch_panel(0);
+    auto sb = scale_b(0);
+    const int lo = ((2 * g) ^ (l16 & 7)) * 16, hi = lo ^ 16;
+    for (int64_t kb = 0; kb < p.blocks; ++kb) {
+        const int buf = (int)(kb & 1), k = (int)(kb % P);
+        if (k == 0 && kb > 0) {
+            __syncthreads();   // the last panel's readers are done
+            fetch_panel(kb);
+        }
+        __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this step's rows are in LDS
+        __syncthreads();
+        const auto cb = sb;
+        if (kb + 1 < p.blocks) {
+            sb = scale_b(kb + 1);
+            if (kb + 1 < whole) fetch(kb + 1, buf ^ 1);
+            else fetch_end(kb + 1, buf ^ 1);
+        }
+        const uint8_t* xrow = &lds[buf][(wm * (BM / WM) + l16) * 128];
+        const uint8_t* wrow = &lds[buf][(BM + wn * (BN / WN) + l16) * 128];
+        Frag<MODE> xq[FM];
+#pragma unroll
+        for (int j = 0; j < FM; ++j)
+            xq[j].set(*reinterpret_cast<const u32x4*>(xrow + j * 2048 + lo),
+                      *reinterpret_cast<const u32x4*>(xrow + j * 2048 + hi));
+        S sa[FM];
+        __builtin_memcpy(sa, panel[k][wm][l16], sizeof(sa));
+        int words[FM / 4];
+        float cs[FM];
+        if constexpr (MODE == kBytes) {
+            __builtin_memcpy(words, sa, sizeof(words));
+        } else {
+#pragma unroll
+            for (int j = 0; j < FM; ++j) cs[j] = sa[j] * cb;
+        }
+#pragma unroll
+        for (int i = 0; i < FN; ++i) {
+            Frag<MODE> wq;
+            wq.set(*reinterpret_cast<const u32x4*>(wrow + i * 2048 + lo),
+                   *reinterpret_cast<const u32x4*>(wrow + i * 2048 + hi));
+            if constexpr (MODE == kBytes) {
+#pragma unroll
+                for (int j = 0; j < FM; j += 4) {
+#define CDX_MFMA8(J) \
+    acc[i][j + J] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wq.q, xq[j + J].q, acc[i][j + J], \
+                                                                     0, 0, 0, cb, J, words[j / 4])
+                    CDX_MFMA8(0);
+                    CDX_MFMA8(1);
+                    CDX_MFMA8(2);
+                    CDX_MFMA8(3);
+#undef CDX_MFMA8
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < FM; ++j)
+                    acc[i][j] = block_product<MODE>(wq, xq[j], acc[i][j], 0, 0, cs[j]);
+            }
+        }
+    }
+    store_tile<T>(p, m0 + wm * (BM / WM), n0 + wn * (BN / WN), acc);
+}
+
+// K = 0: act(bias), a thread to a 16 x 16 tile's lane.
 template <class T>
-__global__ __launch_bounds__(256)
+__global__ __launch_bounds__(64)
 void gemm8_empty_kernel(Params p) {
-    const int64_t four = ceil_div(p.N, (int64_t)4), n = p.M * four;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (int64_t)gridDim.x * 256)
-        store_four<T>(p, i / four, i % four * 4, floatx4{0.0f, 0.0f, 0.0f, 0.0f});
+    const floatx4 zero[1][1] = {};
+    const int64_t tiles_m = ceil_div(p.M, (int64_t)16), n = tiles_m * ceil_div(p.N, (int64_t)16);
+    for (int64_t i = blockIdx.x; i < n; i += gridDim.x)
+        store_tile<T>(p, i % tiles_m * 16, i / tiles_m * 16, zero);
 }
 
 // Calls f with the way a result type and scale types call for.
@@ -207,10 +389,29 @@ template <class T, class F> int with_mode(const Params& p, F f) {
 template <class T>
 int run(const Params& p, hipStream_t stream) {
     if (p.K == 0) {
-        const int64_t g = ceil_div(p.M * ceil_div(p.N, (int64_t)4), (int64_t)256);
-        hipLaunchKernelGGL(gemm8_empty_kernel<T>, dim3((unsigned)(g < 65536 ? g : 65536)), dim3(256), 0,
+        const int64_t g = ceil_div(p.M, (int64_t)16) * ceil_div(p.N, (int64_t)16);
+        hipLaunchKernelGGL(gemm8_empty_kernel<T>, dim3((unsigned)(g < 65536 ? g : 65536)), dim3(64), 0,
                            stream, p);
         return hip_error(hipGetLastError(), "gemm8_empty_kernel launch");
+    }
+    const bool aligned = p.lda % 16 == 0 && p.ldb % 16 == 0 && ((uintptr_t)p.a | (uintptr_t)p.b) % 16 == 0;
+    if (aligned && p.M > 64 && p.K >= kBlock && p.lda <= kMaxLd && p.ldb <= kMaxLd) {
+        const int64_t big = ceil_div(p.M, (int64_t)256) * ceil_div(p.N, (int64_t)256);
+        const int64_t mid = ceil_div(p.M, (int64_t)128) * ceil_div(p.N, (int64_t)128);
+        if (mid >= (int64_t)1 << 31) return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");
+        return with_mode<T>(p, [&](auto mode) {
+            constexpr int MODE = decltype(mode)::value;
+            if constexpr (MODE != kWide) {
+                if (big >= 200) {
+                    hipLaunchKernelGGL((gemm8_tile_kernel<T, MODE, 256, 256, 2, 4>), dim3((unsigned)big),
+                                       dim3(512), 0, stream, p);
+                    return hip_error(hipGetLastError(), "gemm8_tile_kernel launch");
+                }
+            }
+            hipLaunchKernelGGL((gemm8_tile_kernel<T, MODE, 128, 128, 2, 2>), dim3((unsigned)mid),
+                               dim3(256), 0, stream, p);
+            return hip_error(hipGetLastError(), "gemm8_tile_kernel launch");
+        });
     }
     const int64_t grid = ceil_div(p.M, (int64_t)64) * ceil_div(p.N, (int64_t)64);
     if (grid >= (int64_t)1 << 31) return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");

@@ -215,6 +215,13 @@ __device__ __forceinline__ void unpack_e4m3(uint32_t w, float (&v)[4]) {
     v[0] = lo[0]; v[1] = lo[1]; v[2] = hi[0]; v[3] = hi[1];
 }
 
+// The workgroup's tile number as its XCD's share (workgroup b runs on XCD b % 8):
+// each XCD takes a run of neighbouring tiles, which share operands in its L2.
+__device__ __forceinline__ int64_t xcd_tile(int64_t b, int64_t count) {
+    const int64_t each = count / 8, more = count % 8, x = b % 8;
+    return x * each + (x < more ? x : more) + b / 8;
+}
+
 // An 8-bit matrix: codes with leading dimension ldq, scales [rows (or tiles
 // of 128 rows)][ceil(cols / 128)] with leading dimension lds.
 struct Mat8 {

@@ -208,13 +208,6 @@ void gemm8_any_kernel(Params p) {
     store_tile<T>(p, m0 + 32 * wm, n0 + 32 * wn, acc);
 }
 
-// The workgroup's tile number as its XCD's share (workgroup b runs on XCD b % 8):
-// each XCD takes a run of neighbouring tiles, which share operands in its L2.
-__device__ __forceinline__ int64_t xcd_tile(int64_t b, int64_t count) {
-    const int64_t each = count / 8, more = count % 8, x = b % 8;
-    return x * each + (x < more ? x : more) + b / 8;
-}
-
 // Aligned operands (16-byte rows) of at least one whole block, BM x BN tiles (BM rows
 // of A, BN of B), WM x WN waves.  A block of 128 columns is one step: its rows go
 // from global memory straight into LDS, one step ahead of the products, two

@@ -8,10 +8,13 @@
 // may lose bits).  Every product is then exact in fp32 and the sums are fp32, so
 // the gradient is that of the restored input with no rounding but the sums'.
 //
-// Both operands have the sum's index m as their slow one.  Tiles are staged in
-// LDS as they lie, [m][n] and [m][k], and ds_read_b64_tr_b16 gives each lane the
-// four m of its column.  Few output tiles: m is split over workgroups, whose
-// partials a second kernel adds in a fixed order.
+// Both operands have the sum's index m as their slow one.  Tiles lie in LDS as they
+// do in memory, [m][n] and [m][k], and ds_read_b64_tr_b16 gives each lane the four m of
+// its column: 16 lanes read 32 bytes of each of four rows, and a row's 32-byte
+// units are exchanged (unit ^ (m & 3)) so that the four lie on different banks.
+// The next step's loads are in flight while a step is multiplied; two buffers, one
+// barrier a step.  Few output tiles: m is split over workgroups, whose partials a second
+// kernel adds in a fixed order.
 #include "block8.hpp"
 
 namespace cdx {
@@ -21,8 +24,6 @@ using namespace b8;
 
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 
-constexpr int kStep = 32;   // m per step: one v_mfma_f32_16x16x32_bf16
-
 template <class T> constexpr int kParts = std::is_same_v<T, float> ? 3 : std::is_same_v<T, f16> ? 2 : 1;
 
 struct Params {
@@ -30,7 +31,7 @@ struct Params {
     const uint8_t* q; int64_t ldq;
     const uint8_t* s; int64_t lds;
     int64_t M, N, K;
-    int64_t chunk;             // m per slice, a multiple of kStep
+    int64_t chunk;             // m per slice, a multiple of a step
     float* dw; float* db;      // slice z at dw + z * N * K, db + z * N
 };
 
@@ -87,105 +88,166 @@ __device__ __forceinline__ u32x4 restore_bf16(u32x2 w, float scale) {
     return o;
 }
 
-// BN x BK output tiles, WN x WK waves.  LDS rows are padded by 32 bytes: the
-// four rows that 16 lanes read together then fill all banks.
-template <class T, int BN, int BK, int WN, int WK>
+// Eight 16- or 32-bit values as loaded.
+template <class T> struct Raw {
+    u32x4 u[sizeof(T) / 2];
+    __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = load16(reinterpret_cast<const char*>(p) + 16 * i);
+    }
+    __device__ __forceinline__ void load(const T* p, int n) {   // the first n, then zeros
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) u[i] = u32x4{0u, 0u, 0u, 0u};
+        if (n >= 8) {
+            load(p);
+        } else if (n > 0) {
+            T e[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) e[j] = j < n ? p[j] : T(0);
+            __builtin_memcpy(u, e, sizeof(e));
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        T e[8];
+        __builtin_memcpy(e, u, sizeof(e));
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)e[j];
+    }
+};
+
+// BN x BK output tiles, WN x WK waves, MS (a multiple of 32) m a step.
+template <class T, int BN, int BK, int WN, int WK, int MS>
 __global__ __launch_bounds__(64 * WN * WK)
 void wgrad8_kernel(Params p) {
     constexpr int PARTS = kParts<T>, NT = 64 * WN * WK;
     constexpr int FN = BN / WN / 16, FK = BK / WK / 16;
-    constexpr int PN = BN + 16, PK = BK + 16;   // LDS row lengths
-    __shared__ __attribute__((aligned(16))) uint16_t zs[PARTS][kStep][PN];
-    __shared__ __attribute__((aligned(16))) uint16_t xs[kStep][PK];
-    const int tid = threadIdx.x, wave = tid >> 6, l16 = tid & 15, g = (tid >> 4) & 3;
+    __shared__ __attribute__((aligned(128))) uint16_t zs[2][PARTS][MS][BN];
+    __shared__ __attribute__((aligned(128))) uint16_t xs[2][MS][BK];
+    const int tid = threadIdx.x, l16 = tid & 15, g = (tid >> 4) & 3;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave % WN, wk = wave / WN;
     const int64_t tiles_n = ceil_div(p.N, (int64_t)BN);
-    const int64_t n0 = (blockIdx.x % tiles_n) * BN, k0 = (blockIdx.x / tiles_n) * BK;
+    const int64_t id = xcd_tile(blockIdx.x, gridDim.x);
+    const int64_t n0 = id % tiles_n * BN, k0 = id / tiles_n * BK;
     const int64_t m_begin = (int64_t)blockIdx.y * p.chunk;
     const int64_t m_end = m_begin + p.chunk < p.M ? m_begin + p.chunk : p.M;
-    // pieces of eight columns: a thread stages piece column zc (xc) of rows zr, zr + ZR, ...
-    constexpr int ZR = NT / (BN / 8), XR = NT / (BK / 8);
-    static_assert(kStep % ZR == 0 && kStep % XR == 0, "whole rows of pieces");
-    const int zc = 8 * (tid % (BN / 8)), zr = tid / (BN / 8);
-    const int xc = 8 * (tid % (BK / 8)), xr = tid / (BK / 8);
+    // a thread stages eight columns (zc, xc) of rows zr, zr + ZR, ... (xr, xr + XR, ...)
+    constexpr int ZR = NT / (BN / 8), XR = NT / (BK / 8), ZI = MS / ZR, XI = MS / XR;
+    static_assert(MS % ZR == 0 && MS % XR == 0 && ZR % 4 == 0 && XR % 4 == 0, "whole rounds of rows");
+    const int zp = tid % (BN / 8), zr = tid / (BN / 8), zc = 8 * zp;
+    const int xp = tid % (BK / 8), xr = tid / (BK / 8), xc = 8 * xp;
+    const int zpos = 16 * (((zp >> 1) ^ (zr & 3)) << 1 | (zp & 1));   // bytes in an LDS row
+    const int xpos = 16 * (((xp >> 1) ^ (xr & 3)) << 1 | (xp & 1));
     const int64_t z_left = p.N - n0 - zc, x_left = p.K - k0 - xc;
     const int zn = z_left < 0 ? 0 : z_left > 8 ? 8 : (int)z_left;
     const int xn = x_left < 0 ? 0 : x_left > 8 ? 8 : (int)x_left;
+    const bool inner = n0 + BN <= p.N && k0 + BK <= p.K;
     const bool sums = p.db && k0 == 0;
-    float zv[kStep / ZR][8], bsum[8] = {};
-    u32x2 xv[kStep / XR];
-    float xscale[kStep / XR];
-    auto load = [&](int64_t m) {
+    const T* zsrc = static_cast<const T*>(p.dz) + (m_begin + zr) * p.lddz + n0 + zc;
+    const uint8_t* xsrc = p.q + (m_begin + xr) * p.ldq + k0 + xc;
+    const uint8_t* ssrc = p.s + (m_begin + xr) * p.lds + (k0 + xc) / kBlock;
+    const int64_t zstep = ZR * p.lddz, xstep = XR * p.ldq, sstep = XR * p.lds;
+    Raw<T> zv[ZI];
+    u32x2 xv[XI];
+    uint32_t sv[XI];
+    float bsum[8] = {};
+    auto load = [&](int64_t m) {   // rows m .. m + MS - 1; advances the sources
+        if (inner && m + MS <= m_end) {
 #pragma unroll
-        for (int i = 0; i < kStep / ZR; ++i) {
-            const int64_t r = m + zr + i * ZR;
-            load_n<8>(static_cast<const T*>(p.dz) + r * p.lddz + n0 + zc, r < m_end ? zn : 0, zv[i]);
-        }
+            for (int i = 0; i < ZI; ++i) zv[i].load(zsrc + i * zstep);
 #pragma unroll
-        for (int i = 0; i < kStep / XR; ++i) {
-            const int64_t r = m + xr + i * XR;
-            const uint8_t* q = p.q + r * p.ldq + k0 + xc;
-            u32x2 w = {0u, 0u};
-            float sc = 1.0f;
-            if (r < m_end && xn > 0) {
-                uint32_t b = p.s[r * p.lds + (k0 + xc) / kBlock];
-                sc = e8m0_value(b);
-                if (xn == 8) {
-                    w = load8b(q);
+            for (int i = 0; i < XI; ++i) {
+                xv[i] = load8b(xsrc + i * xstep);
+                sv[i] = ssrc[i * sstep];
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < ZI; ++i) zv[i].load(zsrc + i * zstep, m + zr + i * ZR < m_end ? zn : 0);
+#pragma unroll
+            for (int i = 0; i < XI; ++i) {
+                const int n = m + xr + i * XR < m_end ? xn : 0;
+                u32x2 w = {0u, 0u};
+                if (n == 8) {
+                    w = load8b(xsrc + i * xstep);
                 } else {
 #pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (j < xn) w[j >> 2] |= (uint32_t)q[j] << (8 * (j & 3));
+                    for (int j = 0; j < 7; ++j)
+                        if (j < n) w[j >> 2] |= (uint32_t)xsrc[i * xstep + j] << (8 * (j & 3));
                 }
-                if (b == 255) w = u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};   // a NaN scale: NaN codes
+                xv[i] = w;
+                sv[i] = n > 0 ? ssrc[i * sstep] : 127;
             }
-            xv[i] = w;
-            xscale[i] = sc;
         }
+        zsrc += ZI * zstep;
+        xsrc += XI * xstep;
+        ssrc += XI * sstep;
     };
-    floatx4 acc[FN][FK] = {};
-    if (m_begin < m_end) load(m_begin);
-    for (int64_t m = m_begin; m < m_end; m += kStep) {
-        __syncthreads();
+    auto stage = [&](int buf) {
 #pragma unroll
-        for (int i = 0; i < kStep / ZR; ++i) {
+        for (int i = 0; i < ZI; ++i) {
+            float v[8];
+            if (PARTS > 1 || sums) zv[i].get(v);
             u32x4 parts[PARTS];
-            split_parts<PARTS>(zv[i], parts);
+            if constexpr (PARTS == 1) parts[0] = zv[i].u[0];
+            else split_parts<PARTS>(v, parts);
 #pragma unroll
             for (int q = 0; q < PARTS; ++q)
-                *reinterpret_cast<u32x4*>(&zs[q][zr + i * ZR][zc]) = parts[q];
+                *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(zs[buf][q][zr + i * ZR]) + zpos) = parts[q];
             if (sums) {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) bsum[j] += zv[i][j];
+                for (int j = 0; j < 8; ++j) bsum[j] += v[j];
             }
         }
 #pragma unroll
-        for (int i = 0; i < kStep / XR; ++i)
-            *reinterpret_cast<u32x4*>(&xs[xr + i * XR][xc]) = restore_bf16(xv[i], xscale[i]);
-        __syncthreads();
-        if (m + kStep < m_end) load(m + kStep);
-        // operand of lane (l16, g): column l16, m = 8 g + 0..7, as two transposed
-        // reads of four rows; lane i of 16 points at row i / 4, columns 4 (i % 4)
-        const int row = 8 * g + (l16 >> 2), col = 4 * (l16 & 3);
-        auto operand = [&](const uint16_t* base, int pitch) {
-            typedef __attribute__((address_space(3))) shortx4* P3;
-            const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P3)(base + row * pitch + col));
-            const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P3)(base + (row + 4) * pitch + col));
-            return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
-        };
-        bf16x8 xo[FK];
+        for (int i = 0; i < XI; ++i) {
+            u32x2 w = xv[i];
+            if (sv[i] == 255) w = u32x2{0x7f7f7f7fu, 0x7f7f7f7fu};   // a NaN scale: NaN codes
+            *reinterpret_cast<u32x4*>(reinterpret_cast<char*>(xs[buf][xr + i * XR]) + xpos) =
+                restore_bf16(w, e8m0_value(sv[i]));
+        }
+    };
+    // operand of lane (l16, g): column l16 of a unit, m = 8 g + 0..7 of 32, as two reads of
+    // four rows; lane i of 16 points at row i / 4, columns 4 (i % 4)
+    int unit[4];
 #pragma unroll
-        for (int j = 0; j < FK; ++j) xo[j] = operand(&xs[0][16 * (wk * FK + j)], PK);
-        // smallest parts first, as the larger ones then round their sum once
+    for (int b = 0; b < 4; ++b) unit[b] = 32 * (b ^ (l16 >> 2)) + 8 * (l16 & 3);
+    const int row = 8 * g + (l16 >> 2);
+    auto operand = [&](const uint16_t* tile, int pitch, int u) {   // tile: row 0 of 32 m; unit u
+        typedef __attribute__((address_space(3))) shortx4* P3;
+        const char* at = reinterpret_cast<const char*>(tile) + row * pitch + (u >> 2) * 128 + unit[u & 3];
+        const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P3)at);
+        const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P3)(at + 4 * pitch));
+        return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+    };
+    floatx4 acc[FN][FK] = {};
+    if (m_begin < m_end) {
+        load(m_begin);
+        stage(0);
+        if (m_begin + MS < m_end) load(m_begin + MS);
+    }
+    int buf = 0;
+    for (int64_t m = m_begin; m < m_end; m += MS, buf ^= 1) {
+        __syncthreads();   // this step's tiles are whole, and nobody reads the other buffer
+        if (m + MS < m_end) {
+            stage(buf ^ 1);
+            if (m + 2 * MS < m_end) load(m + 2 * MS);
+        }
 #pragma unroll
-        for (int q = PARTS - 1; q >= 0; --q)
+        for (int h = 0; h < MS / 32; ++h) {
+            bf16x8 xo[FK];
 #pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                const bf16x8 zo = operand(&zs[q][0][16 * (wn * FN + i)], PN);
+            for (int j = 0; j < FK; ++j) xo[j] = operand(xs[buf][32 * h], 2 * BK, wk * FK + j);
+            // smallest parts first, as the larger ones then round their sum once
 #pragma unroll
-                for (int j = 0; j < FK; ++j)
-                    acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(zo, xo[j], acc[i][j], 0, 0, 0);
-            }
+            for (int q = PARTS - 1; q >= 0; --q)
+#pragma unroll
+                for (int i = 0; i < FN; ++i) {
+                    const bf16x8 zo = operand(zs[buf][q][32 * h], 2 * BN, wn * FN + i);
+#pragma unroll
+                    for (int j = 0; j < FK; ++j)
+                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(zo, xo[j], acc[i][j], 0, 0, 0);
+                }
+        }
     }
     float* dw = p.dw + (int64_t)blockIdx.y * p.N * p.K;
 #pragma unroll
@@ -193,22 +255,23 @@ void wgrad8_kernel(Params p) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int64_t n = n0 + 16 * (wn * FN + i) + 4 * g + r;
+            float* out = dw + n * p.K + k0 + 16 * wk * FK + l16;
 #pragma unroll
-            for (int j = 0; j < FK; ++j) {
-                const int64_t k = k0 + 16 * (wk * FK + j) + l16;
-                if (n < p.N && k < p.K) dw[n * p.K + k] = acc[i][j][r];
-            }
+            for (int j = 0; j < FK; ++j)
+                if (n < p.N && k0 + 16 * (wk * FK + j) + l16 < p.K) out[16 * j] = acc[i][j][r];
         }
     if (sums) {
         // the staging threads' sums of a column, added in the order of their rows
-        __shared__ float red[ZR][BN];
+        __syncthreads();
+        float* red = reinterpret_cast<float*>(zs);
+        static_assert(sizeof(zs) >= ZR * BN * sizeof(float), "room for the sums");
 #pragma unroll
-        for (int j = 0; j < 8; ++j) red[zr][zc + j] = bsum[j];
+        for (int j = 0; j < 8; ++j) red[zr * BN + zc + j] = bsum[j];
         __syncthreads();
         for (int c = tid; c < BN; c += NT) {
             if (n0 + c >= p.N) break;
-            float a = red[0][c];
-            for (int i = 1; i < ZR; ++i) a += red[i][c];
+            float a = red[c];
+            for (int i = 1; i < ZR; ++i) a += red[i * BN + c];
             p.db[(int64_t)blockIdx.y * p.N + n0 + c] = a;
         }
     }
@@ -238,17 +301,39 @@ void wgrad8_sum_kernel(const float* __restrict__ part, int slices, int64_t nk, i
     }
 }
 
-struct Plan { int64_t tiles; int slices; int64_t chunk; };
+// Tiles of 256, 128 or 64 by as many, and slices of m.
+struct Plan { int side; int64_t tiles; int slices; int64_t chunk; };
 
-// Slices of m: enough workgroups for the 256 CUs, at least 256 m each.
+constexpr int kMost = 64;   // m of the longest step
+
+// (a layer without inputs still has its bias's column of tiles)
+int64_t tiles_of(int64_t N, int64_t K, int side) {
+    return ceil_div(N, (int64_t)side) * (K > 0 ? ceil_div(K, (int64_t)side) : 1);
+}
+
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
-    // (a layer without inputs still has its bias's column of tiles)
-    const int64_t tiles = ceil_div(N, (int64_t)64) * (K > 0 ? ceil_div(K, (int64_t)64) : 1);
-    int64_t s = tiles < 512 ? 512 / tiles : 1;
+    int side = 64;
+    if (tiles_of(N, K, 256) >= 128) side = 256;
+    else if (tiles_of(N, K, 128) >= 8 && M >= 256) side = 128;
+    const int64_t tiles = tiles_of(N, K, side);
+    int64_t s = tiles < 256 ? 256 / tiles : 1;
     if (s > M / 256) s = M / 256;
     if (s < 1) s = 1;
-    const int64_t chunk = ceil_div(ceil_div(M, s), (int64_t)kStep) * kStep;
-    return {tiles, (int)ceil_div(M, chunk), chunk};
+    const int64_t chunk = ceil_div(ceil_div(M, s), (int64_t)kMost) * kMost;
+    return {side, tiles, (int)ceil_div(M, chunk), chunk};
+}
+
+template <class T>
+int run(const Params& p, const Plan& pl, hipStream_t stream) {
+    constexpr int MS = kParts<T> == 1 ? 64 : 32;   // (two steps of three parts fill LDS)
+    const dim3 grid((unsigned)pl.tiles, (unsigned)pl.slices);
+    if (pl.side == 256)
+        hipLaunchKernelGGL((wgrad8_kernel<T, 256, 256, 2, 4, MS>), grid, dim3(512), 0, stream, p);
+    else if (pl.side == 128)
+        hipLaunchKernelGGL((wgrad8_kernel<T, 128, 128, 2, 4, MS>), grid, dim3(512), 0, stream, p);
+    else
+        hipLaunchKernelGGL((wgrad8_kernel<T, 64, 64, 2, 2, MS>), grid, dim3(256), 0, stream, p);
+    return hip_error(hipGetLastError(), "wgrad8_kernel launch");
 }
 
 }  // namespace
@@ -270,11 +355,7 @@ int launch_wgrad8(const void* dz, int64_t lddz, int dtype, const Mat8& x, float*
         p.dw = part;
         p.db = db ? part + (int64_t)pl.slices * N * K : nullptr;
     }
-    const int st = with_dtype(dtype, [&](auto t) {
-        hipLaunchKernelGGL((wgrad8_kernel<decltype(t), 64, 64, 2, 2>),
-                           dim3((unsigned)pl.tiles, (unsigned)pl.slices), dim3(256), 0, stream, p);
-        return hip_error(hipGetLastError(), "wgrad8_kernel launch");
-    });
+    const int st = with_dtype(dtype, [&](auto t) { return run<decltype(t)>(p, pl, stream); });
     if (st || pl.slices == 1) return st;
     const int64_t grid = ceil_div(N * K + (db ? N : 0), (int64_t)256);
     hipLaunchKernelGGL(wgrad8_sum_kernel, dim3((unsigned)(grid < 65536 ? grid : 65536)), dim3(256), 0,

@@ -186,10 +186,11 @@ __device__ __forceinline__ float exp_value(int biased) {   // 2^(biased - 127), 
     return __builtin_bit_cast(float, (uint32_t)biased << 23);
 }
 
-// A scale byte's value: 2^(b - 127), NaN for 255.
+// A scale byte's value: 2^(b - 127) (0: the subnormal 2^-127), NaN for 255; no branches.
 __device__ __forceinline__ float e8m0_value(uint32_t b) {
-    return b == 0 ? __builtin_bit_cast(float, 0x00400000u)
-                  : b == 255 ? __builtin_nanf("") : exp_value((int)b);
+    uint32_t u = b << 23;
+    u = u > 0x00400000u ? u : 0x00400000u;
+    return __builtin_bit_cast(float, u | (b + 1) >> 8 << 22);
 }
 
 __device__ __forceinline__ float load_scale(const void* s, int64_t i, bool e8m0) {

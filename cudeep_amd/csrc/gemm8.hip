@@ -142,7 +142,7 @@ __device__ __forceinline__ void store_tile(const Params& p, int64_t m0, int64_t 
 
 // Operands of any alignment and any K, 64 x 64 tiles: four waves of 32 x 32,
 // each block of 128 staged through registers into LDS.  A row's 16-byte pieces
-// lie at piece ^ (row & 7), so that the 16 rows that lanes read together spread
+// lie at piece ^ (row / 2 & 7), so that the 16 rows that lanes read together spread
 // over all banks.
 template <class T, int MODE>
 __global__ __launch_bounds__(256)
@@ -177,7 +177,7 @@ void gemm8_any_kernel(Params p) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int piece = tid + 256 * i, row = (piece >> 3) & 63, c = piece & 7;
-            lds[piece >= 512][row][c ^ (row & 7)] = stage[i];
+            lds[piece >= 512][row][c ^ (row >> 1 & 7)] = stage[i];
         }
         __syncthreads();
         if (kb + 1 < p.blocks) load(kb + 1);
@@ -196,8 +196,8 @@ void gemm8_any_kernel(Params p) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
             const int ra = 32 * wm + 16 * j + l16, rb = 32 * wn + 16 * j + l16;
-            xq[j].set(lds[0][ra][(2 * g) ^ (ra & 7)], lds[0][ra][(2 * g + 1) ^ (ra & 7)]);
-            wq[j].set(lds[1][rb][(2 * g) ^ (rb & 7)], lds[1][rb][(2 * g + 1) ^ (rb & 7)]);
+            xq[j].set(lds[0][ra][g ^ (ra >> 1 & 7)], lds[0][ra][(g + 4) ^ (ra >> 1 & 7)]);
+            wq[j].set(lds[1][rb][g ^ (rb >> 1 & 7)], lds[1][rb][(g + 4) ^ (rb >> 1 & 7)]);
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -212,7 +212,9 @@ void gemm8_any_kernel(Params p) {
 // of A, BN of B), WM x WN waves.  A block of 128 columns is one step: its rows go
 // from global memory straight into LDS, one step ahead of the products, two
 // buffers, one barrier a step.  LDS is filled in the order of the lanes, so that
-// the exchange of 16-byte pieces (piece ^ (row & 7)) is made on the side of the
+// the exchange of 16-byte pieces (piece ^ (row / 2 & 7); a lane takes pieces g and g + 4:
+// the 16 rows that the hardware reads at a time then lie on all 64 banks, where pieces 2 g
+// and 2 g + 1 under row & 7 took 87 us against 78 at 4096^3) is made on the side of the
 // global addresses.  The scales of kPanel steps are laid out in LDS at once, the
 // ones that a lane wants in a step side by side: as bytes they are the
 // instruction's scale operand, which picks one byte of a register per 16 rows.
@@ -229,6 +231,7 @@ void gemm8_tile_kernel(Params p) {
     using S = std::conditional_t<MODE == kBytes, uint8_t, float>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2][ROWS * 128];
     __shared__ __attribute__((aligned(16))) S panel[P][WM][16][FM];
+    __shared__ S panel_b[P][BN / kBlock];
     const int tid = threadIdx.x, lane = tid & 63, l16 = tid & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave % WM, wn = wave / WM;
@@ -245,7 +248,7 @@ void gemm8_tile_kernel(Params p) {
     const uint8_t* base_a = p.a + m0 * p.lda;
     const uint8_t* base_b = p.b + n0 * p.ldb;
     const int rows_a = p.M - m0 < BM ? (int)(p.M - m0) : BM, rows_b = p.N - n0 < BN ? (int)(p.N - n0) : BN;
-    const int c16 = 16 * ((tid & 7) ^ ((tid >> 3) & 7));
+    const int c16 = 16 * ((tid & 7) ^ ((tid >> 4) & 7));
     uint32_t off[LOADS];
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
@@ -279,7 +282,18 @@ void gemm8_tile_kernel(Params p) {
             *reinterpret_cast<u32x4*>(&lds[buf][(i * NT + tid) * 16]) = load_codes(s, kb * kBlock + c16, p.K);
         }
     };
-    auto fetch_panel = [&](int64_t kb) {   // A's scales of steps kb .. kb + P - 1
+    auto fetch_panel = [&](int64_t kb) {   // the scales of steps kb .. kb + P - 1
+        for (int i = tid; i < P * (BN / kBlock); i += NT) {
+            const int k = i % P;
+            int64_t t = n0 / kBlock + i / P;
+            t = t < (p.N - 1) / kBlock ? t : (p.N - 1) / kBlock;
+            S v = 0;
+            if (kb + k < p.blocks) {
+                if constexpr (MODE == kBytes) v = static_cast<const uint8_t*>(p.sb)[t * p.ldsb + kb + k];
+                else v = load_scale(p.sb, t * p.ldsb + kb + k, p.b_e8m0);
+            }
+            panel_b[k][i / P] = v;
+        }
         for (int i = tid; i < BM * P; i += NT) {
             const int row = i / P, k = i % P;   // a row's scales lie side by side
             const int64_t m = m0 + (row < rows_a ? row : rows_a - 1);
@@ -291,18 +305,10 @@ void gemm8_tile_kernel(Params p) {
             panel[k][row / (16 * FM)][row % 16][row % (16 * FM) / 16] = v;
         }
     };
-    // the wave's rows of B lie in one tile of 128
-    const int64_t tile_b = (n0 + wn * (BN / WN)) / kBlock, last_tile = (p.N - 1) / kBlock;
-    const int64_t sb_row = (tile_b < last_tile ? tile_b : last_tile) * p.ldsb;
-    auto scale_b = [&](int64_t kb) {
-        if constexpr (MODE == kBytes) return (int)static_cast<const uint8_t*>(p.sb)[sb_row + kb];
-        else return load_scale(p.sb, sb_row + kb, p.b_e8m0);
-    };
     floatx4 acc[FN][FM] = {};
     fetch(0, 0);
     fetch_panel(0);
-    auto sb = scale_b(0);
-    const int lo = ((2 * g) ^ (l16 & 7)) * 16, hi = lo ^ 16;
+    const int lo = (g ^ (l16 >> 1)) * 16, hi = lo ^ 64;   // pieces g and g + 4
     for (int64_t kb = 0; kb < p.blocks; ++kb) {
         const int buf = (int)(kb & 1), k = (int)(kb % P);
         if (k == 0 && kb > 0) {
@@ -311,9 +317,7 @@ void gemm8_tile_kernel(Params p) {
         }
         __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0): this step's rows are in LDS
         __syncthreads();
-        const auto cb = sb;
         if (kb + 1 < p.blocks) {
-            sb = scale_b(kb + 1);
             if (kb + 1 < whole) fetch(kb + 1, buf ^ 1);
             else fetch_end(kb + 1, buf ^ 1);
         }
@@ -326,6 +330,7 @@ void gemm8_tile_kernel(Params p) {
                       *reinterpret_cast<const u32x4*>(xrow + j * 2048 + hi));
         S sa[FM];
         __builtin_memcpy(sa, panel[k][wm][l16], sizeof(sa));
+        const S cb = panel_b[k][wn * (BN / WN) / kBlock];   // the wave's rows of B lie in one tile
         int words[FM / 4];
         float cs[FM];
         if constexpr (MODE == kBytes) {
@@ -361,6 +366,136 @@ void gemm8_tile_kernel(Params p) {
     store_tile<T>(p, m0 + wm * (BM / WM), n0 + wn * (BN / WN), acc);
 }
 
+// Few rows of A: operands from global memory straight into registers, a block's
+// 128 columns split over eight waves, whose sums meet in LDS in the order of the
+// waves.  A workgroup takes 16 NT rows of B and 16 MT of A; each wave has the codes of
+// U blocks in flight.  With X the rows of A are quantised here, as they are used:
+// every workgroup does it again, in the shadow of its loads of B.
+constexpr int kDirectWaves = 8;
+
+template <class X, int MODE>
+__device__ __forceinline__ void quantize_frag(const X* x, int n, Frag<MODE>& f, int& e) {
+    float v[4][8];
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        load_n<8>(x + 8 * j, n - 8 * j, v[j]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_mag(v[j][k]));
+    }
+    m = fmaxf(m, __shfl_xor(m, 16));   // the four lanes of a row and block
+    m = fmaxf(m, __shfl_xor(m, 32));
+    e = scale_exp(m);
+    const float inv = exp_value(254 - e);
+    u32x4 q[2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        q[j >> 1][2 * (j & 1)] = pack_e4m3(v[j][0], v[j][1], v[j][2], v[j][3], inv);
+        q[j >> 1][2 * (j & 1) + 1] = pack_e4m3(v[j][4], v[j][5], v[j][6], v[j][7], inv);
+    }
+    f.set(q[0], q[1]);
+}
+
+template <class T, int MODE, int MT, int NT, class X>
+__global__ __launch_bounds__(64 * kDirectWaves)
+void gemm8_direct_kernel(Params p, const X* __restrict__ x, int64_t ldx) {
+    constexpr int NW = kDirectWaves, U = MT * NT <= 2 ? 4 : 2;
+    __shared__ floatx4 red[NW][NT * MT][64];
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t tiles_n = ceil_div(p.N, (int64_t)(16 * NT));
+    const int64_t n0 = blockIdx.x % tiles_n * (16 * NT), m0 = blockIdx.x / tiles_n * (16 * MT);
+    // a lane's row of each operand tile (rows past the last read it again)
+    const uint8_t *b[NT], *a[MT];
+    const X* xr[MT];
+    int64_t sa_row[MT];
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+        const int64_t n = n0 + 16 * i + l16;
+        b[i] = p.b + (n < p.N ? n : p.N - 1) * p.ldb;
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        int64_t m = m0 + 16 * j + l16;
+        m = m < p.M ? m : p.M - 1;
+        a[j] = p.a + m * p.lda;
+        xr[j] = x + m * ldx;
+        sa_row[j] = m * p.ldsa;
+    }
+    const int64_t sb_row = n0 / kBlock * p.ldsb;
+    floatx4 acc[NT][MT] = {};
+    auto product = [&](int64_t kb, const Frag<MODE> (&wq)[NT], auto ragged) {
+        constexpr bool RAGGED = decltype(ragged)::value;
+        const int64_t k = kb * kBlock + 32 * g;
+        int sb = 0;
+        float fb = 0.0f;
+        if constexpr (MODE == kBytes) sb = static_cast<const uint8_t*>(p.sb)[sb_row + kb];
+        else fb = load_scale(p.sb, sb_row + kb, p.b_e8m0);
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+            Frag<MODE> xq;
+            int sa = 0;
+            float s = 0.0f;
+            if constexpr (std::is_same_v<X, uint8_t>) {   // codes
+                if constexpr (RAGGED) xq.set(load_codes(a[j], k, p.K), load_codes(a[j], k + 16, p.K));
+                else xq.set(load16(a[j] + k), load16(a[j] + k + 16));
+                if constexpr (MODE == kBytes) sa = static_cast<const uint8_t*>(p.sa)[sa_row[j] + kb];
+                else s = load_scale(p.sa, sa_row[j] + kb, p.a_e8m0);
+            } else {
+                const int64_t left = RAGGED ? p.K - k : 32;
+                quantize_frag<X, MODE>(xr[j] + k, left < 32 ? (int)left : 32, xq, sa);
+                s = exp_value(sa);
+            }
+#pragma unroll
+            for (int i = 0; i < NT; ++i) acc[i][j] = block_product<MODE>(wq[i], xq, acc[i][j], sa, sb, s * fb);
+        }
+    };
+    const int64_t whole = p.K / kBlock;
+    int64_t kb = wave;
+    for (; kb + (U - 1) * NW < whole; kb += U * NW) {
+        u32x4 w[U][NT][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < NT; ++i) {
+                const uint8_t* q = b[i] + (kb + u * NW) * kBlock + 32 * g;
+                w[u][i][0] = load16(q);
+                w[u][i][1] = load16(q + 16);
+            }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            Frag<MODE> wq[NT];
+#pragma unroll
+            for (int i = 0; i < NT; ++i) wq[i].set(w[u][i][0], w[u][i][1]);
+            product(kb + u * NW, wq, std::false_type{});
+        }
+    }
+    for (; kb < p.blocks; kb += NW) {
+        Frag<MODE> wq[NT];
+        const int64_t k = kb * kBlock + 32 * g;
+        if (kb < whole) {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) wq[i].set(load16(b[i] + k), load16(b[i] + k + 16));
+            product(kb, wq, std::false_type{});
+        } else {
+#pragma unroll
+            for (int i = 0; i < NT; ++i) wq[i].set(load_codes(b[i], k, p.K), load_codes(b[i], k + 16, p.K));
+            product(kb, wq, std::true_type{});
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int j = 0; j < MT; ++j) red[wave][i * MT + j][lane] = acc[i][j];
+    __syncthreads();
+    for (int t = wave; t < NT * MT; t += NW) {
+        floatx4 v[1][1] = {{red[0][t][lane]}};
+#pragma unroll
+        for (int w = 1; w < NW; ++w) v[0][0] += red[w][t][lane];
+        store_tile<T>(p, m0 + 16 * (t % MT), n0 + 16 * (t / MT), v);
+    }
+}
+
 // K = 0: act(bias), a thread to a 16 x 16 tile's lane.
 template <class T>
 __global__ __launch_bounds__(64)
@@ -379,6 +514,37 @@ template <class T, class F> int with_mode(const Params& p, F f) {
     else return f(integral_constant<int, kFloats>{});
 }
 
+// The direct kernel's rows: all products of up to 64 rows, and those whose tiles of
+// 128 x 128 would leave most CUs without one.
+bool is_direct(int64_t M, int64_t N) {
+    return M <= 64 || ceil_div(M, (int64_t)128) * ceil_div(N, (int64_t)128) < 64;
+}
+// ... and those that quantise x as they read it: one tile of 16 rows.
+bool quantizes_inside(int64_t M) { return M <= 16; }
+
+template <class T, class X>
+int run_direct(const Params& p, const X* x, int64_t ldx, hipStream_t stream) {
+    return with_mode<T>(p, [&](auto mode) {
+        constexpr int MODE = decltype(mode)::value;
+        auto go = [&](auto mt, auto nt) {
+            constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value;
+            const int64_t grid = ceil_div(p.M, (int64_t)(16 * MT)) * ceil_div(p.N, (int64_t)(16 * NT));
+            if (grid >= (int64_t)1 << 31) return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");
+            hipLaunchKernelGGL((gemm8_direct_kernel<T, MODE, MT, NT, X>), dim3((unsigned)grid),
+                               dim3(64 * kDirectWaves), 0, stream, p, x, ldx);
+            return hip_error(hipGetLastError(), "gemm8_direct_kernel launch");
+        };
+        using std::integral_constant;
+        if (p.M <= 16) return go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
+        if constexpr (std::is_same_v<X, uint8_t>) {
+            if (p.M <= 32) return go(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+            return go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
+        } else {
+            return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many rows");
+        }
+    });
+}
+
 template <class T>
 int run(const Params& p, hipStream_t stream) {
     if (p.K == 0) {
@@ -387,31 +553,28 @@ int run(const Params& p, hipStream_t stream) {
                            stream, p);
         return hip_error(hipGetLastError(), "gemm8_empty_kernel launch");
     }
-    const bool aligned = p.lda % 16 == 0 && p.ldb % 16 == 0 && ((uintptr_t)p.a | (uintptr_t)p.b) % 16 == 0;
-    if (aligned && p.M > 64 && p.K >= kBlock && p.lda <= kMaxLd && p.ldb <= kMaxLd) {
-        const int64_t big = ceil_div(p.M, (int64_t)256) * ceil_div(p.N, (int64_t)256);
-        const int64_t mid = ceil_div(p.M, (int64_t)128) * ceil_div(p.N, (int64_t)128);
-        if (mid >= (int64_t)1 << 31) return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");
-        return with_mode<T>(p, [&](auto mode) {
-            constexpr int MODE = decltype(mode)::value;
-            if constexpr (MODE != kWide) {
-                if (big >= 200) {
-                    hipLaunchKernelGGL((gemm8_tile_kernel<T, MODE, 256, 256, 2, 4>), dim3((unsigned)big),
-                                       dim3(512), 0, stream, p);
-                    return hip_error(hipGetLastError(), "gemm8_tile_kernel launch");
-                }
-            }
-            hipLaunchKernelGGL((gemm8_tile_kernel<T, MODE, 128, 128, 2, 2>), dim3((unsigned)mid),
-                               dim3(256), 0, stream, p);
-            return hip_error(hipGetLastError(), "gemm8_tile_kernel launch");
-        });
-    }
+    if (is_direct(p.M, p.N)) return run_direct<T>(p, static_cast<const uint8_t*>(nullptr), (int64_t)0, stream);
+    const int64_t big = ceil_div(p.M, (int64_t)256) * ceil_div(p.N, (int64_t)256);
+    const int64_t mid = ceil_div(p.M, (int64_t)128) * ceil_div(p.N, (int64_t)128);
     const int64_t grid = ceil_div(p.M, (int64_t)64) * ceil_div(p.N, (int64_t)64);
     if (grid >= (int64_t)1 << 31) return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");
+    const bool aligned = p.lda % 16 == 0 && p.ldb % 16 == 0 && ((uintptr_t)p.a | (uintptr_t)p.b) % 16 == 0 &&
+                         p.K >= kBlock && p.lda <= kMaxLd && p.ldb <= kMaxLd;
     return with_mode<T>(p, [&](auto mode) {
-        hipLaunchKernelGGL((gemm8_any_kernel<T, decltype(mode)::value>), dim3((unsigned)grid), dim3(256),
-                           0, stream, p);
-        return hip_error(hipGetLastError(), "gemm8_any_kernel launch");
+        constexpr int MODE = decltype(mode)::value;
+        if constexpr (MODE != kWide) {
+            if (aligned && big >= 200) {
+                hipLaunchKernelGGL((gemm8_tile_kernel<T, MODE, 256, 256, 2, 4>), dim3((unsigned)big),
+                                   dim3(512), 0, stream, p);
+                return hip_error(hipGetLastError(), "gemm8_tile_kernel launch");
+            }
+        }
+        if (aligned)
+            hipLaunchKernelGGL((gemm8_tile_kernel<T, MODE, 128, 128, 2, 2>), dim3((unsigned)mid),
+                               dim3(256), 0, stream, p);
+        else
+            hipLaunchKernelGGL((gemm8_any_kernel<T, MODE>), dim3((unsigned)grid), dim3(256), 0, stream, p);
+        return hip_error(hipGetLastError(), "gemm8 kernel launch");
     });
 }
 
@@ -423,7 +586,7 @@ size_t codes_bytes(int64_t M, int64_t K) { return ((size_t)M * (size_t)codes_ld(
 
 size_t gemm8_workspace(int64_t M, int64_t N, int64_t K, bool from_x) {
     (void)N;
-    if (!from_x || M == 0 || K == 0) return 0;
+    if (!from_x || M == 0 || K == 0 || quantizes_inside(M)) return 0;
     return codes_bytes(M, K) + (size_t)M * (size_t)ceil_div(K, (int64_t)kBlock) * 4;
 }
 
@@ -431,6 +594,15 @@ int launch_gemm8(const Gemm8Args& g, hipStream_t stream) {
     const int64_t blocks = ceil_div(g.K, (int64_t)kBlock);
     Params p{g.a.q, g.b.q, g.a.s, g.b.s, g.M, g.N, g.K, g.a.ldq, g.b.ldq, g.a.lds, g.b.lds, g.ldc,
              blocks, g.a.e8m0, g.b.e8m0, g.C, g.bias, g.epilogue};
+    if (g.x && g.K > 0 && quantizes_inside(g.M)) {
+        p.a_e8m0 = p.b_e8m0;   // (the way of the same product from codes)
+        return with_dtype(g.cdtype, [&](auto t) {
+            return with_dtype(g.xdtype, [&](auto xt) {
+                using X = decltype(xt);
+                return run_direct<decltype(t)>(p, static_cast<const X*>(g.x), g.ldx, stream);
+            });
+        });
+    }
     if (g.x && g.K > 0) {
         uint8_t* q = static_cast<uint8_t*>(g.ws);
         void* s = q + codes_bytes(g.M, g.K);

@@ -11,7 +11,7 @@
 // Both operands have the sum's index m as their slow one.  Tiles lie in LDS as they
 // do in memory, [m][n] and [m][k], and ds_read_b64_tr_b16 gives each lane the four m of
 // its column: 16 lanes read 32 bytes of each of four rows, and a row's 32-byte
-// units are exchanged (unit ^ (m & 3)) so that the four lie on different banks.
+// units are exchanged so that the eight rows of 32 lanes lie on different banks.
 // The next step's loads are in flight while a step is multiplied; two buffers, one
 // barrier a step.  Few output tiles: m is split over workgroups, whose partials a second
 // kernel adds in a fixed order.
@@ -115,6 +115,13 @@ template <class T> struct Raw {
     }
 };
 
+// What a row's 32-byte units are exchanged by: rows 0 to 3 and 8 to 11 (4 to 7 and 12 to
+// 15), which 32 lanes read together, differ in it and in the half of the 64
+// banks that they begin at (rows of 64 columns).
+template <int COLS> __device__ __forceinline__ int unit_swap(int m) {
+    return COLS == 64 ? (m >> 1 & 1) | (m >> 2 & 2) : (m & 3) | (m >> 1 & 4);
+}
+
 // BN x BK output tiles, WN x WK waves, MS (a multiple of 32) m a step.
 template <class T, int BN, int BK, int WN, int WK, int MS>
 __global__ __launch_bounds__(64 * WN * WK)
@@ -133,11 +140,11 @@ void wgrad8_kernel(Params p) {
     const int64_t m_end = m_begin + p.chunk < p.M ? m_begin + p.chunk : p.M;
     // a thread stages eight columns (zc, xc) of rows zr, zr + ZR, ... (xr, xr + XR, ...)
     constexpr int ZR = NT / (BN / 8), XR = NT / (BK / 8), ZI = MS / ZR, XI = MS / XR;
-    static_assert(MS % ZR == 0 && MS % XR == 0 && ZR % 4 == 0 && XR % 4 == 0, "whole rounds of rows");
+    static_assert(MS % ZR == 0 && MS % XR == 0 && ZR % 16 == 0 && XR % 16 == 0, "whole rounds of rows");
     const int zp = tid % (BN / 8), zr = tid / (BN / 8), zc = 8 * zp;
     const int xp = tid % (BK / 8), xr = tid / (BK / 8), xc = 8 * xp;
-    const int zpos = 16 * (((zp >> 1) ^ (zr & 3)) << 1 | (zp & 1));   // bytes in an LDS row
-    const int xpos = 16 * (((xp >> 1) ^ (xr & 3)) << 1 | (xp & 1));
+    const int zpos = 16 * (((zp >> 1) ^ unit_swap<BN>(zr)) << 1 | (zp & 1));   // bytes in an LDS row
+    const int xpos = 16 * (((xp >> 1) ^ unit_swap<BK>(xr)) << 1 | (xp & 1));
     const int64_t z_left = p.N - n0 - zc, x_left = p.K - k0 - xc;
     const int zn = z_left < 0 ? 0 : z_left > 8 ? 8 : (int)z_left;
     const int xn = x_left < 0 ? 0 : x_left > 8 ? 8 : (int)x_left;
@@ -208,13 +215,15 @@ void wgrad8_kernel(Params p) {
     };
     // operand of lane (l16, g): column l16 of a unit, m = 8 g + 0..7 of 32, as two reads of
     // four rows; lane i of 16 points at row i / 4, columns 4 (i % 4)
-    int unit[4];
-#pragma unroll
-    for (int b = 0; b < 4; ++b) unit[b] = 32 * (b ^ (l16 >> 2)) + 8 * (l16 & 3);
+    static_assert(BN == BK, "one set of unit offsets");
+    constexpr int UNITS = BN == 64 ? 4 : 8;   // exchanged among each other
     const int row = 8 * g + (l16 >> 2);
+    int unit[UNITS];
+#pragma unroll
+    for (int b = 0; b < UNITS; ++b) unit[b] = 32 * (b ^ unit_swap<BN>(row)) + 8 * (l16 & 3);
     auto operand = [&](const uint16_t* tile, int pitch, int u) {   // tile: row 0 of 32 m; unit u
         typedef __attribute__((address_space(3))) shortx4* P3;
-        const char* at = reinterpret_cast<const char*>(tile) + row * pitch + (u >> 2) * 128 + unit[u & 3];
+        const char* at = reinterpret_cast<const char*>(tile) + row * pitch + u / UNITS * (32 * UNITS) + unit[u % UNITS];
         const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P3)at);
         const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P3)(at + 4 * pitch));
         return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -225,10 +234,13 @@ void wgrad8_kernel(Params p) {
         stage(0);
         if (m_begin + MS < m_end) load(m_begin + MS);
     }
+    // Half of the waves stage the next step before their products and half after them: a
+    // SIMD's two waves are then at different work.
+    const bool early = wave < WN * WK / 2;
     int buf = 0;
     for (int64_t m = m_begin; m < m_end; m += MS, buf ^= 1) {
         __syncthreads();   // this step's tiles are whole, and nobody reads the other buffer
-        if (m + MS < m_end) {
+        if (early && m + MS < m_end) {
             stage(buf ^ 1);
             if (m + 2 * MS < m_end) load(m + 2 * MS);
         }
@@ -237,16 +249,26 @@ void wgrad8_kernel(Params p) {
             bf16x8 xo[FK];
 #pragma unroll
             for (int j = 0; j < FK; ++j) xo[j] = operand(xs[buf][32 * h], 2 * BK, wk * FK + j);
-            // smallest parts first, as the larger ones then round their sum once
+            // smallest parts first, as the larger ones then round their sum once; an
+            // operand of dz is read ahead of the products of the one before it
+            auto dz_operand = [&](int t) {   // t-th of PARTS * FN
+                return operand(zs[buf][PARTS - 1 - t / FN][32 * h], 2 * BN, wn * FN + t % FN);
+            };
+            bf16x8 zo[2];
+            zo[0] = dz_operand(0);
 #pragma unroll
-            for (int q = PARTS - 1; q >= 0; --q)
+            for (int t = 0; t < PARTS * FN; ++t) {
+                if (t + 1 < PARTS * FN) zo[(t + 1) & 1] = dz_operand(t + 1);
+                __builtin_amdgcn_sched_barrier(0);   // (the compiler would read it after them)
 #pragma unroll
-                for (int i = 0; i < FN; ++i) {
-                    const bf16x8 zo = operand(zs[buf][q][32 * h], 2 * BN, wn * FN + i);
-#pragma unroll
-                    for (int j = 0; j < FK; ++j)
-                        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(zo, xo[j], acc[i][j], 0, 0, 0);
-                }
+                for (int j = 0; j < FK; ++j)
+                    acc[t % FN][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(zo[t & 1], xo[j], acc[t % FN][j], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        if (!early && m + MS < m_end) {
+            stage(buf ^ 1);
+            if (m + 2 * MS < m_end) load(m + 2 * MS);
         }
     }
     float* dw = p.dw + (int64_t)blockIdx.y * p.N * p.K;

@@ -15,6 +15,8 @@
 // sums for dw and db in registers over all their rows; one row of partials per
 // workgroup, added in a fixed order by a second kernel: no atomics, the same
 // bits every time.
+#include <algorithm>
+
 #include "block8.hpp"
 
 namespace cdx {
@@ -175,6 +177,28 @@ void layer_norm_long_kernel(const T* __restrict__ x, int64_t ldx, const W* __res
     }
 }
 
+// A 16-byte piece of a row as loaded, zeros past its n elements.
+template <class T> struct Piece {
+    u32x4 u;
+    __device__ __forceinline__ void load(const T* p, int n) {
+        u = u32x4{0u, 0u, 0u, 0u};
+        if (n == kVec<T>) {
+            u = load16(p);
+        } else if (n > 0) {
+            T e[kVec<T>];
+#pragma unroll
+            for (int j = 0; j < kVec<T>; ++j) e[j] = j < n ? p[j] : T(0);
+            __builtin_memcpy(&u, e, 16);
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[kVec<T>]) const {
+        T e[kVec<T>];
+        __builtin_memcpy(e, &u, 16);
+#pragma unroll
+        for (int j = 0; j < kVec<T>; ++j) v[j] = (float)e[j];
+    }
+};
+
 template <int TPR> constexpr int kBwdThreads = TPR > 512 ? TPR : 512;
 
 template <class T, class W, int TPR, int E, bool PARAMS>
@@ -191,37 +215,67 @@ void layer_norm_backward_kernel(const T* __restrict__ dy, int64_t lddy, const T*
     int n[E];
     // the weight stays in registers where 128 of them hold it too
     constexpr bool HOLD_W = TPR < 1024 || E * V < 16;
-    float wv[HOLD_W ? E : 1][V], dw[E][V], db[E][V];
+    W wv[HOLD_W ? E : 1][V];
+    float dw[E][V], db[E][V];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
         const int64_t c = (int64_t)(e * TPR + t) * V;
         n[e] = clip(dim - c, V);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            wv[HOLD_W ? e : 0][j] = 1.0f;
+            wv[HOLD_W ? e : 0][j] = W(1.0f);
             dw[e][j] = db[e][j] = 0.0f;
+            if (HOLD_W && w && j < n[e]) wv[e][j] = w[c + j];
         }
-        if (HOLD_W && w) load_n<V>(w + c, n[e], wv[HOLD_W ? e : 0]);
     }
     // every thread of a workgroup takes the same number of turns (barriers);
-    // past the last row nothing is loaded, added or stored
+    // past the last row nothing is loaded, added or stored.  The next row is on its way
+    // while this one is summed, as loaded (registers hold it for 16-bit types, and for
+    // fp32 up to 8 elements a thread).
+    constexpr bool AHEAD = E * V <= 8 || (sizeof(T) == 2 && TPR < 1024);
+    const int64_t step = (int64_t)gridDim.x * RPB;
+    Piece<T> nx[AHEAD ? E : 1], ng[AHEAD ? E : 1];
+    float nmu = 0.0f, nr = 0.0f;
+    auto fetch = [&](int64_t row) {
+        const bool live = row < rows;
+        nmu = live ? mean[row] : 0.0f;
+        nr = live ? rstd[row] : 0.0f;
+#pragma unroll
+        for (int e = 0; e < (AHEAD ? E : 0); ++e) {
+            const int64_t c = (int64_t)(e * TPR + t) * V;
+            nx[e].load(x + row * ldx + c, live ? n[e] : 0);
+            ng[e].load(dy + row * lddy + c, live ? n[e] : 0);
+        }
+    };
     int phase = 0;
-    for (int64_t base = (int64_t)blockIdx.x * RPB; base < rows; base += (int64_t)gridDim.x * RPB) {
+    fetch((int64_t)blockIdx.x * RPB + sub);
+    for (int64_t base = (int64_t)blockIdx.x * RPB; base < rows; base += step) {
         const int64_t row = base + sub;
         const bool live = row < rows;
         float xv[E][V], gv[E][V];
-        const float mu = live ? mean[row] : 0.0f, r = live ? rstd[row] : 0.0f;
+        const float mu = nmu, r = nr;
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int64_t c = (int64_t)(e * TPR + t) * V;
             const int m = live ? n[e] : 0;
-            load_n<V>(x + row * ldx + c, m, xv[e], mu);
-            load_n<V>(dy + row * lddy + c, m, gv[e]);
+            if constexpr (AHEAD) {
+                nx[e].get(xv[e]);
+                ng[e].get(gv[e]);
+#pragma unroll
+                for (int j = 0; j < V; ++j) xv[e][j] = j < m ? xv[e][j] : mu;
+            } else {
+                const int64_t c = (int64_t)(e * TPR + t) * V;
+                load_n<V>(x + row * ldx + c, m, xv[e], mu);
+                load_n<V>(dy + row * lddy + c, m, gv[e]);
+            }
         }
+        if (base + step < rows) fetch(row + step);
         float s[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            if (!HOLD_W && w) load_n<V>(w + (int64_t)(e * TPR + t) * V, n[e], wv[0]);
+            if (!HOLD_W && w) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) wv[0][j] = j < n[e] ? w[(int64_t)(e * TPR + t) * V + j] : W(0.0f);
+            }
 #pragma unroll
             for (int j = 0; j < V; ++j) {
                 const float xh = (xv[e][j] - mu) * r, d = gv[e][j];
@@ -229,7 +283,7 @@ void layer_norm_backward_kernel(const T* __restrict__ dy, int64_t lddy, const T*
                     dw[e][j] += d * xh;
                     db[e][j] += d;
                 }
-                const float g = d * wv[HOLD_W ? e : 0][j];
+                const float g = d * (float)wv[HOLD_W ? e : 0][j];
                 s[0] += g;
                 s[1] += g * xh;
                 xv[e][j] = xh;
@@ -334,26 +388,35 @@ void layer_norm_backward_long_kernel(const T* __restrict__ dy, int64_t lddy,
     }
 }
 
-// Partials of dw and db of such rows: a thread per column, `chunk` rows.
+// Partials of dw and db of wide rows: 16 bytes of columns a thread, `chunk` rows.
 template <class T>
 __global__ __launch_bounds__(256)
 void layer_norm_columns_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
                                int64_t ldx, const float* __restrict__ mean,
                                const float* __restrict__ rstd, float* __restrict__ part,
                                int64_t rows, int64_t dim, int64_t chunk) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    constexpr int V = kVec<T>;
+    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
     if (c >= dim) return;
+    const int n = clip(dim - c, V);
     const int64_t r0 = (int64_t)blockIdx.y * chunk;
     const int64_t r1 = r0 + chunk < rows ? r0 + chunk : rows;
-    float a = 0.0f, b = 0.0f;
+    float a[V] = {}, b[V] = {};
+#pragma unroll 4
     for (int64_t row = r0; row < r1; ++row) {
-        const float d = (float)dy[row * lddy + c];
-        a += d * (((float)x[row * ldx + c] - mean[row]) * rstd[row]);
-        b += d;
+        const float mu = mean[row], r = rstd[row];
+        float xv[V], gv[V];
+        load_n<V>(x + row * ldx + c, n, xv);
+        load_n<V>(dy + row * lddy + c, n, gv);
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            a[j] += gv[j] * ((xv[j] - mu) * r);
+            b[j] += gv[j];
+        }
     }
-    float* out = part + (int64_t)blockIdx.y * 2 * dim;
-    out[c] = a;
-    out[dim + c] = b;
+    float* out = part + (int64_t)blockIdx.y * 2 * dim + c;
+    store_n<V>(out, n, a);
+    store_n<V>(out + dim, n, b);
 }
 
 // dw and db from `count` rows of partials [2][dim]: 64 columns by 16 lanes of
@@ -393,8 +456,9 @@ void layer_norm_params_kernel(const float* __restrict__ part, int count, int64_t
 }
 
 // The threads per row and 16-byte pieces per thread for a width: the fewest
-// threads that hold it, with up to 32 elements each in the forward pass and 16
-// in the backward one, which keeps five values of each (32 spill).
+// threads that hold it, with up to 32 elements each in the forward pass.  The
+// backward one keeps five values of each and the next row: 8 elements (8192 x 4096
+// in bf16: 47 us, with 16 of half the threads and no row ahead 63), 16 without sums.
 template <class T, bool BWD, class F>
 int with_shape(int64_t dim, F f) {
     constexpr int V = kVec<T>;
@@ -403,13 +467,14 @@ int with_shape(int64_t dim, F f) {
     if (dim <= (int64_t)TPR * EL) return f(integral_constant<int, TPR>{}, integral_constant<int, EL / V>{})
     CDX_LN_SHAPE(16, 8);
     CDX_LN_SHAPE(64, 8);
-    CDX_LN_SHAPE(64, 16);
     if constexpr (BWD) {
+        CDX_LN_SHAPE(128, 8);
         CDX_LN_SHAPE(256, 8);
-        CDX_LN_SHAPE(256, 16);
+        CDX_LN_SHAPE(512, 8);
         CDX_LN_SHAPE(1024, 8);
         CDX_LN_SHAPE(1024, 16);
     } else {
+        CDX_LN_SHAPE(64, 16);
         CDX_LN_SHAPE(64, 32);
         CDX_LN_SHAPE(256, 16);
         CDX_LN_SHAPE(256, 32);
@@ -420,20 +485,22 @@ int with_shape(int64_t dim, F f) {
     return f(integral_constant<int, 0>{}, integral_constant<int, 0>{});
 }
 
-// Rows of partials: workgroups of the backward kernel (two per CU at most).
+// Rows of partials: workgroups of the backward kernel, two per CU at most (one of
+// 1024 threads).  Rows of more than 8192 elements keep no column sums, which would
+// spill: a second pass over x and dy forms them, 32 rows at least each (2048 x 16384:
+// 88 us in bf16 and 140 in fp32, with the sums kept 127 and 161).
 constexpr int kBwdGroups = 512;
-
-int64_t bwd_groups(int64_t rows, int rpb) {
-    const int64_t g = ceil_div(rows, (int64_t)rpb);
-    return g < kBwdGroups ? g : kBwdGroups;
-}
 
 template <class T> int64_t partial_rows(int64_t rows, int64_t dim) {
     int64_t out = 0;
-    (void)with_shape<T, true>(dim, [&](auto tpr, auto) {
-        constexpr int TPR = decltype(tpr)::value;
-        if constexpr (TPR == 0) out = bwd_groups(rows, 32);
-        else out = bwd_groups(rows, kBwdThreads<TPR> / TPR);
+    (void)with_shape<T, true>(dim, [&](auto tpr, auto e) {
+        constexpr int TPR = decltype(tpr)::value, EL = decltype(e)::value * kVec<T>;
+        if constexpr (TPR == 0 || EL > 8) {
+            out = std::min<int64_t>(ceil_div(rows, (int64_t)32), 128);
+        } else {
+            constexpr int NT = kBwdThreads<TPR>;
+            out = std::min<int64_t>(ceil_div(rows, (int64_t)(NT / TPR)), NT > 512 ? kBwdGroups / 2 : kBwdGroups);
+        }
         return 0;
     });
     return out;
@@ -468,30 +535,34 @@ int backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const W* w, c
     const int64_t count = partial_rows<T>(rows, dim);
     int st = with_shape<T, true>(dim, [&](auto tpr, auto e) {
         constexpr int TPR = decltype(tpr)::value, E = decltype(e)::value;
+        constexpr bool WIDE = TPR == 0 || E * kVec<T> > 8;   // column sums apart
         if constexpr (TPR == 0) {
             const int64_t g = rows < (1 << 20) ? rows : (1 << 20);
             hipLaunchKernelGGL((layer_norm_backward_long_kernel<T, W>), dim3((unsigned)g),
                                dim3(1024), 0, stream, dy, lddy, x, ldx, w, mean, rstd, dx, lddx,
                                rows, dim);
-            int st2 = hip_error(hipGetLastError(), "layer_norm_backward_long_kernel launch");
-            if (st2 || !params) return st2;
-            const int64_t chunk = ceil_div(rows, count);
-            hipLaunchKernelGGL((layer_norm_columns_kernel<T>),
-                               dim3((unsigned)ceil_div(dim, (int64_t)256), (unsigned)count),
-                               dim3(256), 0, stream, dy, lddy, x, ldx, mean, rstd, ws, rows, dim,
-                               chunk);
-            return hip_error(hipGetLastError(), "layer_norm_columns_kernel launch");
         } else {
             constexpr int NT = kBwdThreads<TPR>;
-            const dim3 grid((unsigned)count), block(NT);
-            if (params)
-                hipLaunchKernelGGL((layer_norm_backward_kernel<T, W, TPR, E, true>), grid, block, 0,
-                                   stream, dy, lddy, x, ldx, w, mean, rstd, dx, lddx, ws, rows, dim);
-            else
-                hipLaunchKernelGGL((layer_norm_backward_kernel<T, W, TPR, E, false>), grid, block, 0,
-                                   stream, dy, lddy, x, ldx, w, mean, rstd, dx, lddx, ws, rows, dim);
-            return hip_error(hipGetLastError(), "layer_norm_backward_kernel launch");
+            constexpr int most = NT > 512 ? kBwdGroups / 2 : kBwdGroups;
+            const dim3 grid((unsigned)std::min<int64_t>(ceil_div(rows, (int64_t)(NT / TPR)), most));
+            if constexpr (!WIDE) {
+                if (params) {
+                    hipLaunchKernelGGL((layer_norm_backward_kernel<T, W, TPR, E, true>), grid,
+                                       dim3(NT), 0, stream, dy, lddy, x, ldx, w, mean, rstd, dx,
+                                       lddx, ws, rows, dim);
+                    return hip_error(hipGetLastError(), "layer_norm_backward_kernel launch");
+                }
+            }
+            hipLaunchKernelGGL((layer_norm_backward_kernel<T, W, TPR, E, false>), grid, dim3(NT), 0,
+                               stream, dy, lddy, x, ldx, w, mean, rstd, dx, lddx, ws, rows, dim);
         }
+        int st2 = hip_error(hipGetLastError(), "layer_norm_backward_kernel launch");
+        if (st2 || !params || !WIDE) return st2;
+        hipLaunchKernelGGL((layer_norm_columns_kernel<T>),
+                           dim3((unsigned)ceil_div(dim, (int64_t)(256 * kVec<T>)), (unsigned)count),
+                           dim3(256), 0, stream, dy, lddy, x, ldx, mean, rstd, ws, rows, dim,
+                           ceil_div(rows, count));
+        return hip_error(hipGetLastError(), "layer_norm_columns_kernel launch");
     });
     if (st || !params) return st;
     hipLaunchKernelGGL(layer_norm_params_kernel<W>, dim3((unsigned)ceil_div(2 * dim, (int64_t)64)),

@@ -42,22 +42,40 @@ __device__ __forceinline__ float act_value(float v, float alpha) {
     return v;
 }
 
-// grad * act'(v).  s (1 - s) is formed from both exponentials, as neither
-// factor then cancels or meets infinity times zero.
+// s = 1 / (1 + exp(-x)) and r = 1 - s, neither by subtraction.  fp32: from both
+// exponentials, as the elementwise kernels.  16 bits: r = exp(-x) s from one exponential,
+// held finite there: where s is 0, so is r (only s and s r are used).  The GELU backward
+// pass is bound by its exponentials and reciprocals: 8192 x 4096 in bf16 45.6 us with two
+// of each, 38.9 with one.
+template <class T> __device__ __forceinline__ void logistic(float x, float& s, float& r) {
+    if constexpr (std::is_same_v<T, float>) {
+        s = 1.0f / (1.0f + expf(-x));
+        r = 1.0f / (1.0f + expf(x));
+    } else {
+        const float e = __builtin_amdgcn_exp2f(x * -1.44269504f);
+        s = __builtin_amdgcn_rcpf(1.0f + e);
+        r = fminf(e, 0x1p126f) * s;
+    }
+}
+
+// grad * act'(v).
 template <class T, int ACT>
 __device__ __forceinline__ float act_slope(float g, float v, float alpha) {
     if constexpr (ACT == CDX_EPI_RELU) return v > 0.0f ? g : 0.0f;
     if constexpr (ACT == CDX_ACT_LEAKY_RELU) return v > 0.0f ? g : alpha * g;
+    float s, r;
     if constexpr (ACT == CDX_EPI_GELU) {
-        const float u = 0.7978845608f * (v + 0.044715f * v * v * v);
-        const float s = inverse<T>(1.0f + fast_exp<T>(-2.0f * u));
-        const float r = inverse<T>(1.0f + fast_exp<T>(2.0f * u));
+        logistic<T>(2.0f * 0.7978845608f * (v + 0.044715f * v * v * v), s, r);
         const float du = 0.7978845608f * (1.0f + 3.0f * 0.044715f * v * v);
         return g * (s + 2.0f * v * s * r * du);
     }
-    if constexpr (ACT == CDX_EPI_SILU || ACT == CDX_EPI_SIGMOID) {
-        const float s = inverse<T>(1.0f + fast_exp<T>(-v)), r = inverse<T>(1.0f + fast_exp<T>(v));
-        return ACT == CDX_EPI_SILU ? g * (s + v * s * r) : g * (s * r);
+    if constexpr (ACT == CDX_EPI_SILU) {
+        logistic<T>(v, s, r);
+        return g * (s + v * s * r);
+    }
+    if constexpr (ACT == CDX_EPI_SIGMOID) {
+        logistic<T>(v, s, r);
+        return g * (s * r);
     }
     if constexpr (ACT == CDX_ACT_TANH) {
         const float t = tanhf(v);

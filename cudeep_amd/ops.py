@@ -615,24 +615,33 @@ def _float_code(t, name):
 def _rows(t, name):
     """(rows, columns, leading dimension) of a tensor seen as a matrix of its last
     dimension: any strides for two dimensions but a unit one in the last, dense beyond."""
-    shape = t.shape
-    if len(shape) == 2:
-        rows, cols = shape
-        ld, step = t.stride()
-        if step != 1 and cols > 1:
-            raise ValueError(f"{name} must have unit column stride")
-        if rows > 1 and ld < cols:
-            raise ValueError(f"{name}: rows overlap")
-        return rows, cols, ld if ld >= cols and rows > 1 else cols
-    if not shape:
-        raise ValueError(f"{name} must have a last dimension")
-    if not t.is_contiguous():
+    if t.is_contiguous():
+        shape = t.shape
+        if len(shape) == 2:
+            return shape[0], shape[1], shape[1]
+        if not shape:
+            raise ValueError(f"{name} must have a last dimension")
+        cols = shape[-1]
+        rows = 1
+        for d in shape[:-1]:
+            rows *= d
+        return rows, cols, cols
+    if t.dim() != 2:
         raise ValueError(f"{name} must be contiguous (or 2-D with unit column stride)")
-    cols = shape[-1]
-    rows = 1
-    for d in shape[:-1]:
-        rows *= d
-    return rows, cols, cols
+    rows, cols = t.shape
+    ld, step = t.stride()
+    if step != 1 and cols > 1:
+        raise ValueError(f"{name} must have unit column stride")
+    if rows > 1 and ld < cols:
+        raise ValueError(f"{name}: rows overlap")
+    return rows, cols, ld if rows > 1 else cols
+
+
+def _new_like(t):
+    """An uninitialised contiguous tensor of t's shape and type."""
+    if t.is_contiguous():
+        return torch.empty_like(t)   # (half the time of empty with a shape)
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _workspace(workspace, nbytes, device):
@@ -644,13 +653,12 @@ def _workspace(workspace, nbytes, device):
     return _scratch(workspace, nbytes, device)
 
 
-def _like(out, name, shape, dtype, device):
-    if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    _need(out, name, dtype)
+def _out(out, shape, dtype):
+    """Leading dimension of a caller's `out`, checked."""
+    _need(out, "out", dtype)
     if out.shape != shape:
-        raise ValueError(f"{name} has the wrong shape")
-    return out
+        raise ValueError("out has the wrong shape")
+    return _rows(out, "out")[2]
 
 
 def _param(p, name, dim, dtype):
@@ -671,7 +679,10 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, stats=False, out=None):
     rows, dim, ldx = _rows(x, "input")
     if dim < 1:
         raise ValueError("layer_norm: the last dimension is empty")
-    y = _like(out, "out", x.shape, x.dtype, x.device)
+    if out is None:
+        y, ldy = _new_like(x), dim
+    else:
+        y, ldy = out, _out(out, x.shape, x.dtype)
     wptr = bptr = None
     pcode = code
     if weight is not None:
@@ -685,12 +696,11 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5, *, stats=False, out=None):
     mean = rstd = None
     mptr = rptr = None
     if stats:
-        both = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-        mean, rstd = both[0], both[1]
-        mptr = both.data_ptr()
-        rptr = mptr + 4 * rows
-    L.call("cdx_layer_norm_forward", x.data_ptr(), ldx, wptr, bptr, y.data_ptr(),
-           _rows(y, "out")[2], mptr, rptr, rows, dim, eps, code, pcode, _stream())
+        mean = torch.empty((rows,), dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+        mptr, rptr = mean.data_ptr(), rstd.data_ptr()
+    L.call("cdx_layer_norm_forward", x.data_ptr(), ldx, wptr, bptr, y.data_ptr(), ldy, mptr, rptr,
+           rows, dim, eps, code, pcode, _stream())
     return (y, mean, rstd) if stats else y
 
 
@@ -721,19 +731,21 @@ def layer_norm_backward(grad_out, x, mean, rstd, weight=None, *, params=True, pa
         pdtype = weight.dtype
     if pdtype != x.dtype and pdtype != torch.float32:
         raise TypeError(f"param_dtype must be {x.dtype} or float32")
-    dx = _like(out, "out", x.shape, x.dtype, x.device)
+    if out is None:
+        dx, lddx = _new_like(x), dim
+    else:
+        dx, lddx = out, _out(out, x.shape, x.dtype)
     dw = db = None
     wsp, wsb, _keep = None, 0, None
     dwp = dbp = None
     if params:
-        both = torch.empty((2, dim), dtype=pdtype, device=x.device)
-        dw, db = both[0], both[1]
-        dwp = both.data_ptr()
-        dbp = dwp + dim * both.element_size()
+        dw = torch.empty((dim,), dtype=pdtype, device=x.device)
+        db = torch.empty_like(dw)
+        dwp, dbp = dw.data_ptr(), db.data_ptr()
         wsp, wsb, _keep = _workspace(
             workspace, lambda: layer_norm_backward_workspace_bytes(rows, dim, x.dtype), x.device)
     L.call("cdx_layer_norm_backward", grad_out.data_ptr(), ldg, x.data_ptr(), ldx, wptr,
-           mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), _rows(dx, "out")[2], dwp, dbp,
+           mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), lddx, dwp, dbp,
            rows, dim, code, _FLOATS[pdtype], wsp, wsb, _stream())
     return dx, dw, db
 
@@ -760,7 +772,7 @@ def _block8(b, name, tile_rows=None):
     """(rows, cols, q pointer, ld, scale pointer, ld, scale code) of a checked Block8."""
     if not isinstance(b, Block8):
         raise TypeError(f"{name} must be a Block8")
-    q, s = b.q, b.scale
+    q, s, tr = b
     if q.dtype != _E4M3:
         raise TypeError(f"{name}.q must be float8_e4m3fn, got {q.dtype}")
     code = _SCALES.get(s.dtype)
@@ -770,14 +782,15 @@ def _block8(b, name, tile_rows=None):
         raise ValueError(f"{name} must be on the device")
     if q.dim() != 2 or s.dim() != 2:
         raise ValueError(f"{name}: q and scale must be 2-D")
-    if b.tile_rows not in (1, _BLOCK) or (tile_rows is not None and b.tile_rows != tile_rows):
+    if tr not in (1, _BLOCK) or (tile_rows is not None and tr != tile_rows):
         raise ValueError(f"{name}: tile_rows must be "
-                         f"{tile_rows if tile_rows is not None else '1 or 128'}, got {b.tile_rows}")
+                         f"{tile_rows if tile_rows is not None else '1 or 128'}, got {tr}")
     rows, cols, ldq = _rows(q, f"{name}.q")
-    want = (rows if b.tile_rows == 1 else -(-rows // _BLOCK), -(-cols // _BLOCK))
-    if tuple(s.shape) != want:
-        raise ValueError(f"{name}.scale must be {list(want)}, got {list(s.shape)}")
-    return rows, cols, q.data_ptr(), ldq, s.data_ptr(), _rows(s, f"{name}.scale")[2], code
+    srows, scols, lds = _rows(s, f"{name}.scale")
+    if scols != -(-cols // _BLOCK) or srows != (rows if tr == 1 else -(-rows // _BLOCK)):
+        raise ValueError(f"{name}.scale must hold one value for each block, got {list(s.shape)} "
+                         f"for {[rows, cols]} (tile_rows {tr})")
+    return rows, cols, q.data_ptr(), ldq, s.data_ptr(), lds, code
 
 
 def _empty8(rows, cols, tile_rows, scale_dtype, device):
@@ -818,9 +831,12 @@ def dequantize8(b, dtype=torch.float32, out=None):
     code = _FLOATS.get(dtype)
     if code is None:
         raise TypeError("dequantize8: dtype must be float32, float16 or bfloat16")
-    out = _like(out, "out", b.q.shape, dtype, b.q.device)
-    L.call("cdx_dequantize_e4m3", q, ldq, s, lds, scode, b.tile_rows, out.data_ptr(),
-           _rows(out, "out")[2], rows, cols, code, _stream())
+    if out is None:
+        out, ldo = torch.empty((rows, cols), dtype=dtype, device=b.q.device), cols
+    else:
+        ldo = _out(out, (rows, cols), dtype)
+    L.call("cdx_dequantize_e4m3", q, ldq, s, lds, scode, b.tile_rows, out.data_ptr(), ldo, rows,
+           cols, code, _stream())
     return out
 
 
@@ -844,11 +860,14 @@ def gemm8(a, b, *, bias=None, epilogue=L.EPI_NONE, dtype=torch.bfloat16, out=Non
     code = _FLOATS.get(dtype)
     if code is None:
         raise TypeError("gemm8: dtype must be float32, float16 or bfloat16")
-    out = _like(out, "out", (M, N), dtype, a.q.device)
+    if out is None:
+        out, ldo = torch.empty((M, N), dtype=dtype, device=a.q.device), N
+    else:
+        ldo = _out(out, (M, N), dtype)
     ws_ptr, ws_bytes, _keep = _workspace(
         workspace, lambda: L.lib().cdx_gemm_e4m3_workspace_size(M, N, K), a.q.device)
     L.call("cdx_gemm_e4m3", M, N, K, aq, lda, asc, ldsa, acode, bq, ldb, bsc, ldsb, bcode,
-           out.data_ptr(), _rows(out, "out")[2], code, _vector(bias, N), epilogue, ws_ptr,
+           out.data_ptr(), ldo, code, _vector(bias, N), epilogue, ws_ptr,
            ws_bytes, _stream())
     return out
 
@@ -871,11 +890,14 @@ def linear8(x, weight, bias=None, *, epilogue=L.EPI_NONE, dtype=None, out=None, 
     code = _FLOATS.get(dtype)
     if code is None:
         raise TypeError("linear8: dtype must be float32, float16 or bfloat16")
-    out = _like(out, "out", (M, N), dtype, x.device)
+    if out is None:
+        out, ldo = torch.empty((M, N), dtype=dtype, device=x.device), N
+    else:
+        ldo = _out(out, (M, N), dtype)
     ws_ptr, ws_bytes, _keep = _workspace(
         workspace, lambda: L.lib().cdx_linear_e4m3_workspace_size(M, N, K), x.device)
     L.call("cdx_linear_e4m3", M, N, K, x.data_ptr(), ldx, xcode, bq, ldb, bsc, ldsb, bcode,
-           out.data_ptr(), _rows(out, "out")[2], code, _vector(bias, N), epilogue, ws_ptr,
+           out.data_ptr(), ldo, code, _vector(bias, N), epilogue, ws_ptr,
            ws_bytes, _stream())
     return out
 
@@ -894,9 +916,12 @@ def activation8(z, act, *, alpha=0.01, scale_dtype=torch.float8_e8m0fnu, out=Non
     if scode is None:
         raise TypeError("activation8: scale_dtype must be float8_e8m0fnu or float32")
     rows, cols, ldz = _rows(z, "input")
-    y = _like(out, "out", z.shape, z.dtype, z.device)
+    if out is None:
+        y, ldy = _new_like(z), cols
+    else:
+        y, ldy = out, _out(out, z.shape, z.dtype)
     b, ld = _empty8(rows, cols, 1, scale_dtype, z.device)
-    L.call("cdx_activation_forward_e4m3", z.data_ptr(), ldz, y.data_ptr(), _rows(y, "out")[2],
+    L.call("cdx_activation_forward_e4m3", z.data_ptr(), ldz, y.data_ptr(), ldy,
            b.q.data_ptr(), ld, b.scale.data_ptr(), b.scale.shape[1], scode, rows, cols, code, act,
            alpha, _stream())
     return y, b
@@ -909,9 +934,12 @@ def activation_backward8(grad_out, z, act, *, alpha=0.01, out=None):
     if tuple(grad_out.shape) != (rows, cols):
         raise ValueError("activation_backward8: grad_out and input differ in shape")
     ldg = _rows(grad_out, "grad_out")[2]
-    out = _like(out, "out", grad_out.shape, grad_out.dtype, grad_out.device)
+    if out is None:
+        out, ldo = _new_like(grad_out), cols
+    else:
+        ldo = _out(out, grad_out.shape, grad_out.dtype)
     L.call("cdx_activation_backward_e4m3", grad_out.data_ptr(), ldg, q, ldq, s, lds, scode,
-           out.data_ptr(), _rows(out, "out")[2], rows, cols, code, act, alpha, _stream())
+           out.data_ptr(), ldo, rows, cols, code, act, alpha, _stream())
     return out
 
 

@@ -140,6 +140,71 @@ __device__ __forceinline__ void store_tile(const Params& p, int64_t m0, int64_t 
     }
 }
 
+// The same for a whole workgroup's BM x BN tile through LDS that is no longer read (the
+// upper half of its rows in `low`, the others in `high`), so that a wave stores whole rows:
+// a product of 4096 x 4096 x 256 takes 17 us, 25 with each lane's 8 bytes stored alone.
+// Row m's 4-element units lie at unit ^ 4 (m & 15): 16 rows are then on all banks.
+template <class T, int ACT, int BM, int BN, int NT, int FN, int FM>
+__device__ __forceinline__ void store_rows_act(const Params& p, uint8_t* low, uint8_t* high,
+                                               int64_t m0, int64_t n0, int wm0, int wn0,
+                                               const floatx4 (&acc)[FN][FM]) {
+    constexpr int UNIT = 4 * sizeof(T), UNITS = BN / 4, ROW = BN * sizeof(T);
+    constexpr int SWAP = UNITS / 4 - 1 < 15 ? UNITS / 4 - 1 : 15;
+    const int l16 = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
+    uint8_t* mine = wm0 < BM / 2 ? low + wm0 * ROW : high + (wm0 - BM / 2) * ROW;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < FN; ++i) {
+        const int64_t nn = n0 + wn0 + 16 * i + 4 * g;
+        float b[4] = {};
+        if (p.bias) load_n<4>(p.bias + nn, p.N - nn < 0 ? 0 : p.N - nn < 4 ? (int)(p.N - nn) : 4, b);
+        const int unit = (wn0 / 4 + 4 * i + g) ^ (4 * (l16 & SWAP));
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            float o[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) o[r] = act_fixed<ACT>(acc[i][j][r] + b[r]);
+            store_n<4>(reinterpret_cast<T*>(mine + (16 * j + l16) * ROW + unit * UNIT), 4, o);
+        }
+    }
+    __syncthreads();
+    constexpr int CHUNKS = ROW / 16, PER = 16 / sizeof(T);
+    const int c = threadIdx.x % CHUNKS, r0 = threadIdx.x / CHUNKS;
+    const int64_t n = n0 + c * PER;
+    T* out = static_cast<T*>(p.C) + m0 * p.ldc + n;
+    const int rows = p.M - m0 < BM ? (int)(p.M - m0) : BM;
+#pragma unroll 4
+    for (int row = r0; row < rows; row += NT / CHUNKS) {
+        const int chunk = UNIT == 16 ? c ^ (4 * (row & SWAP)) : c ^ (2 * (row & SWAP));
+        const u32x4 v = *reinterpret_cast<const u32x4*>((row < BM / 2 ? low : high) + row % (BM / 2) * ROW + chunk * 16);
+        T* dst = out + row * p.ldc;
+        if (n + PER <= p.N) {
+            store16(dst, v);
+        } else {
+            T e[PER];
+            __builtin_memcpy(e, &v, 16);
+#pragma unroll
+            for (int k = 0; k < PER; ++k)
+                if (n + k < p.N) dst[k] = e[k];
+        }
+    }
+}
+
+template <class T, int BM, int BN, int NT, int FN, int FM>
+__device__ __forceinline__ void store_rows(const Params& p, uint8_t* low, uint8_t* high, int64_t m0,
+                                           int64_t n0, int wm0, int wn0,
+                                           const floatx4 (&acc)[FN][FM]) {
+#define CDX_ROWS(ACT) store_rows_act<T, ACT, BM, BN, NT>(p, low, high, m0, n0, wm0, wn0, acc)
+    switch (p.epilogue) {
+        case CDX_EPI_RELU: CDX_ROWS(CDX_EPI_RELU); break;
+        case CDX_EPI_GELU: CDX_ROWS(CDX_EPI_GELU); break;
+        case CDX_EPI_SILU: CDX_ROWS(CDX_EPI_SILU); break;
+        case CDX_EPI_SIGMOID: CDX_ROWS(CDX_EPI_SIGMOID); break;
+        default: CDX_ROWS(CDX_EPI_NONE); break;
+    }
+#undef CDX_ROWS
+}
+
 // Operands of any alignment and any K, 64 x 64 tiles: four waves of 32 x 32,
 // each block of 128 staged through registers into LDS.  A row's 16-byte pieces
 // lie at piece ^ (row / 2 & 7), so that the 16 rows that lanes read together spread
@@ -214,7 +279,7 @@ void gemm8_any_kernel(Params p) {
 // buffers, one barrier a step.  LDS is filled in the order of the lanes, so that
 // the exchange of 16-byte pieces (piece ^ (row / 2 & 7); a lane takes pieces g and g + 4:
 // the 16 rows that the hardware reads at a time then lie on all 64 banks, where pieces 2 g
-// and 2 g + 1 under row & 7 took 87 us against 78 at 4096^3) is made on the side of the
+// and 2 g + 1 under row & 7 took a tenth more time at 4096^3) is made on the side of the
 // global addresses.  The scales of kPanel steps are laid out in LDS at once, the
 // ones that a lane wants in a step side by side: as bytes they are the
 // instruction's scale operand, which picks one byte of a register per 16 rows.
@@ -222,7 +287,7 @@ constexpr int64_t kMaxLd = 1 << 23;   // 256 rows within 32-bit offsets
 template <int MODE> constexpr int kPanel = MODE == kBytes ? 32 : 16;
 
 template <class T, int MODE, int BM, int BN, int WM, int WN>
-__global__ __launch_bounds__(64 * WM * WN)
+__global__ __launch_bounds__(64 * WM * WN, 2)   // (two waves a SIMD: 256 registers)
 void gemm8_tile_kernel(Params p) {
     constexpr int NT = 64 * WM * WN, ROWS = BM + BN, LOADS = ROWS * 8 / NT;
     constexpr int FM = BM / WM / 16, FN = BN / WN / 16, P = kPanel<MODE>;
@@ -294,15 +359,29 @@ void gemm8_tile_kernel(Params p) {
             }
             panel_b[k][i / P] = v;
         }
-        for (int i = tid; i < BM * P; i += NT) {
-            const int row = i / P, k = i % P;   // a row's scales lie side by side
-            const int64_t m = m0 + (row < rows_a ? row : rows_a - 1);
-            S v = 0;
-            if (kb + k < p.blocks) {
-                if constexpr (MODE == kBytes) v = static_cast<const uint8_t*>(p.sa)[m * p.ldsa + kb + k];
-                else v = load_scale(p.sa, m * p.ldsa + kb + k, p.a_e8m0);
-            }
-            panel[k][row / (16 * FM)][row % 16][row % (16 * FM) / 16] = v;
+        // a thread takes its row's next steps; lanes along the rows meet no bank twice
+        constexpr int PART = P / (NT / BM);
+        const int row = tid % BM, from = tid / BM * PART;
+        const int64_t at = (m0 + (row < rows_a ? row : rows_a - 1)) * p.ldsa;
+        auto keep = [&](int k, S v) { panel[from + k][row / (16 * FM)][row % 16][row % (16 * FM) / 16] = v; };
+        if constexpr (MODE == kBytes) {
+            static_assert(PART == 16, "one load");
+            const u32x4 v = load_codes(static_cast<const uint8_t*>(p.sa) + at, kb + from, p.blocks);
+#pragma unroll
+            for (int k = 0; k < PART; ++k) keep(k, (uint8_t)(v[k / 4] >> (8 * (k % 4))));
+        } else {
+            float v[PART];
+            auto take = [&](bool e8m0) {
+#pragma unroll
+                for (int k = 0; k < PART; ++k) {
+                    const int64_t b = kb + from + k;
+                    v[k] = load_scale(p.sa, at + (b < p.blocks ? b : p.blocks - 1), e8m0);
+                }
+            };
+            if (p.a_e8m0) take(true);
+            else take(false);
+#pragma unroll
+            for (int k = 0; k < PART; ++k) keep(k, v[k]);
         }
     };
     floatx4 acc[FN][FM] = {};
@@ -363,7 +442,7 @@ void gemm8_tile_kernel(Params p) {
             }
         }
     }
-    store_tile<T>(p, m0 + wm * (BM / WM), n0 + wn * (BN / WN), acc);
+    store_rows<T, BM, BN, NT>(p, lds[0], lds[1], m0, n0, wm * (BM / WM), wn * (BN / WN), acc);
 }
 
 // Few rows of A: operands from global memory straight into registers, a block's

@@ -140,18 +140,15 @@ __device__ __forceinline__ void store_tile(const Params& p, int64_t m0, int64_t 
     }
 }
 
-// The same for a whole workgroup's BM x BN tile through LDS that is no longer read (the
-// upper half of its rows in `low`, the others in `high`), so that a wave stores whole rows:
-// a product of 4096 x 4096 x 256 takes 17 us, 25 with each lane's 8 bytes stored alone.
+// The same for a whole workgroup's BM x BN tile through LDS (`buf`) that is no longer
+// read or written, so that a wave stores whole rows: a product of 4096 x 4096 x 256 takes 17 us, 25 with each lane's 8 bytes stored alone.
 // Row m's 4-element units lie at unit ^ 4 (m & 15): 16 rows are then on all banks.
 template <class T, int ACT, int BM, int BN, int NT, int FN, int FM>
-__device__ __forceinline__ void store_rows_act(const Params& p, uint8_t* low, uint8_t* high,
-                                               int64_t m0, int64_t n0, int wm0, int wn0,
-                                               const floatx4 (&acc)[FN][FM]) {
+__device__ __forceinline__ void store_rows_act(const Params& p, uint8_t* buf, int64_t m0, int64_t n0,
+                                               int wm0, int wn0, const floatx4 (&acc)[FN][FM]) {
     constexpr int UNIT = 4 * sizeof(T), UNITS = BN / 4, ROW = BN * sizeof(T);
     constexpr int SWAP = UNITS / 4 - 1 < 15 ? UNITS / 4 - 1 : 15;
     const int l16 = threadIdx.x & 15, g = (threadIdx.x >> 4) & 3;
-    uint8_t* mine = wm0 < BM / 2 ? low + wm0 * ROW : high + (wm0 - BM / 2) * ROW;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < FN; ++i) {
@@ -164,7 +161,7 @@ __device__ __forceinline__ void store_rows_act(const Params& p, uint8_t* low, ui
             float o[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) o[r] = act_fixed<ACT>(acc[i][j][r] + b[r]);
-            store_n<4>(reinterpret_cast<T*>(mine + (16 * j + l16) * ROW + unit * UNIT), 4, o);
+            store_n<4>(reinterpret_cast<T*>(buf + (wm0 + 16 * j + l16) * ROW + unit * UNIT), 4, o);
         }
     }
     __syncthreads();
@@ -176,7 +173,7 @@ __device__ __forceinline__ void store_rows_act(const Params& p, uint8_t* low, ui
 #pragma unroll 4
     for (int row = r0; row < rows; row += NT / CHUNKS) {
         const int chunk = UNIT == 16 ? c ^ (4 * (row & SWAP)) : c ^ (2 * (row & SWAP));
-        const u32x4 v = *reinterpret_cast<const u32x4*>((row < BM / 2 ? low : high) + row % (BM / 2) * ROW + chunk * 16);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(buf + row * ROW + chunk * 16);
         T* dst = out + row * p.ldc;
         if (n + PER <= p.N) {
             store16(dst, v);
@@ -191,10 +188,9 @@ __device__ __forceinline__ void store_rows_act(const Params& p, uint8_t* low, ui
 }
 
 template <class T, int BM, int BN, int NT, int FN, int FM>
-__device__ __forceinline__ void store_rows(const Params& p, uint8_t* low, uint8_t* high, int64_t m0,
-                                           int64_t n0, int wm0, int wn0,
-                                           const floatx4 (&acc)[FN][FM]) {
-#define CDX_ROWS(ACT) store_rows_act<T, ACT, BM, BN, NT>(p, low, high, m0, n0, wm0, wn0, acc)
+__device__ __forceinline__ void store_rows(const Params& p, uint8_t* buf, int64_t m0, int64_t n0,
+                                           int wm0, int wn0, const floatx4 (&acc)[FN][FM]) {
+#define CDX_ROWS(ACT) store_rows_act<T, ACT, BM, BN, NT>(p, buf, m0, n0, wm0, wn0, acc)
     switch (p.epilogue) {
         case CDX_EPI_RELU: CDX_ROWS(CDX_EPI_RELU); break;
         case CDX_EPI_GELU: CDX_ROWS(CDX_EPI_GELU); break;
@@ -284,16 +280,88 @@ void gemm8_any_kernel(Params p) {
 // ones that a lane wants in a step side by side: as bytes they are the
 // instruction's scale operand, which picks one byte of a register per 16 rows.
 constexpr int64_t kMaxLd = 1 << 23;   // 256 rows within 32-bit offsets
-template <int MODE> constexpr int kPanel = MODE == kBytes ? 32 : 16;
+template <int MODE> using Scale = std::conditional_t<MODE == kBytes, uint8_t, float>;
+template <int MODE> constexpr int kPart = MODE == kBytes ? 16 : 8;   // a thread's share of a panel
+
+// Offsets of a thread's 16-byte pieces (BM rows of A, then B's) from the tile's first row;
+// rows past the last one read it again, and what they give is not stored.
+template <int BM, int NT, int LOADS>
+__device__ __forceinline__ void row_offsets(const Params& p, int rows_a, int rows_b, uint32_t (&off)[LOADS]) {
+    const int tid = threadIdx.x, c16 = 16 * ((tid & 7) ^ ((tid >> 4) & 7));
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        const bool is_b = i * NT >= BM * 8;
+        const int row = (i * NT + tid) / 8 - (is_b ? BM : 0), rows = is_b ? rows_b : rows_a;
+        off[i] = (uint32_t)(row < rows ? row : rows - 1) * (uint32_t)(is_b ? p.ldb : p.lda) + c16;
+    }
+}
+
+// One block's rows into LDS: `a` and `b` are the addresses of the tile's first rows in it.
+template <int BM, int NT, int LOADS>
+__device__ __forceinline__ void rows_to_lds(uint64_t a, uint64_t b, const uint32_t (&off)[LOADS],
+                                            uint8_t* buf, int wave) {
+    typedef const __attribute__((address_space(1))) uint32_t* G;
+    typedef const __attribute__((address_space(1))) uint8_t* G8;
+    typedef __attribute__((address_space(3))) uint32_t* L;
+    // (kept apart from the offsets: scalar base + 32-bit offset, one VGPR a load)
+    asm("" : "+s"(a), "+s"(b));
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+        uint32_t o = off[i];
+        asm("" : "+v"(o));
+        __builtin_amdgcn_global_load_lds((G)((G8)(i * NT >= BM * 8 ? b : a) + o),
+                                         (L)(buf + (i * NT + wave * 64) * 16), 16, 0, 0);
+    }
+}
+
+// The scales of blocks kb .. kb + P - 1.  Of A a thread takes its row's next kPart: lanes
+// along the rows meet no bank twice (along the blocks they took 8 us a panel).
+template <int MODE, int BM, int BN, int NT, int WM, int FM, int P>
+__device__ __forceinline__ void scales_to_lds(const Params& p, int64_t m0, int64_t n0, int rows_a,
+                                              int64_t kb, Scale<MODE> (&panel)[P][WM][16][FM],
+                                              Scale<MODE> (&panel_b)[P][(BN + kBlock - 1) / kBlock]) {
+    constexpr int PART = kPart<MODE>;
+    const int tid = threadIdx.x;
+    for (int i = tid; i < P * ((BN + kBlock - 1) / kBlock); i += NT) {
+        const int k = i % P;
+        int64_t t = n0 / kBlock + i / P;
+        t = t < (p.N - 1) / kBlock ? t : (p.N - 1) / kBlock;
+        const int64_t at = t * p.ldsb + (kb + k < p.blocks ? kb + k : p.blocks - 1);
+        if constexpr (MODE == kBytes) panel_b[k][i / P] = static_cast<const uint8_t*>(p.sb)[at];
+        else panel_b[k][i / P] = load_scale(p.sb, at, p.b_e8m0);
+    }
+    const int row = tid % BM, from = tid / BM * PART;
+    const int64_t at = (m0 + (row < rows_a ? row : rows_a - 1)) * p.ldsa;
+    auto keep = [&](int k, Scale<MODE> v) { panel[from + k][row / (16 * FM)][row % 16][row % (16 * FM) / 16] = v; };
+    if constexpr (MODE == kBytes) {
+        const u32x4 v = load_codes(static_cast<const uint8_t*>(p.sa) + at, kb + from, p.blocks);
+#pragma unroll
+        for (int k = 0; k < PART; ++k) keep(k, (uint8_t)(v[k / 4] >> (8 * (k % 4))));
+    } else {
+        float v[PART];
+        auto take = [&](bool e8m0) {
+#pragma unroll
+            for (int k = 0; k < PART; ++k) {
+                const int64_t b = kb + from + k;
+                v[k] = load_scale(p.sa, at + (b < p.blocks ? b : p.blocks - 1), e8m0);
+            }
+        };
+        if (p.a_e8m0) take(true);
+        else take(false);
+#pragma unroll
+        for (int k = 0; k < PART; ++k) keep(k, v[k]);
+    }
+}
 
 template <class T, int MODE, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN, 2)   // (two waves a SIMD: 256 registers)
 void gemm8_tile_kernel(Params p) {
     constexpr int NT = 64 * WM * WN, ROWS = BM + BN, LOADS = ROWS * 8 / NT;
-    constexpr int FM = BM / WM / 16, FN = BN / WN / 16, P = kPanel<MODE>;
+    constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+    constexpr int P = kPart<MODE> * NT / BM;
     static_assert(ROWS * 8 % NT == 0 && BM * 8 % NT == 0, "whole rounds of loads");
     static_assert(FM % 4 == 0, "whole registers of scale bytes");
-    using S = std::conditional_t<MODE == kBytes, uint8_t, float>;
+    using S = Scale<MODE>;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[2][ROWS * 128];
     __shared__ __attribute__((aligned(16))) S panel[P][WM][16][FM];
     __shared__ S panel_b[P][BN / kBlock];
@@ -308,34 +376,15 @@ void gemm8_tile_kernel(Params p) {
     id -= first * tiles_n;
     const int64_t m0 = (first + id % high) * BM, n0 = id / high * BN;
 
-    // offsets from the tile's first row; rows past the last one read it again, and
-    // what they give is not stored
     const uint8_t* base_a = p.a + m0 * p.lda;
     const uint8_t* base_b = p.b + n0 * p.ldb;
     const int rows_a = p.M - m0 < BM ? (int)(p.M - m0) : BM, rows_b = p.N - n0 < BN ? (int)(p.N - n0) : BN;
     const int c16 = 16 * ((tid & 7) ^ ((tid >> 4) & 7));
     uint32_t off[LOADS];
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-        const bool is_b = i * NT >= BM * 8;
-        const int row = (i * NT + tid) / 8 - (is_b ? BM : 0), rows = is_b ? rows_b : rows_a;
-        off[i] = (uint32_t)(row < rows ? row : rows - 1) * (uint32_t)(is_b ? p.ldb : p.lda) + c16;
-    }
+    row_offsets<BM, NT>(p, rows_a, rows_b, off);
     const int64_t whole = p.K / kBlock;   // blocks without a ragged end
     auto fetch = [&](int64_t kb, int buf) {
-        typedef const __attribute__((address_space(1))) uint32_t* G;
-        typedef const __attribute__((address_space(1))) uint8_t* G8;
-        typedef __attribute__((address_space(3))) uint32_t* L;
-        // (kept apart from the offsets: scalar base + 32-bit offset, one VGPR a load)
-        uint64_t a = (uint64_t)(base_a + kb * kBlock), b = (uint64_t)(base_b + kb * kBlock);
-        asm("" : "+s"(a), "+s"(b));
-#pragma unroll
-        for (int i = 0; i < LOADS; ++i) {
-            uint32_t o = off[i];
-            asm("" : "+v"(o));
-            __builtin_amdgcn_global_load_lds((G)((G8)(i * NT >= BM * 8 ? b : a) + o),
-                                             (L)(&lds[buf][(i * NT + wave * 64) * 16]), 16, 0, 0);
-        }
+        rows_to_lds<BM, NT>((uint64_t)(base_a + kb * kBlock), (uint64_t)(base_b + kb * kBlock), off, lds[buf], wave);
     };
     auto fetch_end = [&](int64_t kb, int buf) {   // the last, ragged block: zeros past K
 #pragma unroll 1
@@ -347,42 +396,8 @@ void gemm8_tile_kernel(Params p) {
             *reinterpret_cast<u32x4*>(&lds[buf][(i * NT + tid) * 16]) = load_codes(s, kb * kBlock + c16, p.K);
         }
     };
-    auto fetch_panel = [&](int64_t kb) {   // the scales of steps kb .. kb + P - 1
-        for (int i = tid; i < P * (BN / kBlock); i += NT) {
-            const int k = i % P;
-            int64_t t = n0 / kBlock + i / P;
-            t = t < (p.N - 1) / kBlock ? t : (p.N - 1) / kBlock;
-            S v = 0;
-            if (kb + k < p.blocks) {
-                if constexpr (MODE == kBytes) v = static_cast<const uint8_t*>(p.sb)[t * p.ldsb + kb + k];
-                else v = load_scale(p.sb, t * p.ldsb + kb + k, p.b_e8m0);
-            }
-            panel_b[k][i / P] = v;
-        }
-        // a thread takes its row's next steps; lanes along the rows meet no bank twice
-        constexpr int PART = P / (NT / BM);
-        const int row = tid % BM, from = tid / BM * PART;
-        const int64_t at = (m0 + (row < rows_a ? row : rows_a - 1)) * p.ldsa;
-        auto keep = [&](int k, S v) { panel[from + k][row / (16 * FM)][row % 16][row % (16 * FM) / 16] = v; };
-        if constexpr (MODE == kBytes) {
-            static_assert(PART == 16, "one load");
-            const u32x4 v = load_codes(static_cast<const uint8_t*>(p.sa) + at, kb + from, p.blocks);
-#pragma unroll
-            for (int k = 0; k < PART; ++k) keep(k, (uint8_t)(v[k / 4] >> (8 * (k % 4))));
-        } else {
-            float v[PART];
-            auto take = [&](bool e8m0) {
-#pragma unroll
-                for (int k = 0; k < PART; ++k) {
-                    const int64_t b = kb + from + k;
-                    v[k] = load_scale(p.sa, at + (b < p.blocks ? b : p.blocks - 1), e8m0);
-                }
-            };
-            if (p.a_e8m0) take(true);
-            else take(false);
-#pragma unroll
-            for (int k = 0; k < PART; ++k) keep(k, v[k]);
-        }
+    auto fetch_panel = [&](int64_t kb) {
+        scales_to_lds<MODE, BM, BN, NT>(p, m0, n0, rows_a, kb, panel, panel_b);
     };
     floatx4 acc[FN][FM] = {};
     fetch(0, 0);
@@ -442,7 +457,103 @@ void gemm8_tile_kernel(Params p) {
             }
         }
     }
-    store_rows<T, BM, BN, NT>(p, lds[0], lds[1], m0, n0, wm * (BM / WM), wn * (BN / WN), acc);
+    store_rows<T, BM, BN, NT>(p, lds[0], m0, n0, wm * (BM / WM), wn * (BN / WN), acc);
+}
+
+// Few tiles and whole blocks: a CU has one workgroup or two, whose time is that of their
+// loads on their way.  64 x 64 tiles, four waves along B's rows, four LDS buffers: three
+// blocks are in flight.  Buffers of their own names tell the compiler that a block's reads
+// need not wait for the later blocks' loads.
+template <class T, int MODE>
+__global__ __launch_bounds__(256, 2)
+void gemm8_ring_kernel(Params p) {
+    constexpr int D = 4, NT = 256, SIDE = 64, LOADS = 2 * SIDE * 8 / NT, FM = SIDE / 16;
+    constexpr int P = kPart<MODE> * NT / SIDE, SIZE = 2 * SIDE * 128;
+    static_assert(P % D == 0, "whole rounds of buffers");
+    static_assert(SIZE >= SIDE * SIDE * (int)sizeof(T), "the results fit one buffer");
+    using S = Scale<MODE>;
+    __shared__ __attribute__((aligned(1024))) uint8_t r0[SIZE];
+    __shared__ __attribute__((aligned(1024))) uint8_t r1[SIZE];
+    __shared__ __attribute__((aligned(1024))) uint8_t r2[SIZE];
+    __shared__ __attribute__((aligned(1024))) uint8_t r3[SIZE];
+    __shared__ __attribute__((aligned(16))) S panel[P][1][16][FM];
+    __shared__ S panel_b[P][1];
+    const int tid = threadIdx.x, lane = tid & 63, l16 = tid & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int64_t tiles_m = ceil_div(p.M, (int64_t)SIDE);
+    const int64_t id = xcd_tile(blockIdx.x, tiles_m * ceil_div(p.N, (int64_t)SIDE));
+    const int64_t m0 = id % tiles_m * SIDE, n0 = id / tiles_m * SIDE;
+    const uint8_t* base_a = p.a + m0 * p.lda;
+    const uint8_t* base_b = p.b + n0 * p.ldb;
+    const int rows_a = p.M - m0 < SIDE ? (int)(p.M - m0) : SIDE;
+    const int rows_b = p.N - n0 < SIDE ? (int)(p.N - n0) : SIDE;
+    uint32_t off[LOADS];
+    row_offsets<SIDE, NT>(p, rows_a, rows_b, off);
+    auto fetch = [&](int64_t kb, uint8_t* buf) {
+        // (past the last block the last one again, which nobody reads: the waits count loads)
+        kb = kb < p.blocks ? kb : p.blocks - 1;
+        rows_to_lds<SIDE, NT>((uint64_t)(base_a + kb * kBlock), (uint64_t)(base_b + kb * kBlock), off, buf, wave);
+    };
+    floatx4 acc[1][FM] = {};
+    const int lo = (g ^ (l16 >> 1)) * 16, hi = lo ^ 64;   // pieces g and g + 4
+    const int xoff = l16 * 128, woff = (SIDE + 16 * wave + l16) * 128;
+    auto block = [&](const uint8_t* rows, int k) {
+        auto frag = [&](int o) {
+            Frag<MODE> f;
+            f.set(*reinterpret_cast<const u32x4*>(rows + o + lo), *reinterpret_cast<const u32x4*>(rows + o + hi));
+            return f;
+        };
+        const Frag<MODE> wq = frag(woff);
+        S sa[FM];
+        __builtin_memcpy(sa, panel[k][0][l16], sizeof(sa));
+        const S sb = panel_b[k][0];
+        Frag<MODE> xq[FM];
+#pragma unroll
+        for (int j = 0; j < FM; ++j) xq[j] = frag(xoff + j * 2048);
+        if constexpr (MODE == kBytes) {
+            int word;
+            __builtin_memcpy(&word, sa, sizeof(word));
+#define CDX_MFMA8(J) \
+    acc[0][J] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wq.q, xq[J].q, acc[0][J], 0, 0, 0, sb, J, word)
+            CDX_MFMA8(0);
+            CDX_MFMA8(1);
+            CDX_MFMA8(2);
+            CDX_MFMA8(3);
+#undef CDX_MFMA8
+        } else {
+#pragma unroll
+            for (int j = 0; j < FM; ++j) acc[0][j] = block_product<MODE>(wq, xq[j], acc[0][j], 0, 0, sa[j] * sb);
+        }
+    };
+    fetch(0, r0);
+    fetch(1, r1);
+    fetch(2, r2);
+    for (int64_t k0 = 0; k0 < p.blocks; k0 += P) {
+        const int count = p.blocks - k0 < P ? (int)(p.blocks - k0) : P;
+        __syncthreads();   // the last panel's readers are done
+        scales_to_lds<MODE, SIDE, SIDE, NT>(p, m0, n0, rows_a, k0, panel, panel_b);
+        auto step = [&](int k, const uint8_t* now, uint8_t* last) {
+            constexpr int N = (D - 2) * LOADS;
+            // vmcnt(N) lgkmcnt(0): this block's rows are in LDS, and the last block's are read
+            __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
+            asm volatile("s_barrier" ::: "memory");
+            fetch(k0 + k + D - 1, last);
+            block(now, k);
+        };
+#pragma unroll 1
+        for (int k = 0; k < count;) {
+            step(k, r0, r3);
+            if (++k == count) break;
+            step(k, r1, r0);
+            if (++k == count) break;
+            step(k, r2, r1);
+            if (++k == count) break;
+            step(k, r3, r2);
+            ++k;
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070);   // nothing is on its way to LDS
+    store_rows<T, SIDE, SIDE, NT>(p, r0, m0, n0, 0, 16 * wave, acc);
 }
 
 // Few rows of A: operands from global memory straight into registers, a block's
@@ -593,12 +704,26 @@ template <class T, class F> int with_mode(const Params& p, F f) {
     else return f(integral_constant<int, kFloats>{});
 }
 
-// The direct kernel's rows: all products of up to 64 rows, and those whose tiles of
-// 128 x 128 would leave most CUs without one.
+// Which kernel (us, scale bytes, bf16 results).
+// Straight from global memory: up to 32 rows (16 x 4096 x 4096 6.9, by the ring of buffers
+// 9.8), more while 128 x 128 tiles would be few and K is short (256 x 1024 x 1024 5.3, 5.6).
 bool is_direct(int64_t M, int64_t N) {
     return M <= 64 || ceil_div(M, (int64_t)128) * ceil_div(N, (int64_t)128) < 64;
 }
-// ... and those that quantise x as they read it: one tile of 16 rows.
+// The ring: 64 x 64 tiles up to two a CU.  64 x 1024 x 4096 9.8, straight from global memory
+// 14.7; 512 x 4096 x 4096 15.8, by 128 x 128 tiles 25.2; 300 x 8192 x 4096 (640 tiles)
+// 23.7 and 25.8 with scale bytes but 31.9 and 31.2 with floats, 46 and 45 for 32 bits.
+bool is_ring(int64_t M, int64_t N, int64_t K) {
+    return M > 32 && ceil_div(M, (int64_t)64) * ceil_div(N, (int64_t)64) <= 512 &&
+           (K >= 2048 || !is_direct(M, N));
+}
+// 256 x 256 tiles when they fill most of the CUs: 200 of them (2560 x 5120 x 1024) 23.1,
+// with 128 x 128 tiles 25.5; 128 of them (2048 x 4096 x 2048) 32.7 and 23.0.
+bool is_large(int64_t M, int64_t N) {
+    return ceil_div(M, (int64_t)256) * ceil_div(N, (int64_t)256) >= 200;
+}
+// One pass over x and the weights instead of two kernels: 16 rows (every workgroup
+// quantises all of x again).
 bool quantizes_inside(int64_t M) { return M <= 16; }
 
 template <class T, class X>
@@ -632,17 +757,24 @@ int run(const Params& p, hipStream_t stream) {
                            stream, p);
         return hip_error(hipGetLastError(), "gemm8_empty_kernel launch");
     }
-    if (is_direct(p.M, p.N)) return run_direct<T>(p, static_cast<const uint8_t*>(nullptr), (int64_t)0, stream);
     const int64_t big = ceil_div(p.M, (int64_t)256) * ceil_div(p.N, (int64_t)256);
     const int64_t mid = ceil_div(p.M, (int64_t)128) * ceil_div(p.N, (int64_t)128);
     const int64_t grid = ceil_div(p.M, (int64_t)64) * ceil_div(p.N, (int64_t)64);
     if (grid >= (int64_t)1 << 31) return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");
     const bool aligned = p.lda % 16 == 0 && p.ldb % 16 == 0 && ((uintptr_t)p.a | (uintptr_t)p.b) % 16 == 0 &&
                          p.K >= kBlock && p.lda <= kMaxLd && p.ldb <= kMaxLd;
+    if (aligned && p.K % kBlock == 0 && is_ring(p.M, p.N, p.K)) {
+        return with_mode<T>(p, [&](auto mode) {
+            hipLaunchKernelGGL((gemm8_ring_kernel<T, decltype(mode)::value>), dim3((unsigned)grid), dim3(256),
+                               0, stream, p);
+            return hip_error(hipGetLastError(), "gemm8_ring_kernel launch");
+        });
+    }
+    if (is_direct(p.M, p.N)) return run_direct<T>(p, static_cast<const uint8_t*>(nullptr), (int64_t)0, stream);
     return with_mode<T>(p, [&](auto mode) {
         constexpr int MODE = decltype(mode)::value;
         if constexpr (MODE != kWide) {
-            if (aligned && big >= 200) {
+            if (aligned && is_large(p.M, p.N)) {
                 hipLaunchKernelGGL((gemm8_tile_kernel<T, MODE, 256, 256, 2, 4>), dim3((unsigned)big),
                                    dim3(512), 0, stream, p);
                 return hip_error(hipGetLastError(), "gemm8_tile_kernel launch");

@@ -722,9 +722,10 @@ bool is_ring(int64_t M, int64_t N, int64_t K) {
 bool is_large(int64_t M, int64_t N) {
     return ceil_div(M, (int64_t)256) * ceil_div(N, (int64_t)256) >= 200;
 }
-// One pass over x and the weights instead of two kernels: 16 rows (every workgroup
-// quantises all of x again).
-bool quantizes_inside(int64_t M) { return M <= 16; }
+// x quantised by every workgroup for itself instead of by a kernel before: up to 16 rows of
+// 4096 (16 x 4096 x 4096 9.0 and 9.2, 8 x 4096 x 4096 7.8 and 8.3, 16 x 1024 x 1024 3.9 and
+// 5.6; 8 x 8192 x 8192 21.7 and 18.7, 1 x 8192 x 8192 19.0 and 16.5).
+bool quantizes_inside(int64_t M, int64_t K) { return M <= 16 && K <= 4096; }
 
 template <class T, class X>
 int run_direct(const Params& p, const X* x, int64_t ldx, hipStream_t stream) {
@@ -797,7 +798,7 @@ size_t codes_bytes(int64_t M, int64_t K) { return ((size_t)M * (size_t)codes_ld(
 
 size_t gemm8_workspace(int64_t M, int64_t N, int64_t K, bool from_x) {
     (void)N;
-    if (!from_x || M == 0 || K == 0 || quantizes_inside(M)) return 0;
+    if (!from_x || M == 0 || K == 0 || quantizes_inside(M, K)) return 0;
     return codes_bytes(M, K) + (size_t)M * (size_t)ceil_div(K, (int64_t)kBlock) * 4;
 }
 
@@ -805,7 +806,7 @@ int launch_gemm8(const Gemm8Args& g, hipStream_t stream) {
     const int64_t blocks = ceil_div(g.K, (int64_t)kBlock);
     Params p{g.a.q, g.b.q, g.a.s, g.b.s, g.M, g.N, g.K, g.a.ldq, g.b.ldq, g.a.lds, g.b.lds, g.ldc,
              blocks, g.a.e8m0, g.b.e8m0, g.C, g.bias, g.epilogue};
-    if (g.x && g.K > 0 && quantizes_inside(g.M)) {
+    if (g.x && g.K > 0 && quantizes_inside(g.M, g.K)) {
         p.a_e8m0 = p.b_e8m0;   // (the way of the same product from codes)
         return with_dtype(g.cdtype, [&](auto t) {
             return with_dtype(g.xdtype, [&](auto xt) {

@@ -333,12 +333,22 @@ int64_t tiles_of(int64_t N, int64_t K, int side) {
     return ceil_div(N, (int64_t)side) * (K > 0 ? ceil_div(K, (int64_t)side) : 1);
 }
 
+// Sides (us): 256 where 256 workgroups get a tile or 512 m and more each.  bf16, 256 and 128:
+// 8192 x 1024 x 4096 153 and 187, 4096 x 2048 x 1024 62 and 66, 256 x 4096 x 4096 28.6 and
+// 34.6; with 256 m each, 4096 x 1024 x 1024 47 and 40.  128 likewise where they get 192 m, or
+// two tiles: 128 and 64, 4096 x 256 x 784 fp32 22.9 and 25.9, 64 x 2048 x 4096 10.9 and
+// 12.1; with less 2048 x 256 x 784 fp32 20.5 and 16.6, 512 x 1024 x 1024 18.3 and 13.4.
+// Slices: one workgroup a CU of side 256, which fills LDS; two of the others (8192 x 256 x
+// 784 fp32 31.1, with one 33.7; 4096 x 768 x 768 bf16 28.9 and 31.2), but one slice of as
+// many tiles as CUs (1024 x 2048 x 2048 bf16 36.8, two 42.5).
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
     int side = 64;
-    if (tiles_of(N, K, 256) >= 128) side = 256;
-    else if (tiles_of(N, K, 128) >= 8 && M >= 256) side = 128;
+    const int64_t big = tiles_of(N, K, 256), mid = tiles_of(N, K, 128);
+    const int64_t m = M < 512 * 256 ? M : 512 * 256;   // (their products stay in 64 bits)
+    if (big >= 256 || big * m >= 512 * 256) side = 256;
+    else if (mid >= 512 || mid * m >= 192 * 256) side = 128;
     const int64_t tiles = tiles_of(N, K, side);
-    int64_t s = tiles < 256 ? 256 / tiles : 1;
+    int64_t s = tiles >= 256 ? 1 : (side == 256 ? 256 : 512) / tiles;
     if (s > M / 256) s = M / 256;
     if (s < 1) s = 1;
     const int64_t chunk = ceil_div(ceil_div(M, s), (int64_t)kMost) * kMost;

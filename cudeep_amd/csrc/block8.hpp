@@ -197,6 +197,33 @@ __device__ __forceinline__ float load_scale(const void* s, int64_t i, bool e8m0)
     return e8m0 ? e8m0_value(static_cast<const uint8_t*>(s)[i]) : static_cast<const float*>(s)[i];
 }
 
+// Activations on values of T: fp32 results with the accurate functions of the
+// elementwise kernels; results that are rounded to 16 bits with the hardware's
+// exponential and reciprocal (relative error 2^-22, below 2^-9 and 2^-12 by far;
+// with expf and divisions the GELU pair of 8-bit checkpoints is bound by them, not by memory).
+template <class T> __device__ __forceinline__ float fast_exp(float x) {
+    if constexpr (std::is_same_v<T, float>) return expf(x);
+    else return __builtin_amdgcn_exp2f(x * 1.44269504f);
+}
+template <class T> __device__ __forceinline__ float inverse(float x) {
+    if constexpr (std::is_same_v<T, float>) return 1.0f / x;
+    else return __builtin_amdgcn_rcpf(x);
+}
+
+template <class T, int ACT>
+__device__ __forceinline__ float act_value(float v, float alpha) {
+    if constexpr (ACT == CDX_EPI_RELU) return v > 0.0f ? v : 0.0f;
+    if constexpr (ACT == CDX_EPI_GELU) {
+        const float u = 0.7978845608f * (v + 0.044715f * v * v * v);
+        return v * inverse<T>(1.0f + fast_exp<T>(-2.0f * u));
+    }
+    if constexpr (ACT == CDX_EPI_SILU) return v * inverse<T>(1.0f + fast_exp<T>(-v));
+    if constexpr (ACT == CDX_EPI_SIGMOID) return inverse<T>(1.0f + fast_exp<T>(-v));
+    if constexpr (ACT == CDX_ACT_TANH) return tanhf(v);
+    if constexpr (ACT == CDX_ACT_LEAKY_RELU) return v > 0.0f ? v : alpha * v;
+    return v;
+}
+
 // Four values times `inv` (a power of two that brings them to at most 448 in
 // magnitude), rounded to nearest even; infinities become NaN first.
 __device__ __forceinline__ uint32_t pack_e4m3(float a, float b, float c, float d, float inv) {

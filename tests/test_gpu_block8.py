@@ -232,6 +232,44 @@ def test_product_of_whole_numbers(size, scale):
         assert torch.equal(ops.gemm8(a, b, dtype=dt).cpu(), exact.to(torch.float32).to(dt)), dt
 
 
+# more tiles, and blocks in a ring of buffers: fewer blocks than buffers, a panel of scales that ends
+# before the last block, ragged tiles and a ragged last block
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("scale", ["e8m0", "f32"])
+@pytest.mark.parametrize("size", [(1000, 1100, 128), (300, 4096, 256), (520, 2000, 384), (40, 70, 2048),
+                                  (129, 130, 2176), (33, 65, 4224), (70, 200, 8320), (1100, 2300, 512),
+                                  (1025, 2176, 2500), (3590, 3601, 300), (3601, 3590, 2432)])
+def test_product_by_many_tiles(size, scale, dtype):
+    import torch
+    ops = _ops()
+    M, N, K = size
+    a, b = _operands(M, N, K, scale, 7)
+    say("gemm8 tiles", size, scale, dtype)
+    got = ops.gemm8(a, b, dtype=_dtype(dtype))
+    _check_product(got, _values(a), _values(b), None, "none", K)
+    # operands and result inside larger ones
+    q = torch.zeros((M, K + 16), device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn)
+    q[:, :K] = a.q
+    out = torch.zeros((M, N + 3), device="cuda", dtype=_dtype(dtype))
+    ops.gemm8(ops.Block8(q[:, :K], a.scale), b, dtype=_dtype(dtype), out=out[:, 1:N + 1])
+    assert torch.equal(out[:, 1:N + 1], got) and not out[:, 0].any() and not out[:, N + 1:].any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu", "sigmoid"])
+@pytest.mark.parametrize("size", [(1, 333, 640), (40, 130, 2048), (300, 260, 250), (600, 2048, 300)])
+def test_epilogues_of_16_bits(size, act, dtype):
+    ops = _ops()
+    from cudeep_amd import _lib as L
+    M, N, K = size
+    epi = {"relu": L.EPI_RELU, "gelu": L.EPI_GELU, "silu": L.EPI_SILU, "sigmoid": L.EPI_SIGMOID}[act]
+    a, b = _operands(M, N, K, "e8m0", 3)
+    bias = _normal((1, N), 9)[0]
+    say("gemm8 epilogue", size, act, dtype)
+    got = ops.gemm8(a, b, bias=bias, epilogue=epi, dtype=_dtype(dtype))
+    _check_product(got, _values(a), _values(b), bias.double().cpu().numpy(), act, K)
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "silu", "sigmoid"])
 @pytest.mark.parametrize("size", [(1, 333, 640), (40, 130, 1000), (300, 260, 256), (600, 1024, 300)])
 def test_epilogues(size, act):

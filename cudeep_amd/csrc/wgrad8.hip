@@ -134,8 +134,13 @@ void wgrad8_kernel(Params p) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wn = wave % WN, wk = wave / WN;
     const int64_t tiles_n = ceil_div(p.N, (int64_t)BN);
-    const int64_t id = xcd_tile(blockIdx.x, gridDim.x);
-    const int64_t n0 = id % tiles_n * BN, k0 = id / tiles_n * BK;
+    // four tiles of n at a time, all of k: an XCD's tiles share more of dz (fp32 8192 x 4096 x
+    // 4096 592 us, one column of tiles after the other 631; bf16 262 and 261)
+    int64_t id = xcd_tile(blockIdx.x, gridDim.x);
+    const int64_t tiles_k = gridDim.x / tiles_n, first = id / (4 * tiles_k) * 4;
+    const int64_t wide = tiles_n - first < 4 ? tiles_n - first : 4;
+    id -= first * tiles_k;
+    const int64_t n0 = (first + id % wide) * BN, k0 = id / wide * BK;
     const int64_t m_begin = (int64_t)blockIdx.y * p.chunk;
     const int64_t m_end = m_begin + p.chunk < p.M ? m_begin + p.chunk : p.M;
     // a thread stages eight columns (zc, xc) of rows zr, zr + ZR, ... (xr, xr + XR, ...)
@@ -333,19 +338,20 @@ int64_t tiles_of(int64_t N, int64_t K, int side) {
     return ceil_div(N, (int64_t)side) * (K > 0 ? ceil_div(K, (int64_t)side) : 1);
 }
 
-// Sides (us): 256 where 256 workgroups get a tile or 512 m and more each.  bf16, 256 and 128:
-// 8192 x 1024 x 4096 153 and 187, 4096 x 2048 x 1024 62 and 66, 256 x 4096 x 4096 28.6 and
-// 34.6; with 256 m each, 4096 x 1024 x 1024 47 and 40.  128 likewise where they get 192 m, or
-// two tiles: 128 and 64, 4096 x 256 x 784 fp32 22.9 and 25.9, 64 x 2048 x 4096 10.9 and
-// 12.1; with less 2048 x 256 x 784 fp32 20.5 and 16.6, 512 x 1024 x 1024 18.3 and 13.4.
+// Sides (us, bf16 where nothing else is said): 256 where 256 workgroups get a tile or 1024 m
+// and more each.  256 and 128: 8192 x 1024 x 4096 98 and 123, 16384 x 1024 x 1024 65 and 67, 256
+// x 4096 x 4096 21.5 and 23.6; with 512 m each, 4096 x 2048 x 1024 47 and 42 (f16 62 and 66).
+// 128 likewise where they get 192 m, or two tiles: 128 and 64, 4096 x 256 x 784 20.5 and 19.6,
+// in fp32 22.9 and 25.9, 64 x 2048 x 4096 9.8 and 11.8; with less 2048 x 256 x 784 15.9 and
+// 12.9, 512 x 1024 x 1024 13.0 and 9.3.
 // Slices: one workgroup a CU of side 256, which fills LDS; two of the others (8192 x 256 x
-// 784 fp32 31.1, with one 33.7; 4096 x 768 x 768 bf16 28.9 and 31.2), but one slice of as
-// many tiles as CUs (1024 x 2048 x 2048 bf16 36.8, two 42.5).
+// 784 23.7, with one 25.6, in fp32 31.1 and 33.7; 4096 x 768 x 768 23.5 and 22.2, in f16 28.9
+// and 31.2), but one slice of as many tiles as CUs (1024 x 2048 x 2048 f16 36.8, two 42.5).
 Plan plan_of(int64_t M, int64_t N, int64_t K) {
     int side = 64;
     const int64_t big = tiles_of(N, K, 256), mid = tiles_of(N, K, 128);
-    const int64_t m = M < 512 * 256 ? M : 512 * 256;   // (their products stay in 64 bits)
-    if (big >= 256 || big * m >= 512 * 256) side = 256;
+    const int64_t m = M < 1024 * 256 ? M : 1024 * 256;   // (their products stay in 64 bits)
+    if (big >= 256 || big * m >= 1024 * 256) side = 256;
     else if (mid >= 512 || mid * m >= 192 * 256) side = 128;
     const int64_t tiles = tiles_of(N, K, side);
     int64_t s = tiles >= 256 ? 1 : (side == 256 ? 256 : 512) / tiles;

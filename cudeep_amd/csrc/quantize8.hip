@@ -1,5 +1,6 @@
 // Into and out of the 8-bit block-scaled format (block8.hpp), alone or with an
-// activation: all of them read and write each value once.
+// activation: all of them read and write each value once, by the thread that read it (an activation's
+// result may take the place of its input, a gradient's that of the other: no __restrict__ there).
 //
 // Rows: the 16 lanes of a DPP row take the 128 columns of a block, eight values
 // each (one 16-byte load of 16-bit values), so a block's largest magnitude is
@@ -101,9 +102,8 @@ __device__ __forceinline__ void row_of(const Pieces& p, int64_t i, int64_t& row,
 
 template <class T, int ACT, bool E8M0>
 __global__ __launch_bounds__(256)
-void quantize_rows_kernel(Pieces p, const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q,
-                          int64_t ldq, void* __restrict__ s, int64_t lds, T* __restrict__ y,
-                          int64_t ldy, float alpha) {
+void quantize_rows_kernel(Pieces p, const T* x, int64_t ldx, uint8_t* __restrict__ q, int64_t ldq,
+                          void* __restrict__ s, int64_t lds, T* y, int64_t ldy, float alpha) {
     const int lane = threadIdx.x & 15;
     for (int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); i < p.count;
          i += (int64_t)gridDim.x * 16) {
@@ -195,8 +195,8 @@ void quantize_tiles_kernel(const T* __restrict__ x, int64_t ldx, int64_t rows, i
 // out = q * s, or grad * act'(q * s).
 template <class T, int ACT, bool BWD>
 __global__ __launch_bounds__(256)
-void dequantize_kernel(Pieces p, Mat8 a, int tile_shift, const T* __restrict__ grad, int64_t ldg,
-                       T* __restrict__ out, int64_t ldo, float alpha) {
+void dequantize_kernel(Pieces p, Mat8 a, int tile_shift, const T* grad, int64_t ldg, T* out,
+                       int64_t ldo, float alpha) {
     const int lane = threadIdx.x & 15;
     for (int64_t i = (int64_t)blockIdx.x * 16 + (threadIdx.x >> 4); i < p.count;
          i += (int64_t)gridDim.x * 16) {

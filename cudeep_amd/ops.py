@@ -674,7 +674,8 @@ def _param(p, name, dim, dtype):
 def layer_norm(x, weight=None, bias=None, eps=1e-5, *, stats=False, out=None):
     """Layer norm over the last dimension of a float32, float16 or bfloat16 tensor (2-D: any
     row stride); sums in float32.  weight and bias are of x's type or float32 (both the
-    same).  With stats, (y, mean, rstd), float32 [rows], as layer_norm_backward takes them."""
+    same).  With stats, (y, mean, rstd), float32 [rows], as layer_norm_backward takes them.  `out`
+    may be x itself."""
     code = _float_code(x, "input")
     rows, dim, ldx = _rows(x, "input")
     if dim < 1:
@@ -708,8 +709,8 @@ def layer_norm_backward(grad_out, x, mean, rstd, weight=None, *, params=True, pa
                         out=None, workspace=None):
     """(grad of x, of weight, of bias) of layer_norm, from the statistics it returned.  The
     parameters' gradients are of `param_dtype` (weight's type, else x's), None each without
-    `params`.  `workspace` (layer_norm_backward_workspace_bytes) makes the call
-    allocation-free."""
+    `params`.  `out` (x's gradient) may be x or grad_out itself.  `workspace`
+    (layer_norm_backward_workspace_bytes) makes the call allocation-free."""
     code = _float_code(x, "input")
     _need(grad_out, "grad_out", x.dtype)
     if grad_out.shape != x.shape:
@@ -908,7 +909,7 @@ def linear8_workspace_bytes(M: int, N: int, K: int) -> int:
 
 def activation8(z, act, *, alpha=0.01, scale_dtype=torch.float8_e8m0fnu, out=None):
     """(act(z), z as a Block8) in one pass over z [rows, cols]: what the backward pass keeps of
-    an activation's input.  act as for `activation`."""
+    an activation's input.  act as for `activation`; `out` may be z itself."""
     code = _float_code(z, "input")
     if z.dim() != 2:
         raise ValueError("activation8: input must be 2-D")
@@ -928,7 +929,7 @@ def activation8(z, act, *, alpha=0.01, scale_dtype=torch.float8_e8m0fnu, out=Non
 
 
 def activation_backward8(grad_out, z, act, *, alpha=0.01, out=None):
-    """grad_out * act'(z) with z a Block8 (tile_rows 1)."""
+    """grad_out * act'(z) with z a Block8 (tile_rows 1); `out` may be grad_out itself."""
     code = _float_code(grad_out, "grad_out")
     rows, cols, q, ldq, s, lds, scode = _block8(z, "input", 1)
     if tuple(grad_out.shape) != (rows, cols):

@@ -499,8 +499,9 @@ int cdx_activation_backward_f64(const double* grad_output, const double* input,
  * matrix, mu = mean(x), r = 1 / sqrt(mean((x - mu)^2) + eps); sums in fp32.
  * dtype (x, y): CDX_DTYPE_F32, _F16 or _BF16; param_dtype (weight, bias): dtype
  * or CDX_DTYPE_F32.  weight and bias may be NULL (1 and 0); mean and rstd (fp32,
- * one per row, what the backward pass reads) may be NULL.  No counterpart in
- * the reference's dense path. */
+ * one per row, what the backward pass reads) may be NULL.  y may be x itself
+ * (the same pointer and leading dimension; other overlaps are not allowed).  No
+ * counterpart in the reference's dense path. */
 int cdx_layer_norm_forward(const void* x, int64_t ldx, const void* weight, const void* bias,
                            void* y, int64_t ldy, float* mean, float* rstd,
                            int64_t rows, int64_t dim, double eps, int dtype, int param_dtype,
@@ -510,7 +511,8 @@ int cdx_layer_norm_forward(const void* x, int64_t ldx, const void* weight, const
  *   grad_in = r (g - mean(g) - xh mean(g xh)),
  *   grad_weight = sum over rows of grad_out xh, grad_bias = sum of grad_out.
  * grad_weight and grad_bias (param_dtype, dense [dim]; overwritten) may be NULL;
- * weight may be NULL.  The row sums go through per-workgroup partials added in a
+ * weight may be NULL.  grad_in may be x or grad_out itself (the same pointer and
+ * leading dimension).  The row sums go through per-workgroup partials added in a
  * fixed order: the same bits every time.  workspace: the query's bytes (0 where
  * neither is wanted); NULL allocates stream-ordered. */
 size_t cdx_layer_norm_backward_workspace_size(int64_t rows, int64_t dim, int dtype);
@@ -566,12 +568,14 @@ int cdx_linear_e4m3(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
 
 /* y = act(z), and z in 8 bits (tile_rows 1) for the backward pass, in one pass over
  * z.  act: CDX_EPI_RELU to _SIGMOID, CDX_ACT_TANH or CDX_ACT_LEAKY_RELU (alpha: its
- * slope).  16-bit results use the hardware's exponential and reciprocal. */
+ * slope).  16-bit results use the hardware's exponential and reciprocal.  y may be
+ * z itself (the same pointer and leading dimension). */
 int cdx_activation_forward_e4m3(const void* z, int64_t ldz, void* y, int64_t ldy,
                                 void* q, int64_t ldq, void* scale, int64_t lds, int scale_dtype,
                                 int64_t rows, int64_t cols, int dtype, int act, float alpha,
                                 hipStream_t stream);
-/* grad_in = grad_out * act'(z), z restored from its 8 bits. */
+/* grad_in = grad_out * act'(z), z restored from its 8 bits; grad_in may be grad_out
+ * itself. */
 int cdx_activation_backward_e4m3(const void* grad_out, int64_t ldg, const void* q, int64_t ldq,
                                  const void* scale, int64_t lds, int scale_dtype,
                                  void* grad_in, int64_t ldgi, int64_t rows, int64_t cols,

@@ -36,6 +36,15 @@ template <class T> __device__ __forceinline__ void logistic(float x, float& s, f
     }
 }
 
+// v as a factor of s r.  In both tails s r is 0 and a slope is s itself, but v v overflows from
+// 1.8e19 on (and v is infinite where its 8 bits round to 2^128), and 0 times infinity is no slope:
+// 0 there, or for 16 bits, bound by their instructions, v within 2^30.  8192 x 4096 with GELU: fp32
+// 74.5 us, clamped 78.5; bf16 30.3, chosen by s r > 0 32.5.
+template <class T> __device__ __forceinline__ float beside(float v, float sr) {
+    if constexpr (std::is_same_v<T, float>) return sr > 0.0f ? v : 0.0f;
+    else return __builtin_amdgcn_fmed3f(v, -0x1p30f, 0x1p30f);
+}
+
 // grad * act'(v).
 template <class T, int ACT>
 __device__ __forceinline__ float act_slope(float g, float v, float alpha) {
@@ -43,13 +52,14 @@ __device__ __forceinline__ float act_slope(float g, float v, float alpha) {
     if constexpr (ACT == CDX_ACT_LEAKY_RELU) return v > 0.0f ? g : alpha * g;
     float s, r;
     if constexpr (ACT == CDX_EPI_GELU) {
-        logistic<T>(2.0f * 0.7978845608f * (v + 0.044715f * v * v * v), s, r);
-        const float du = 0.7978845608f * (1.0f + 3.0f * 0.044715f * v * v);
-        return g * (s + 2.0f * v * s * r * du);
+        constexpr float c = 0.7978845608f, k = 0.044715f;
+        logistic<T>(2.0f * c * (v + k * v * v * v), s, r);
+        const float n = beside<T>(v, s * r);   // slope s + 2 v s r du, du = c (1 + 3 k v v)
+        return g * (s + n * (s * r) * (2.0f * c + 6.0f * c * k * (n * n)));
     }
     if constexpr (ACT == CDX_EPI_SILU) {
         logistic<T>(v, s, r);
-        return g * (s + v * s * r);
+        return g * (s + beside<T>(v, s * r) * (s * r));
     }
     if constexpr (ACT == CDX_EPI_SIGMOID) {
         logistic<T>(v, s, r);

@@ -853,7 +853,10 @@ def _vector(bias, n, name="bias"):
 def gemm8(a, b, *, bias=None, epilogue=L.EPI_NONE, dtype=torch.bfloat16, out=None,
           workspace=None):
     """C = epi(A B^T + bias) of two Block8 matrices, A [M, K] with tile_rows 1 and B [N, K] (a
-    Linear layer's weight) with tile_rows 128; float32 sums, C of `dtype`, bias float32."""
+    Linear layer's weight) with tile_rows 128; C of `dtype`, bias float32.  Products are exact.  A
+    float32 result has float32 sums; a 16-bit one, at twice the rate, loses up to 2^-10 of the
+    largest of each eight products (consecutive k) before the float32 sums: usually far below its
+    own rounding, more where sums cancel."""
     M, K, aq, lda, asc, ldsa, acode = _block8(a, "A", 1)
     N, K2, bq, ldb, bsc, ldsb, bcode = _block8(b, "B", _BLOCK)
     if K != K2:
@@ -879,7 +882,8 @@ def gemm8_workspace_bytes(M: int, N: int, K: int) -> int:
 
 def linear8(x, weight, bias=None, *, epilogue=L.EPI_NONE, dtype=None, out=None, workspace=None):
     """epi(x W^T + bias) with W a Block8 [N, K] (tile_rows 128) and x [M, K] quantised on the way
-    in as quantize8(x) does; the result is of `dtype` (x's own by default)."""
+    in as quantize8(x) does; the result is of `dtype` (x's own by default), which also decides
+    how sums are formed, as for gemm8."""
     xcode = _float_code(x, "input")
     if x.dim() != 2:
         raise ValueError("linear8: input must be 2-D")

@@ -40,6 +40,33 @@ int check_matrix(const char* fn, const char* name, const void* p, int64_t ld, in
     return CDX_OK;
 }
 
+// A checked row-major matrix as the bytes of its rows.
+struct Span {
+    uintptr_t at; int64_t pitch, width, rows;
+    Span(const void* p, int64_t ld, int64_t rows_, int64_t cols, int dtype)
+        : at((uintptr_t)p), pitch(ld * size(dtype)), width(cols * size(dtype)), rows(rows_) {}
+    static int64_t size(int dtype) { return dtype == CDX_DTYPE_F32 ? 4 : 2; }
+    uintptr_t end() const { return at + (uintptr_t)((rows - 1) * pitch + width); }
+    bool same(const Span& o) const { return at == o.at && (pitch == o.pitch || rows == 1); }
+};
+
+// Whether two of them share a byte.  Columns of one wider matrix that lie beside each other do not;
+// rows of different pitches that mesh are taken to.
+bool overlap(const Span& a, const Span& b) {
+    if (a.rows == 0 || a.width == 0 || b.rows == 0 || b.width == 0) return false;
+    if (a.end() <= b.at || b.end() <= a.at) return false;
+    if (a.pitch != b.pitch) return true;
+    const int64_t off = b.at >= a.at ? (int64_t)((b.at - a.at) % (uintptr_t)a.pitch)
+                                     : a.pitch - 1 - (int64_t)((a.at - b.at - 1) % (uintptr_t)a.pitch);
+    return !(off >= a.width && off + b.width <= a.pitch);
+}
+
+// A row operator's result: its input's own place, or apart from it (workgroups take rows in any order).
+int check_in_place(const char* fn, const char* what, const Span& out, const Span& in) {
+    if (out.same(in) || !overlap(out, in)) return CDX_OK;
+    return bad(fn, (std::string(what) + " overlap without being the same").c_str());
+}
+
 // An 8-bit matrix argument.
 int check_mat8(const char* fn, const char* name, const void* q, int64_t ldq, const void* s,
                int64_t lds, int scale_dtype, int tile_rows, int64_t rows, int64_t cols) {
@@ -103,6 +130,7 @@ int cdx_layer_norm_forward(const void* x, int64_t ldx, const void* weight, const
     int st = check_norm(fn, rows, dim, dtype, param_dtype);
     if (!st) st = check_matrix(fn, "x", x, ldx, rows, dim);
     if (!st) st = check_matrix(fn, "y", y, ldy, rows, dim);
+    if (!st) st = check_in_place(fn, "y and x", {y, ldy, rows, dim, dtype}, {x, ldx, rows, dim, dtype});
     if (st) return st;
     if (!(eps >= 0.0) || !std::isfinite(eps)) return bad(fn, "eps must be finite and not negative");
     if (rows == 0) return CDX_OK;
@@ -125,6 +153,9 @@ int cdx_layer_norm_backward(const void* grad_out, int64_t ldg, const void* x, in
     if (!st) st = check_matrix(fn, "grad_out", grad_out, ldg, rows, dim);
     if (!st) st = check_matrix(fn, "x", x, ldx, rows, dim);
     if (!st) st = check_matrix(fn, "grad_in", grad_in, ldgi, rows, dim);
+    const Span in{grad_in, ldgi, rows, dim, dtype};
+    if (!st) st = check_in_place(fn, "grad_in and x", in, {x, ldx, rows, dim, dtype});
+    if (!st) st = check_in_place(fn, "grad_in and grad_out", in, {grad_out, ldg, rows, dim, dtype});
     if (st) return st;
     if (rows == 0) {   // empty sums
         if (grad_weight) st = cdx::launch_zero(grad_weight, dim, param_dtype, stream);
@@ -214,7 +245,11 @@ int cdx_linear_e4m3(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
     cdx::Gemm8Args g{M, N, K, {}, mat8(B, ldb, b_scale, ldsb, b_scale_dtype)};
     g.x = x; g.ldx = ldx; g.xdtype = x_dtype;
     g.C = C; g.ldc = ldc; g.cdtype = c_dtype; g.bias = bias; g.epilogue = epilogue;
-    return with_workspace(fn, cdx_linear_e4m3_workspace_size(M, N, K), workspace, workspace_bytes,
+    const size_t need = cdx_linear_e4m3_workspace_size(M, N, K);
+    const bool small = workspace && workspace_bytes < need;
+    // (few rows: every workgroup reads all of x while others already write C)
+    if (!small && overlap({C, ldc, M, N, c_dtype}, {x, ldx, M, K, x_dtype})) return bad(fn, "C overlaps x");
+    return with_workspace(fn, need, workspace, workspace_bytes,
                           stream, [&](void* ws) {
                               g.ws = ws;
                               return cdx::launch_gemm8(g, stream);
@@ -232,6 +267,7 @@ int cdx_activation_forward_e4m3(const void* z, int64_t ldz, void* y, int64_t ldy
     int st = check_matrix(fn, "z", z, ldz, rows, cols);
     if (!st) st = check_matrix(fn, "y", y, ldy, rows, cols);
     if (!st) st = check_mat8(fn, "q", q, ldq, scale, lds, scale_dtype, 1, rows, cols);
+    if (!st) st = check_in_place(fn, "y and z", {y, ldy, rows, cols, dtype}, {z, ldz, rows, cols, dtype});
     if (st || rows == 0 || cols == 0) return st;
     return cdx::launch_quantize_rows(z, ldz, rows, cols, dtype, static_cast<uint8_t*>(q), ldq, scale,
                                      lds, scale_dtype == CDX_DTYPE_E8M0, y, ldy, act, alpha, stream);
@@ -248,6 +284,8 @@ int cdx_activation_backward_e4m3(const void* grad_out, int64_t ldg, const void* 
     int st = check_matrix(fn, "grad_out", grad_out, ldg, rows, cols);
     if (!st) st = check_matrix(fn, "grad_in", grad_in, ldgi, rows, cols);
     if (!st) st = check_mat8(fn, "q", q, ldq, scale, lds, scale_dtype, 1, rows, cols);
+    if (!st) st = check_in_place(fn, "grad_in and grad_out", {grad_in, ldgi, rows, cols, dtype},
+                                 {grad_out, ldg, rows, cols, dtype});
     if (st || rows == 0 || cols == 0) return st;
     return cdx::launch_activation_backward8(grad_out, ldg, mat8(q, ldq, scale, lds, scale_dtype),
                                             rows, cols, grad_in, ldgi, dtype, act, alpha, stream);

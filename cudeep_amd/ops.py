@@ -883,7 +883,7 @@ def gemm8_workspace_bytes(M: int, N: int, K: int) -> int:
 def linear8(x, weight, bias=None, *, epilogue=L.EPI_NONE, dtype=None, out=None, workspace=None):
     """epi(x W^T + bias) with W a Block8 [N, K] (tile_rows 128) and x [M, K] quantised on the way
     in as quantize8(x) does; the result is of `dtype` (x's own by default), which also decides
-    how sums are formed, as for gemm8."""
+    how sums are formed, as for gemm8.  `out` must not overlap x."""
     xcode = _float_code(x, "input")
     if x.dim() != 2:
         raise ValueError("linear8: input must be 2-D")

@@ -500,7 +500,7 @@ int cdx_activation_backward_f64(const double* grad_output, const double* input,
  * dtype (x, y): CDX_DTYPE_F32, _F16 or _BF16; param_dtype (weight, bias): dtype
  * or CDX_DTYPE_F32.  weight and bias may be NULL (1 and 0); mean and rstd (fp32,
  * one per row, what the backward pass reads) may be NULL.  y may be x itself
- * (the same pointer and leading dimension; other overlaps are not allowed).  No
+ * (the same pointer and leading dimension; other overlaps are refused).  No
  * counterpart in the reference's dense path. */
 int cdx_layer_norm_forward(const void* x, int64_t ldx, const void* weight, const void* bias,
                            void* y, int64_t ldy, float* mean, float* rstd,
@@ -564,7 +564,8 @@ int cdx_gemm_e4m3(int64_t M, int64_t N, int64_t K,
                   void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /* The same with A given as x [M,K] in x_dtype: quantised by row as
- * cdx_quantize_e4m3 does, then multiplied (sums as above, by c_dtype). */
+ * cdx_quantize_e4m3 does, then multiplied (sums as above, by c_dtype).  C must not
+ * overlap x. */
 size_t cdx_linear_e4m3_workspace_size(int64_t M, int64_t N, int64_t K);
 int cdx_linear_e4m3(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, int x_dtype,
                     const void* B, int64_t ldb, const void* b_scale, int64_t ldsb,

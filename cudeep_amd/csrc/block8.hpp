@@ -305,11 +305,15 @@ struct Gemm8Args {
 };
 size_t gemm8_workspace(int64_t M, int64_t N, int64_t K, bool from_x);
 int launch_gemm8(const Gemm8Args& g, hipStream_t stream);
+// The kernel it runs: aligned operands or not, 32-bit results (wide) or 16-bit ones.
+const char* gemm8_kernel_name(int64_t M, int64_t N, int64_t K, bool aligned, bool wide, bool from_x);
 
 // dw[N,K] = dz[M,N]^T * (q * s)[M,K], db[n] = sum_m dz[m,n] (wgrad8.hip; db may be
 // null).  ws: wgrad8_workspace(...) bytes.
 size_t wgrad8_workspace(int64_t M, int64_t N, int64_t K, int dtype, bool bias);
 int launch_wgrad8(const void* dz, int64_t lddz, int dtype, const b8::Mat8& x, float* dw, float* db,
                   int64_t M, int64_t N, int64_t K, void* ws, hipStream_t stream);
+// The side of its tiles and the number of slices of m.
+void wgrad8_plan(int64_t M, int64_t N, int64_t K, int* side, int* slices);
 
 }  // namespace cdx

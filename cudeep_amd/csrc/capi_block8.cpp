@@ -325,3 +325,16 @@ int cdx_linear_weight_grad_e4m3(const void* dz, int64_t lddz, int dtype, const v
 }
 
 }  // extern "C"
+
+// Internal: the kernel of cdx_gemm_e4m3, or with from_x of cdx_linear_e4m3 (`aligned`: rows of the
+// 8-bit operands begin at 16-byte addresses), and the plan of
+// cdx_linear_weight_grad_e4m3 as 1000 * (side of its tiles) + slices of the batch.
+extern "C" const char* cdxi_gemm8_kernel(int from_x, int c_dtype, int64_t M, int64_t N, int64_t K,
+                                         int aligned) {
+    return cdx::gemm8_kernel_name(M, N, K, aligned, c_dtype == CDX_DTYPE_F32, from_x);
+}
+extern "C" int cdxi_wgrad8_plan(int64_t M, int64_t N, int64_t K) {
+    int side = 0, slices = 0;
+    cdx::wgrad8_plan(M, N, K, &side, &slices);
+    return 1000 * side + slices;
+}

@@ -820,6 +820,18 @@ bool quantizes_inside(int64_t M, int64_t K) {
     return M <= 64 && K <= 4096 && M * K <= (M <= 16 ? 65536 : 49152);
 }
 
+// The kernel of a product; `aligned`: rows of both operands begin at 16-byte addresses; `wide`:
+// 32-bit results.
+enum class Kernel { Empty, Direct, Ring, Tile128, Tile256, Any };
+Kernel kernel_of(int64_t M, int64_t N, int64_t K, bool aligned, bool wide) {
+    if (K == 0) return Kernel::Empty;
+    aligned = aligned && K >= kBlock;
+    if (aligned && is_ring(M, N, K)) return Kernel::Ring;
+    if (is_direct(M, N)) return Kernel::Direct;
+    if (!aligned) return Kernel::Any;
+    return !wide && is_large(M, N) ? Kernel::Tile256 : Kernel::Tile128;
+}
+
 template <class T, class X>
 int run_direct(const Params& p, const X* x, int64_t ldx, hipStream_t stream) {
     return with_mode<T>(p, [&](auto mode) {
@@ -841,7 +853,10 @@ int run_direct(const Params& p, const X* x, int64_t ldx, hipStream_t stream) {
 
 template <class T>
 int run(const Params& p, hipStream_t stream) {
-    if (p.K == 0) {
+    const bool aligned = p.lda % 16 == 0 && p.ldb % 16 == 0 && ((uintptr_t)p.a | (uintptr_t)p.b) % 16 == 0 &&
+                         p.lda <= kMaxLd && p.ldb <= kMaxLd;
+    const Kernel kernel = kernel_of(p.M, p.N, p.K, aligned, std::is_same_v<T, float>);
+    if (kernel == Kernel::Empty) {
         const int64_t g = ceil_div(p.M, (int64_t)16) * ceil_div(p.N, (int64_t)16);
         hipLaunchKernelGGL(gemm8_empty_kernel<T>, dim3((unsigned)(g < 65536 ? g : 65536)), dim3(64), 0,
                            stream, p);
@@ -851,26 +866,24 @@ int run(const Params& p, hipStream_t stream) {
     const int64_t mid = ceil_div(p.M, (int64_t)128) * ceil_div(p.N, (int64_t)128);
     const int64_t grid = ceil_div(p.M, (int64_t)64) * ceil_div(p.N, (int64_t)64);
     if (grid >= (int64_t)1 << 31) return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");
-    const bool aligned = p.lda % 16 == 0 && p.ldb % 16 == 0 && ((uintptr_t)p.a | (uintptr_t)p.b) % 16 == 0 &&
-                         p.K >= kBlock && p.lda <= kMaxLd && p.ldb <= kMaxLd;
-    if (aligned && is_ring(p.M, p.N, p.K)) {
+    if (kernel == Kernel::Ring) {
         return with_mode<T>(p, [&](auto mode) {
             hipLaunchKernelGGL((gemm8_ring_kernel<T, decltype(mode)::value>), dim3((unsigned)grid), dim3(256),
                                0, stream, p);
             return hip_error(hipGetLastError(), "gemm8_ring_kernel launch");
         });
     }
-    if (is_direct(p.M, p.N)) return run_direct<T>(p, static_cast<const uint8_t*>(nullptr), (int64_t)0, stream);
+    if (kernel == Kernel::Direct) return run_direct<T>(p, static_cast<const uint8_t*>(nullptr), (int64_t)0, stream);
     return with_mode<T>(p, [&](auto mode) {
         constexpr int MODE = decltype(mode)::value;
         if constexpr (MODE != kWide) {
-            if (aligned && is_large(p.M, p.N)) {
+            if (kernel == Kernel::Tile256) {
                 hipLaunchKernelGGL((gemm8_tile_kernel<T, MODE, 256, 256, 2, 4>), dim3((unsigned)big),
                                    dim3(512), 0, stream, p);
                 return hip_error(hipGetLastError(), "gemm8_tile_kernel launch");
             }
         }
-        if (aligned)
+        if (kernel == Kernel::Tile128)
             hipLaunchKernelGGL((gemm8_tile_kernel<T, MODE, 128, 128, 2, 2>), dim3((unsigned)mid),
                                dim3(256), 0, stream, p);
         else
@@ -889,6 +902,12 @@ size_t gemm8_workspace(int64_t M, int64_t N, int64_t K, bool from_x) {
     (void)N;
     if (!from_x || M == 0 || K == 0 || quantizes_inside(M, K)) return 0;
     return codes_bytes(M, K) + (size_t)M * (size_t)ceil_div(K, (int64_t)kBlock) * 4;
+}
+
+const char* gemm8_kernel_name(int64_t M, int64_t N, int64_t K, bool aligned, bool wide, bool from_x) {
+    if (from_x && K > 0 && quantizes_inside(M, K)) return "direct, quantises";
+    static const char* const names[] = {"empty", "direct", "ring", "tile 128", "tile 256", "any"};
+    return names[(int)kernel_of(M, N, K, aligned, wide)];
 }
 
 int launch_gemm8(const Gemm8Args& g, hipStream_t stream) {

@@ -387,6 +387,12 @@ size_t wgrad8_workspace(int64_t M, int64_t N, int64_t K, int dtype, bool bias) {
     return pl.slices > 1 ? (size_t)pl.slices * ((size_t)N * (size_t)K + (bias ? (size_t)N : 0)) * 4 : 0;
 }
 
+void wgrad8_plan(int64_t M, int64_t N, int64_t K, int* side, int* slices) {
+    const Plan pl = plan_of(M, N, K);
+    *side = pl.side;
+    *slices = pl.slices;
+}
+
 int launch_wgrad8(const void* dz, int64_t lddz, int dtype, const Mat8& x, float* dw, float* db,
                   int64_t M, int64_t N, int64_t K, void* ws, hipStream_t stream) {
     const Plan pl = plan_of(M, N, K);

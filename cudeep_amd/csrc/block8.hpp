@@ -8,7 +8,8 @@
 // largest finite magnitude is at most 448 * 2^e, and 1 for a block without a
 // finite nonzero: multiplying by a power of two is exact, so a value is
 // rounded once, and code * 2^e is exact in bf16 (the bounds keep the least
-// code, 2^-9, times the scale a normal bf16 and 1 / scale a normal float).
+// code, 2^-9, times the scale a normal bf16 and 1 / scale a normal float), but for
+// magnitudes of 248 * 2^120 and more, which round to 2^128 and come back infinite.
 // Infinities and NaN take the NaN code and stay out of the scale, so that
 // they stay visible and spoil no neighbour.
 #pragma once

@@ -291,7 +291,7 @@ void gemm8_any_kernel(Params p) {
 // ones that a lane wants in a step side by side: as bytes they are the
 // instruction's scale operand, which picks one byte of a register per 16 rows.
 //
-// bf16 results, scale bytes: 4096^3 62 to 70 us, 2.0 to 2.2 PFLOP/s, 8192 x 8192 x 4096 228,
+// bf16 results, scale bytes: 4096^3 58 to 70 us, 2.0 to 2.4 PFLOP/s, 8192 x 8192 x 4096 228,
 // 2.4; float scales 83 and 282, 1.9.  No unit is full (matrix slots 41 % busy, VALU 25 to 39,
 // LDS 20): a step's loads, LDS reads and products meet at its barrier.  32-bit results 134 and
 // 483, 1.1 PFLOP/s of the bf16 instruction.
@@ -479,8 +479,9 @@ void gemm8_tile_kernel(Params p) {
 // Few tiles: a CU has one workgroup or two, whose time is that of their
 // loads on their way.  64 x 64 tiles, four waves along B's rows, four LDS buffers: three
 // blocks are in flight.  Buffers of their own names tell the compiler that a block's reads
-// need not wait for the later blocks' loads.  64 x 4096 x 4096 9.9 us, 512 x 4096 x 4096 15.8,
-// 1.1 PFLOP/s.
+// need not wait for the later blocks' loads.  64 x 4096 x 4096 9.9 us (64 tiles: three of four
+// CUs have none, and each of these goes through all of K), 512 x 4096 x 4096 14 to 16, 1.1 PFLOP/s
+// and more.
 template <class T, int MODE>
 __global__ __launch_bounds__(256, 2)
 void gemm8_ring_kernel(Params p) {
@@ -592,9 +593,11 @@ void gemm8_ring_kernel(Params p) {
 // 128 columns split over eight waves, whose sums meet in LDS in the order of the
 // waves.  A workgroup takes 16 NT rows of B and 16 MT of A; each wave has the codes of
 // U blocks in flight.  With X the rows of A are quantised here, as they are used:
-// every workgroup does it again, in the shadow of its loads of B.  Bound by B's bytes and the
-// latency of a launch: 4096 x 4096 with 1 row 4.8 us, 3.5 TB/s, 16 rows 7.1, 32 rows 9.7; from
-// unquantised rows 1 row 7.1, 16 rows 9.0.
+// every workgroup does it again.  Bound by B's bytes, the latency of a launch, and A, which
+// every workgroup reads whole: with 16 rows of 4096 columns its 256 workgroups take as many
+// bytes of A out of L2 as of B.  4096 x 4096 with 1 row 4.8 us, 3.5 TB/s, 16 rows 7.1, 32 rows 9.7;
+// from unquantised rows 1 row 7.1, 16 rows 9.0: their loads stand behind B's in the queue, so that
+// quantising begins when B is there.
 constexpr int kDirectWaves = 8;
 
 // A lane's 32 values of a row and block as loaded: those of all rows are on their way before

@@ -9,8 +9,8 @@
 // largest magnitude through LDS.
 //
 // Bound by memory, all of them (bf16, bytes read and written over the time): rows of 8192 x
-// 8192 34.3 us, 5.9 TB/s; tiles 35.1, 5.7; restoring 31.4, 6.4; 8192 x 4096 with GELU 29.5,
-// 5.7, its gradient 32.2, 5.2 (38.9 with operands that no cache holds).
+// 8192 34.3 us, 5.9 TB/s; tiles 35.1, 5.7; restoring 31.4, 6.4; 8192 x 4096 with GELU 26.7,
+// 6.3 (28.7 with operands that no cache holds), its gradient 30.3, 5.5 (35.8).
 #include "block8.hpp"
 
 namespace cdx {
@@ -23,8 +23,8 @@ constexpr int kLane = 8;   // values per lane: 16 lanes cover a block
 // s = 1 / (1 + exp(-x)) and r = 1 - s, neither by subtraction.  fp32: from both
 // exponentials, as the elementwise kernels.  16 bits: r = exp(-x) s from one exponential,
 // held finite there: where s is 0, so is r (only s and s r are used).  The GELU backward
-// pass is bound by its exponentials and reciprocals: 8192 x 4096 in bf16 45.6 us with two
-// of each, 38.9 with one.
+// pass is held up by its exponentials and reciprocals: 8192 x 4096 in bf16 45.6 us with two
+// of each, 38.9 with one (operands that no cache holds).
 template <class T> __device__ __forceinline__ void logistic(float x, float& s, float& r) {
     if constexpr (std::is_same_v<T, float>) {
         s = 1.0f / (1.0f + expf(-x));

@@ -533,7 +533,8 @@ int cdx_layer_norm_backward(const void* grad_out, int64_t ldg, const void* x, in
  * cdx_quantize_e4m3: the scale is 2^e with the least e in [-117, 120] for which
  * the block's largest finite magnitude is at most 448 * 2^e (1 for a block
  * without a finite nonzero), a code is x / scale rounded to nearest even;
- * infinities and NaN become the NaN code.  dtype: CDX_DTYPE_F32, _F16 or _BF16.
+ * infinities and NaN become the NaN code.  (Magnitudes of 248 * 2^120 = 3.3e38 and more
+ * round to 2^128, which comes back as an infinity.)  dtype: CDX_DTYPE_F32, _F16 or _BF16.
  * No counterpart in the reference. */
 int cdx_quantize_e4m3(const void* x, int64_t ldx, int64_t rows, int64_t cols, int dtype,
                       int tile_rows, void* q, int64_t ldq, void* scale, int64_t lds,

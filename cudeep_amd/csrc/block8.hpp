@@ -251,6 +251,12 @@ __device__ __forceinline__ int64_t xcd_tile(int64_t b, int64_t count) {
     return x * each + (x < more ? x : more) + b / 8;
 }
 
+// Whether one dimension of a launch holds these workgroups: its threads are counted in 32 bits, and
+// a launch of more runs what is left of the number, without an error.
+inline bool grid_fits(int64_t groups, int threads) {
+    return groups < ((int64_t)1 << 31) && groups * threads < ((int64_t)1 << 32);
+}
+
 // An 8-bit matrix: codes with leading dimension ldq, scales [rows (or tiles
 // of 128 rows)][ceil(cols / 128)] with leading dimension lds.
 struct Mat8 {

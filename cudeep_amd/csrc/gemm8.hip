@@ -842,7 +842,8 @@ int run_direct(const Params& p, const X* x, int64_t ldx, hipStream_t stream) {
         auto go = [&](auto mt, auto nt) {
             constexpr int MT = decltype(mt)::value, NT = decltype(nt)::value;
             const int64_t grid = ceil_div(p.M, (int64_t)(16 * MT)) * ceil_div(p.N, (int64_t)(16 * NT));
-            if (grid >= (int64_t)1 << 31) return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");
+            if (!grid_fits(grid, 64 * kDirectWaves))
+                return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");
             hipLaunchKernelGGL((gemm8_direct_kernel<T, MODE, MT, NT, X>), dim3((unsigned)grid),
                                dim3(64 * kDirectWaves), 0, stream, p, x, ldx);
             return hip_error(hipGetLastError(), "gemm8_direct_kernel launch");
@@ -868,7 +869,7 @@ int run(const Params& p, hipStream_t stream) {
     const int64_t big = ceil_div(p.M, (int64_t)256) * ceil_div(p.N, (int64_t)256);
     const int64_t mid = ceil_div(p.M, (int64_t)128) * ceil_div(p.N, (int64_t)128);
     const int64_t grid = ceil_div(p.M, (int64_t)64) * ceil_div(p.N, (int64_t)64);
-    if (grid >= (int64_t)1 << 31) return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");
+    if (!grid_fits(grid, 256)) return set_error(CDX_ERR_UNSUPPORTED, "gemm8: too many output tiles");
     if (kernel == Kernel::Ring) {
         return with_mode<T>(p, [&](auto mode) {
             hipLaunchKernelGGL((gemm8_ring_kernel<T, decltype(mode)::value>), dim3((unsigned)grid), dim3(256),

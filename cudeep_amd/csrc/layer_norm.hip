@@ -402,27 +402,27 @@ void layer_norm_columns_kernel(const T* __restrict__ dy, int64_t lddy, const T* 
                                const float* __restrict__ rstd, float* __restrict__ part,
                                int64_t rows, int64_t dim, int64_t chunk) {
     constexpr int V = kVec<T>;
-    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
-    if (c >= dim) return;
-    const int n = clip(dim - c, V);
     const int64_t r0 = (int64_t)blockIdx.y * chunk;
     const int64_t r1 = r0 + chunk < rows ? r0 + chunk : rows;
-    float a[V] = {}, b[V] = {};
+    for (int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V; c < dim; c += (int64_t)gridDim.x * 256 * V) {
+        const int n = clip(dim - c, V);
+        float a[V] = {}, b[V] = {};
 #pragma unroll 4
-    for (int64_t row = r0; row < r1; ++row) {
-        const float mu = mean[row], r = rstd[row];
-        float xv[V], gv[V];
-        load_n<V>(x + row * ldx + c, n, xv);
-        load_n<V>(dy + row * lddy + c, n, gv);
+        for (int64_t row = r0; row < r1; ++row) {
+            const float mu = mean[row], r = rstd[row];
+            float xv[V], gv[V];
+            load_n<V>(x + row * ldx + c, n, xv);
+            load_n<V>(dy + row * lddy + c, n, gv);
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            a[j] += gv[j] * ((xv[j] - mu) * r);
-            b[j] += gv[j];
+            for (int j = 0; j < V; ++j) {
+                a[j] += gv[j] * ((xv[j] - mu) * r);
+                b[j] += gv[j];
+            }
         }
+        float* out = part + (int64_t)blockIdx.y * 2 * dim + c;
+        store_n<V>(out, n, a);
+        store_n<V>(out + dim, n, b);
     }
-    float* out = part + (int64_t)blockIdx.y * 2 * dim + c;
-    store_n<V>(out, n, a);
-    store_n<V>(out + dim, n, b);
 }
 
 // dw and db from `count` rows of partials [2][dim]: 64 columns by 16 lanes of
@@ -433,31 +433,34 @@ void layer_norm_params_kernel(const float* __restrict__ part, int count, int64_t
                               W* __restrict__ dw, W* __restrict__ db) {
     __shared__ float red[16][64];
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
-    const int64_t c = (int64_t)blockIdx.x * 64 + tx;
-    float a = 0.0f;
-    if (c < 2 * dim) {
-        const float* p = part + c;
-        int k = ty;
-        for (; k + 7 * 16 < count; k += 8 * 16) {
-            float v[8];
+    for (int64_t c0 = (int64_t)blockIdx.x * 64; c0 < 2 * dim; c0 += (int64_t)gridDim.x * 64) {
+        const int64_t c = c0 + tx;
+        float a = 0.0f;
+        if (c < 2 * dim) {
+            const float* p = part + c;
+            int k = ty;
+            for (; k + 7 * 16 < count; k += 8 * 16) {
+                float v[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) v[u] = p[(int64_t)(k + 16 * u) * 2 * dim];
+                for (int u = 0; u < 8; ++u) v[u] = p[(int64_t)(k + 16 * u) * 2 * dim];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) a += v[u];
+                for (int u = 0; u < 8; ++u) a += v[u];
+            }
+            for (; k < count; k += 16) a += p[(int64_t)k * 2 * dim];
         }
-        for (; k < count; k += 16) a += p[(int64_t)k * 2 * dim];
-    }
-    red[ty][tx] = a;
-    __syncthreads();
-    if (ty == 0 && c < 2 * dim) {
-        a = red[0][tx];
+        red[ty][tx] = a;
+        __syncthreads();
+        if (ty == 0 && c < 2 * dim) {
+            a = red[0][tx];
 #pragma unroll
-        for (int k = 1; k < 16; ++k) a += red[k][tx];
-        if (c < dim) {
-            if (dw) dw[c] = round_to<W>(a);
-        } else if (db) {
-            db[c - dim] = round_to<W>(a);
+            for (int k = 1; k < 16; ++k) a += red[k][tx];
+            if (c < dim) {
+                if (dw) dw[c] = round_to<W>(a);
+            } else if (db) {
+                db[c - dim] = round_to<W>(a);
+            }
         }
+        __syncthreads();
     }
 }
 
@@ -497,6 +500,9 @@ int with_shape(int64_t dim, F f) {
 // 88 us in bf16 and 140 in fp32, with the sums kept 127 and 161).
 constexpr int kBwdGroups = 512;
 
+// Workgroups of a launch: the threads of one are counted in 32 bits.
+constexpr int64_t kMostGroups = 1 << 20;
+
 template <class T> int64_t partial_rows(int64_t rows, int64_t dim) {
     int64_t out = 0;
     (void)with_shape<T, true>(dim, [&](auto tpr, auto e) {
@@ -517,15 +523,13 @@ int forward_t(const T* x, int64_t ldx, const W* w, const W* b, T* y, int64_t ldy
               float* rstd, int64_t rows, int64_t dim, float eps, hipStream_t stream) {
     return with_shape<T, false>(dim, [&](auto tpr, auto e) {
         constexpr int TPR = decltype(tpr)::value, E = decltype(e)::value;
-        constexpr int64_t most = 1 << 20;
         if constexpr (TPR == 0) {
-            const int64_t g = rows < most ? rows : most;
+            const int64_t g = std::min(rows, kMostGroups);
             hipLaunchKernelGGL((layer_norm_long_kernel<T, W>), dim3((unsigned)g), dim3(1024), 0,
                                stream, x, ldx, w, b, y, ldy, mean, rstd, rows, dim, eps);
         } else {
             constexpr int NT = TPR > 256 ? TPR : 256;
-            int64_t g = ceil_div(rows, (int64_t)(NT / TPR));
-            g = g < most ? g : most;
+            const int64_t g = std::min(ceil_div(rows, (int64_t)(NT / TPR)), kMostGroups);
             hipLaunchKernelGGL((layer_norm_kernel<T, W, TPR, E>), dim3((unsigned)g), dim3(NT), 0,
                                stream, x, ldx, w, b, y, ldy, mean, rstd, rows, dim, eps);
         }
@@ -545,7 +549,8 @@ int backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const W* w, c
         if constexpr (WIDE) {
             if (params) {   // (first: dx may be written over x or dy)
                 hipLaunchKernelGGL((layer_norm_columns_kernel<T>),
-                                   dim3((unsigned)ceil_div(dim, (int64_t)(256 * kVec<T>)), (unsigned)count),
+                                   dim3((unsigned)std::min(ceil_div(dim, (int64_t)(256 * kVec<T>)), kMostGroups),
+                                        (unsigned)count),
                                    dim3(256), 0, stream, dy, lddy, x, ldx, mean, rstd, ws, rows, dim,
                                    ceil_div(rows, count));
                 const int st1 = hip_error(hipGetLastError(), "layer_norm_columns_kernel launch");
@@ -553,7 +558,7 @@ int backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const W* w, c
             }
         }
         if constexpr (TPR == 0) {
-            const int64_t g = rows < (1 << 20) ? rows : (1 << 20);
+            const int64_t g = std::min(rows, kMostGroups);
             hipLaunchKernelGGL((layer_norm_backward_long_kernel<T, W>), dim3((unsigned)g),
                                dim3(1024), 0, stream, dy, lddy, x, ldx, w, mean, rstd, dx, lddx,
                                rows, dim);
@@ -575,8 +580,8 @@ int backward_t(const T* dy, int64_t lddy, const T* x, int64_t ldx, const W* w, c
         return hip_error(hipGetLastError(), "layer_norm_backward_kernel launch");
     });
     if (st || !params) return st;
-    hipLaunchKernelGGL(layer_norm_params_kernel<W>, dim3((unsigned)ceil_div(2 * dim, (int64_t)64)),
-                       dim3(1024), 0, stream, ws, (int)count, dim, dw, db);
+    hipLaunchKernelGGL(layer_norm_params_kernel<W>,
+                       dim3((unsigned)std::min(ceil_div(2 * dim, (int64_t)64), kMostGroups)), dim3(1024), 0, stream, ws, (int)count, dim, dw, db);
     return hip_error(hipGetLastError(), "layer_norm_params_kernel launch");
 }
 

@@ -271,17 +271,25 @@ int launch_quantize_tiles(const void* x, int64_t ldx, int64_t rows, int64_t cols
                           uint8_t* q, int64_t ldq, void* s, int64_t lds, int e8m0,
                           hipStream_t stream) {
     const int64_t tiles = ceil_div(rows, (int64_t)kBlock);
-    const dim3 grid((unsigned)ceil_div(cols, (int64_t)kBlock),
-                    (unsigned)(tiles < 65535 ? tiles : 65535));
+    constexpr int64_t most = (int64_t)1 << 21;   // blocks across a launch: 2^31 threads
     return with_dtype(dtype, [&](auto t) {
         using T = decltype(t);
-        if (e8m0)
-            hipLaunchKernelGGL((quantize_tiles_kernel<T, true>), grid, dim3(1024), 0, stream,
-                               static_cast<const T*>(x), ldx, rows, cols, q, ldq, s, lds);
-        else
-            hipLaunchKernelGGL((quantize_tiles_kernel<T, false>), grid, dim3(1024), 0, stream,
-                               static_cast<const T*>(x), ldx, rows, cols, q, ldq, s, lds);
-        return hip_error(hipGetLastError(), "quantize_tiles_kernel launch");
+        for (int64_t c = 0, b = 0; c < cols; c += most * kBlock, b += most) {
+            const int64_t part = cols - c < most * kBlock ? cols - c : most * kBlock;
+            const dim3 grid((unsigned)ceil_div(part, (int64_t)kBlock),
+                            (unsigned)(tiles < 65535 ? tiles : 65535));
+            if (e8m0)
+                hipLaunchKernelGGL((quantize_tiles_kernel<T, true>), grid, dim3(1024), 0, stream,
+                                   static_cast<const T*>(x) + c, ldx, rows, part, q + c, ldq,
+                                   static_cast<uint8_t*>(s) + b, lds);
+            else
+                hipLaunchKernelGGL((quantize_tiles_kernel<T, false>), grid, dim3(1024), 0, stream,
+                                   static_cast<const T*>(x) + c, ldx, rows, part, q + c, ldq,
+                                   static_cast<float*>(s) + b, lds);
+            const int st = hip_error(hipGetLastError(), "quantize_tiles_kernel launch");
+            if (st) return st;
+        }
+        return (int)CDX_OK;
     });
 }
 

@@ -400,7 +400,7 @@ void wgrad8_plan(int64_t M, int64_t N, int64_t K, int* side, int* slices) {
 int launch_wgrad8(const void* dz, int64_t lddz, int dtype, const Mat8& x, float* dw, float* db,
                   int64_t M, int64_t N, int64_t K, void* ws, hipStream_t stream) {
     const Plan pl = plan_of(M, N, K);
-    if (pl.tiles >= (int64_t)1 << 31) return set_error(CDX_ERR_UNSUPPORTED, "wgrad8: too many output tiles");
+    if (!grid_fits(pl.tiles, 512)) return set_error(CDX_ERR_UNSUPPORTED, "wgrad8: too many output tiles");
     float* part = static_cast<float*>(ws);
     Params p{dz, lddz, x.q, x.ldq, static_cast<const uint8_t*>(x.s), x.lds, M, N, K, pl.chunk, dw, db};
     if (pl.slices > 1) {

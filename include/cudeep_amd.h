@@ -549,7 +549,8 @@ int cdx_dequantize_e4m3(const void* q, int64_t ldq, const void* scale, int64_t l
  * layer's weight) with scales by 128 x 128 tile; C in c_dtype (CDX_DTYPE_F32, _F16 or
  * _BF16), bias fp32 [N] or NULL, epilogue CDX_EPI_NONE to _SIGMOID.  The two scale
  * types may differ.  workspace: the query's bytes (scale types and alignments make
- * no difference); NULL allocates stream-ordered.
+ * no difference); NULL allocates stream-ordered.  Products of more tiles than a launch
+ * holds (from 2^27 columns on) are CDX_ERR_UNSUPPORTED.
  *
  * Sums: products are exact.  A CDX_DTYPE_F32 result's are added in fp32.  A 16-bit
  * result's go through the 8-bit matrix instruction at twice the rate, which adds eight

@@ -557,7 +557,9 @@ int cdx_dequantize_e4m3(const void* q, int64_t ldq, const void* scale, int64_t l
  * products (consecutive k) on a grid 2^-13 below the power of two of the largest of
  * them, and those sums in fp32: at most 2^-10 of the largest of each eight products
  * are lost.  On random operands that is a hundredth of bf16's own rounding and a tenth
- * of f16's; sums that cancel may lose more than their rounding. */
+ * of f16's; sums that cancel may lose more than their rounding.  For a 32-bit result or
+ * float scales a block's two scales are multiplied in fp32 first: their product has to be
+ * finite. */
 size_t cdx_gemm_e4m3_workspace_size(int64_t M, int64_t N, int64_t K);
 int cdx_gemm_e4m3(int64_t M, int64_t N, int64_t K,
                   const void* A, int64_t lda, const void* a_scale, int64_t ldsa, int a_scale_dtype,

@@ -20,72 +20,6 @@ using namespace b8;
 
 constexpr int kLane = 8;   // values per lane: 16 lanes cover a block
 
-// s = 1 / (1 + exp(-x)) and r = 1 - s, neither by subtraction.  fp32: from both
-// exponentials, as the elementwise kernels.  16 bits: r = exp(-x) s from one exponential,
-// held finite there: where s is 0, so is r (only s and s r are used).  The GELU backward
-// pass is held up by its exponentials and reciprocals: 8192 x 4096 in bf16 45.6 us with two
-// of each, 38.9 with one (operands that no cache holds).
-template <class T> __device__ __forceinline__ void logistic(float x, float& s, float& r) {
-    if constexpr (std::is_same_v<T, float>) {
-        s = 1.0f / (1.0f + expf(-x));
-        r = 1.0f / (1.0f + expf(x));
-    } else {
-        const float e = __builtin_amdgcn_exp2f(x * -1.44269504f);
-        s = __builtin_amdgcn_rcpf(1.0f + e);
-        r = fminf(e, 0x1p126f) * s;
-    }
-}
-
-// v as a factor of s r.  In both tails s r is 0 and a slope is s itself, but v v overflows from
-// 1.8e19 on (and v is infinite where its 8 bits round to 2^128), and 0 times infinity is no slope:
-// 0 there, or for 16 bits, bound by their instructions, v within 2^30.  8192 x 4096 with GELU: fp32
-// 74.5 us, clamped 78.5; bf16 30.3, chosen by s r > 0 32.5.
-template <class T> __device__ __forceinline__ float beside(float v, float sr) {
-    if constexpr (std::is_same_v<T, float>) return sr > 0.0f ? v : 0.0f;
-    else return __builtin_amdgcn_fmed3f(v, -0x1p30f, 0x1p30f);
-}
-
-// grad * act'(v).
-template <class T, int ACT>
-__device__ __forceinline__ float act_slope(float g, float v, float alpha) {
-    if constexpr (ACT == CDX_EPI_RELU) return v > 0.0f ? g : 0.0f;
-    if constexpr (ACT == CDX_ACT_LEAKY_RELU) return v > 0.0f ? g : alpha * g;
-    float s, r;
-    if constexpr (ACT == CDX_EPI_GELU) {
-        constexpr float c = 0.7978845608f, k = 0.044715f;
-        logistic<T>(2.0f * c * (v + k * v * v * v), s, r);
-        const float n = beside<T>(v, s * r);   // slope s + 2 v s r du, du = c (1 + 3 k v v)
-        return g * (s + n * (s * r) * (2.0f * c + 6.0f * c * k * (n * n)));
-    }
-    if constexpr (ACT == CDX_EPI_SILU) {
-        logistic<T>(v, s, r);
-        return g * (s + beside<T>(v, s * r) * (s * r));
-    }
-    if constexpr (ACT == CDX_EPI_SIGMOID) {
-        logistic<T>(v, s, r);
-        return g * (s * r);
-    }
-    if constexpr (ACT == CDX_ACT_TANH) {
-        const float t = tanhf(v);
-        return g * (1.0f - t) * (1.0f + t);
-    }
-    return g;
-}
-
-// Calls f with the activation's code as a constant.
-template <class F> int with_act(int act, F f) {
-    using std::integral_constant;
-    switch (act) {
-        case CDX_EPI_RELU: return f(integral_constant<int, CDX_EPI_RELU>{});
-        case CDX_EPI_GELU: return f(integral_constant<int, CDX_EPI_GELU>{});
-        case CDX_EPI_SILU: return f(integral_constant<int, CDX_EPI_SILU>{});
-        case CDX_EPI_SIGMOID: return f(integral_constant<int, CDX_EPI_SIGMOID>{});
-        case CDX_ACT_TANH: return f(integral_constant<int, CDX_ACT_TANH>{});
-        case CDX_ACT_LEAKY_RELU: return f(integral_constant<int, CDX_ACT_LEAKY_RELU>{});
-        default: return f(integral_constant<int, CDX_EPI_NONE>{});
-    }
-}
-
 // Walks [rows, cols] in pieces of eight columns, 16 pieces to a block of 128:
 // piece p of row r is number (r * blocks + block) * 16 + p % 16.
 struct Pieces {

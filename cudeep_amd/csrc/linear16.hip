@@ -1,0 +1,175 @@
+// A Linear layer in 16 bits: which kernel runs a product, the sums of its slices, and the slope of the
+// activation.
+#include "linear16_tile.hpp"
+
+namespace cdx {
+namespace {
+
+using namespace l16;
+
+// Sums of slices, added in their order, through the epilogue: a thread has eight n of a row.  Behind
+// them the column sums.
+template <class T, bool EPI>
+__global__ __launch_bounds__(256)
+void linear16_sum_kernel(Params p, const float* __restrict__ part, const float* __restrict__ col_part,
+                         int slices) {
+    const int64_t per_row = ceil_div(p.N, (int64_t)8), body = p.M * per_row;
+    const int64_t total = body + (col_part ? p.M : 0);
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        if (i >= body) {
+            const int64_t m = i - body;
+            float v = 0.0f;
+            for (int s = 0; s < slices; ++s) v += col_part[s * p.M + m];
+            if (p.col_sums) p.col_sums[m] = v;
+            else static_cast<T*>(p.col_y)[m] = (T)v;
+            continue;
+        }
+        const int64_t m = i / per_row, n = i % per_row * 8, left = p.N - n;
+        const int count = left > 8 ? 8 : (int)left;
+        float v[8];
+        load_n<8>(part + m * p.N + n, count, v);
+        for (int s = 1; s < slices; ++s) {
+            float t[8];
+            load_n<8>(part + (s * p.M + m) * p.N + n, count, t);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += t[j];
+        }
+        if (p.out.sums) {
+            store_n<8>(p.out.sums + m * p.N + n, count, v);
+        } else if constexpr (EPI) {
+            float bias[8];
+            load_bias<T>(p.out, n, count, bias);
+            with_epilogue(p.out.act, [&](auto act) { finish8<T, decltype(act)::value>(p.out, m, n, count, v, bias); });
+        } else {
+            store_n<8>(static_cast<T*>(p.out.y) + m * p.out.ldy + n, count, v);
+        }
+    }
+}
+
+// dz = grad act'(z), eight columns a thread.
+template <class T, int ACT>
+__global__ __launch_bounds__(256)
+void linear16_slope_kernel(const T* __restrict__ grad, int64_t ldg, const T* __restrict__ z, int64_t ldz,
+                           T* __restrict__ dz, int64_t lddz, int64_t rows, int64_t cols) {
+    const int64_t per_row = ceil_div(cols, (int64_t)8), total = rows * per_row;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int64_t r = i / per_row, c = i % per_row * 8, left = cols - c;
+        const int count = left > 8 ? 8 : (int)left;
+        float g[8], v[8];
+        load_n<8>(grad + r * ldg + c, count, g);
+        load_n<8>(z + r * ldz + c, count, v);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = act_slope<T, ACT>(g[j], v[j], 0.0f);
+        store_n<8>(dz + r * lddz + c, count, v);
+    }
+}
+
+enum class Kernel { Any };
+struct Plan { Kernel kernel; int64_t tiles; int slices; int64_t chunk; };
+
+// (a layer without inputs still has its bias's column of tiles)
+int64_t tiles_of(int64_t M, int64_t N, int side) {
+    return ceil_div(M, (int64_t)side) * (N > 0 ? ceil_div(N, (int64_t)side) : 1);
+}
+
+Plan plan_of(Linear16Kind, int64_t M, int64_t N, int64_t K, bool) {
+    const int64_t tiles = tiles_of(M, N, 64);
+    int64_t s = tiles >= 256 ? 1 : 512 / tiles;
+    if (s > K / 512) s = K / 512;
+    if (s < 1 || N == 0) s = 1;
+    const int64_t chunk = ceil_div(ceil_div(K, s), (int64_t)kStep) * kStep;
+    return {Kernel::Any, tiles, K > 0 ? (int)ceil_div(K, chunk) : 1, chunk > 0 ? chunk : kStep};
+}
+
+template <class T, bool CA, bool CB>
+int run(const Params& p, const Plan& pl, hipStream_t stream) {
+    const dim3 grid((unsigned)pl.tiles, (unsigned)pl.slices);
+    hipLaunchKernelGGL((linear16_any_kernel<T, CA, CB, 64, 64, 2, 2>), grid, dim3(256), 0, stream, p);
+    return hip_error(hipGetLastError(), "linear16 kernel launch");
+}
+
+template <class F> int with_16(int dtype, F f) {
+    return dtype == CDX_DTYPE_BF16 ? f(bf16{}) : f(f16{});
+}
+
+unsigned wide_grid(int64_t threads) {
+    const int64_t g = ceil_div(threads, (int64_t)256);
+    return (unsigned)(g < 65536 ? g : 65536);
+}
+
+}  // namespace
+
+size_t linear16_workspace(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool col_sums) {
+    if (M == 0 || N == 0) return 0;
+    // (alignment may choose the kernel: the larger of both)
+    size_t most = 0;
+    for (int aligned = 0; aligned < 2; ++aligned) {
+        const Plan pl = plan_of(kind, M, N, K, aligned);
+        const size_t need = pl.slices > 1
+            ? (size_t)pl.slices * ((size_t)M * (size_t)N + (col_sums ? (size_t)M : 0)) * 4 : 0;
+        most = need > most ? need : most;
+    }
+    return most;
+}
+
+const char* linear16_kernel_name(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned,
+                                 int* slices) {
+    static const char* const names[] = {"any"};
+    const Plan pl = plan_of(kind, M, N, K, aligned);
+    *slices = pl.slices;
+    return names[(int)pl.kernel];
+}
+
+int launch_linear16(Linear16Kind kind, const Linear16Product& g, bool out_f32, void* col_y, void* ws,
+                    hipStream_t stream) {
+    const bool ca = kind == Linear16Kind::Weight, cb = kind != Linear16Kind::Forward;
+    const bool aligned = g.lda % 8 == 0 && g.ldb % 8 == 0 && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 &&
+                         g.lda <= kMaxLd && g.ldb <= kMaxLd && (!ca || g.M % 8 == 0) && (!cb || g.N % 8 == 0);
+    const Plan pl = plan_of(kind, g.M, g.N, g.K, aligned);
+    if (!grid_fits(pl.tiles, 512)) return set_error(CDX_ERR_UNSUPPORTED, "linear16: too many output tiles");
+    Params p{static_cast<const uint16_t*>(g.a), static_cast<const uint16_t*>(g.b), g.M, g.N, g.K, g.lda,
+             g.ldb, pl.chunk, g.out, nullptr, nullptr};
+    if (out_f32) {
+        p.out.sums = static_cast<float*>(g.out.y);
+        p.col_sums = static_cast<float*>(col_y);
+    } else {
+        p.col_y = col_y;
+    }
+    Params part = p;
+    float* sums = static_cast<float*>(ws);
+    float* col_part = nullptr;
+    if (pl.slices > 1) {
+        part.out.sums = sums;
+        if (col_y) col_part = part.col_sums = sums + (int64_t)pl.slices * g.M * g.N;
+    }
+    return with_16(g.dtype, [&](auto t) {
+        using T = decltype(t);
+        int st = kind == Linear16Kind::Forward ? run<T, false, false>(part, pl, stream)
+                 : kind == Linear16Kind::Input ? run<T, false, true>(part, pl, stream)
+                                               : run<T, true, true>(part, pl, stream);
+        if (st || pl.slices == 1) return st;
+        const dim3 grid(wide_grid(g.M * ceil_div(g.N, (int64_t)8) + (col_y ? g.M : 0)));
+        if (kind == Linear16Kind::Forward)
+            hipLaunchKernelGGL((linear16_sum_kernel<T, true>), grid, dim3(256), 0, stream, p, sums, col_part, pl.slices);
+        else
+            hipLaunchKernelGGL((linear16_sum_kernel<T, false>), grid, dim3(256), 0, stream, p, sums, col_part, pl.slices);
+        return hip_error(hipGetLastError(), "linear16_sum_kernel launch");
+    });
+}
+
+int launch_linear16_slope(const void* grad, int64_t ldg, const void* z, int64_t ldz, void* dz,
+                          int64_t lddz, int64_t rows, int64_t cols, int dtype, int act,
+                          hipStream_t stream) {
+    return with_16(dtype, [&](auto t) {
+        using T = decltype(t);
+        return with_act(act, [&](auto a) {
+            hipLaunchKernelGGL((linear16_slope_kernel<T, decltype(a)::value>),
+                               dim3(wide_grid(rows * ceil_div(cols, (int64_t)8))), dim3(256), 0, stream,
+                               static_cast<const T*>(grad), ldg, static_cast<const T*>(z), ldz,
+                               static_cast<T*>(dz), lddz, rows, cols);
+            return hip_error(hipGetLastError(), "linear16_slope_kernel launch");
+        });
+    });
+}
+
+}  // namespace cdx

@@ -972,3 +972,136 @@ def linear_weight_grad8(grad_out, x, *, bias=True, workspace=None):
 
 def linear_weight_grad8_workspace_bytes(M: int, N: int, K: int, dtype=torch.float32) -> int:
     return int(L.lib().cdx_linear_weight_grad_e4m3_workspace_size(M, N, K, _FLOATS[dtype]))
+
+
+# ---- Linear layers in 16 bits -----------------------------------------------------------------
+
+_HALF = {torch.float16: L.DTYPE_F16, torch.bfloat16: L.DTYPE_BF16}
+
+
+def _half_code(t, name):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    code = _HALF.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be float16 or bfloat16, got {t.dtype}")
+    _on_current(t, name)
+    return code
+
+
+def _on_current(t, name):
+    """The call's stream is the current device's: tensors of another one are refused."""
+    if _current_device is not None and t.get_device() != _current_device():
+        raise ValueError(f"{name} is on {t.device}, which is not the current device")
+
+
+def _same(t, name, like):
+    """A tensor of `like`'s type on its device."""
+    _need(t, name, like.dtype)
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+
+
+def _layer(x, weight):
+    """(dtype code, M, N, K, ldx, ldw) of a Linear layer's checked input and weight."""
+    code = _half_code(x, "input")
+    _same(weight, "weight", x)
+    if weight.dim() != 2:
+        raise ValueError("weight must be 2-D")
+    M, K, ldx = _rows(x, "input")
+    N, K2, ldw = _rows(weight, "weight")
+    if K != K2:
+        raise ValueError(f"inner dimensions differ: {K} vs {K2}")
+    return code, M, N, K, ldx, ldw
+
+
+def _like_output(t, name, x, shape):
+    """Leading dimension of a checked tensor of a layer's output shape."""
+    _same(t, name, x)
+    if t.shape != shape:
+        raise ValueError(f"{name} must be {list(shape)}, got {list(t.shape)}")
+    return _rows(t, name)[2]
+
+
+def linear16(x, weight, bias=None, *, epilogue=L.EPI_NONE, residual=None, keep=False, out=None,
+             workspace=None):
+    """residual + epi(x W^T + bias) of a float16 or bfloat16 Linear layer, in x's type: sums, bias,
+    activation and residual in float32, rounded once.  x is [..., K] (2-D: any row stride), W [N, K],
+    bias [N] of x's type or float32, residual [..., N].  With keep, (y, z): z = x W^T + bias rounded
+    to x's type, as linear16_backward takes it.  `out` may be residual itself, and must not
+    overlap the other operands.  `workspace` (linear16_workspace_bytes) makes the call
+    allocation-free."""
+    code, M, N, K, ldx, ldw = _layer(x, weight)
+    shape = x.shape[:-1] + (N,)
+    bptr, bcode = None, code
+    if bias is not None:
+        bptr = _param(bias, "bias", N, x.dtype)
+        if bias.device != x.device:
+            raise ValueError(f"bias is on {bias.device}, not on {x.device}")
+        bcode = _FLOATS[bias.dtype]
+    rptr, ldr = None, N
+    if residual is not None:
+        ldr = _like_output(residual, "residual", x, shape)
+        rptr = residual.data_ptr()
+    if out is None:
+        y, ldy = torch.empty(shape, dtype=x.dtype, device=x.device), N
+    else:
+        y, ldy = out, _like_output(out, "out", x, shape)
+    z = zptr = None
+    if keep:
+        z = torch.empty(shape, dtype=x.dtype, device=x.device)
+        zptr = z.data_ptr()
+    ws_ptr, ws_bytes, _keep = _workspace(
+        workspace, lambda: L.lib().cdx_linear16_workspace_size(M, N, K), x.device)
+    L.call("cdx_linear16", M, N, K, x.data_ptr(), ldx, weight.data_ptr(), ldw, bptr, bcode, rptr, ldr,
+           y.data_ptr(), ldy, zptr, N, epilogue, code, ws_ptr, ws_bytes, _stream())
+    return (y, z) if keep else y
+
+
+def linear16_workspace_bytes(M: int, N: int, K: int) -> int:
+    return int(L.lib().cdx_linear16_workspace_size(M, N, K))
+
+
+def linear16_backward(grad_out, x, weight, z=None, *, epilogue=L.EPI_NONE, input=True, params=True,
+                      bias=True, param_dtype=None, workspace=None):
+    """(grad of x, of weight, of bias) of linear16 from its output's gradient and, with an activation,
+    the z that it kept; the residual's gradient is grad_out itself.  grad_out * epi'(z) is rounded to
+    x's type as the products' operand, sums are float32.  The gradient of x has its type, the
+    parameters' are of `param_dtype` (x's type or float32).  None for x's without `input`, for both
+    parameters' without `params`, for the bias's without `bias`.  `workspace`
+    (linear16_backward_workspace_bytes) makes the call allocation-free."""
+    code, M, N, K, ldx, ldw = _layer(x, weight)
+    shape = x.shape[:-1] + (N,)
+    ldg = _like_output(grad_out, "grad_out", x, shape)
+    zptr, ldz = None, N
+    if epilogue != L.EPI_NONE:
+        if z is None:
+            raise ValueError("linear16_backward: an activation's gradient needs z")
+        ldz = _like_output(z, "z", x, shape)
+        zptr = z.data_ptr()
+    pdtype = param_dtype or x.dtype
+    if pdtype != x.dtype and pdtype != torch.float32:
+        raise TypeError(f"param_dtype must be {x.dtype} or float32")
+    dx = dw = db = None
+    xp = wp = bp = None
+    if input:
+        dx = _new_like(x)
+        xp = dx.data_ptr()
+    if params:
+        dw = torch.empty((N, K), dtype=pdtype, device=x.device)
+        wp = dw.data_ptr()
+        if bias:
+            db = torch.empty((N,), dtype=pdtype, device=x.device)
+            bp = db.data_ptr()
+    ws_ptr, ws_bytes, _keep = _workspace(
+        workspace, lambda: L.lib().cdx_linear16_backward_workspace_size(M, N, K, epilogue), x.device)
+    L.call("cdx_linear16_backward", M, N, K, grad_out.data_ptr(), ldg, x.data_ptr(), ldx,
+           weight.data_ptr(), ldw, zptr, ldz, epilogue, xp, K, wp, bp, code, _FLOATS[pdtype], ws_ptr,
+           ws_bytes, _stream())
+    return dx, dw, db
+
+
+def linear16_backward_workspace_bytes(M: int, N: int, K: int, epilogue=L.EPI_NONE) -> int:
+    return int(L.lib().cdx_linear16_backward_workspace_size(M, N, K, epilogue))

@@ -607,6 +607,40 @@ int cdx_linear_weight_grad_e4m3(const void* dz, int64_t lddz, int dtype,
                                 int64_t out_features, int64_t in_features,
                                 void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* ---- Linear layer in 16 bits ------------------------------------------------ */
+
+/* z = x W^T + bias, y = residual + epi(z): x [M,K], W [N,K] (a Linear layer's weight), residual, y
+ * and z [M,N], all in dtype (CDX_DTYPE_F16 or _BF16); bias [N] in dtype or CDX_DTYPE_F32.  Sums,
+ * bias, activation and residual are fp32, y is rounded once.  bias, residual and z (what the
+ * backward pass takes, rounded to dtype; y comes from the unrounded one) may be NULL.  epilogue:
+ * CDX_EPI_NONE to _SIGMOID, with the hardware's exponential and reciprocal.  y may be
+ * residual itself (the same pointer and leading dimension); y and z must not overlap anything
+ * else.  workspace: the query's bytes; NULL allocates stream-ordered.  Products of more tiles
+ * than a launch holds (from 2^23 of 64 x 64 on) are CDX_ERR_UNSUPPORTED.  The same bits every
+ * time.  No counterpart in the reference. */
+size_t cdx_linear16_workspace_size(int64_t M, int64_t N, int64_t K);
+int cdx_linear16(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
+                 const void* weight, int64_t ldw, const void* bias, int bias_dtype,
+                 const void* residual, int64_t ldr, void* y, int64_t ldy, void* z, int64_t ldz,
+                 int epilogue, int dtype, void* workspace, size_t workspace_bytes,
+                 hipStream_t stream);
+
+/* Gradients of the same layer: with dz = grad_out epi'(z), rounded to dtype as the products'
+ * operand (grad_out itself for CDX_EPI_NONE, where z may be NULL),
+ *   grad_x[m][k] = sum_n dz[m][n] W[n][k]            (dtype),
+ *   grad_weight[n][k] = sum_m dz[m][n] x[m][k]       (param_dtype, dense),
+ *   grad_bias[n] = sum_m dz[m][n]                    (param_dtype, dense),
+ * overwritten; sums fp32, the same bits every time.  (The residual's gradient is grad_out.)
+ * param_dtype: dtype or CDX_DTYPE_F32.  grad_x, grad_weight and grad_bias may be NULL (W and x
+ * then too), but grad_bias needs grad_weight.  Results must not overlap anything.
+ * workspace as above. */
+size_t cdx_linear16_backward_workspace_size(int64_t M, int64_t N, int64_t K, int epilogue);
+int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out, int64_t ldg,
+                          const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                          const void* z, int64_t ldz, int epilogue, void* grad_x, int64_t ldgx,
+                          void* grad_weight, void* grad_bias, int dtype, int param_dtype,
+                          void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 /* ---- tensor runtime ----------------------------------------------------- */
 
 /* dst (contiguous) <- src viewed with `shape` / `src_strides` (elements,

@@ -114,6 +114,14 @@ SIGNATURES = {
     "cdx_linear16_backward_workspace_size": (_sz, [_i64] * 3 + [_int]),
     "cdx_linear16_backward": (_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _int,
                                      _vp, _i64, _vp, _vp, _int, _int, _vp, _sz, _vp]),
+    "cdx_token_logprobs_workspace_size": (_sz, [_i64, _i64, _int]),
+    "cdx_token_logprobs": (_int, [_vp, _i64, _i64, _i64, _int, ctypes.c_double, _vp, _vp, _vp, _vp, _int,
+                                  _vp, _vp, _vp, _sz, _vp]),
+    "cdx_token_logprobs_backward": (_int, [_vp, _vp, _i64, _i64, _i64, _int, ctypes.c_double, _vp, _vp,
+                                           _vp, _vp, _vp, _i64, _vp]),
+    "cdx_distill_loss_workspace_size": (_sz, [_i64, _i64, _int]),
+    "cdx_distill_loss": (_int, [_vp, _i64, _i64, _i64, _int, ctypes.c_double, _vp, _i64, _int, _vp, _i64,
+                                _int, _int, _vp, _vp, _vp, _i64, _vp, _sz, _vp]),
 }
 
 DTYPE_F32, DTYPE_F64, DTYPE_F16, DTYPE_BF16, DTYPE_E8M0 = 0, 1, 2, 3, 4

@@ -1105,3 +1105,133 @@ def linear16_backward(grad_out, x, weight, z=None, *, epilogue=L.EPI_NONE, input
 
 def linear16_backward_workspace_bytes(M: int, N: int, K: int, epilogue=L.EPI_NONE) -> int:
     return int(L.lib().cdx_linear16_backward_workspace_size(M, N, K, epilogue))
+
+
+# ---- what reads a model's logits --------------------------------------------------------------
+
+class TokenLogprobs(NamedTuple):
+    """What token_logprobs returns, float32 [rows] each but for the alternatives ([rows, top]; index
+    int64) and `stats` [rows, 2], which the backward pass takes."""
+    logprob: torch.Tensor
+    stats: torch.Tensor
+    entropy: torch.Tensor | None = None
+    top_logprob: torch.Tensor | None = None
+    top_index: torch.Tensor | None = None
+
+
+def _logits(logits):
+    """(dtype code, rows, vocabulary, leading dimension) of a checked tensor of logits."""
+    code = _float_code(logits, "logits")
+    _on_current(logits, "logits")
+    rows, vocab, ld = _rows(logits, "logits")
+    return code, rows, vocab, ld
+
+
+def _per_row(t, name, rows, dtype, like):
+    """Pointer of a checked contiguous vector of a value a row."""
+    _need(t, name, dtype)
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+    if t.numel() != rows or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of {rows} elements")
+    return t.data_ptr()
+
+
+def _grad_like(out, logits, ld):
+    """(tensor, leading dimension) of a gradient in the logits' shape and type."""
+    if out is None:
+        return _new_like(logits), logits.shape[-1]
+    if out is logits:
+        return out, ld
+    _same(out, "out", logits)
+    return out, _out(out, logits.shape, logits.dtype)
+
+
+def token_logprobs(logits, targets, *, temperature=1.0, entropy=False, top=0, workspace=None):
+    """Log probabilities of given tokens: with l = log softmax(logits / temperature) over the last
+    dimension (float32, float16 or bfloat16; 2-D: any row stride), l at targets (int64, one a row; 0
+    for a negative target), with `entropy` -sum exp(l) l, and the `top` (up to 64) likeliest tokens, the
+    lowest index first among equals.  All float32.  -infinity masks a token.  `workspace`
+    (token_logprobs_workspace_bytes) makes the call allocate its results only."""
+    code, rows, vocab, ld = _logits(logits)
+    tptr = _per_row(targets, "targets", rows, torch.int64, logits)
+    dev = logits.device
+    lp = torch.empty((rows,), dtype=torch.float32, device=dev)
+    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
+    h = torch.empty_like(lp) if entropy else None
+    tl = ti = None
+    if top:
+        tl = torch.empty((rows, top), dtype=torch.float32, device=dev)
+        ti = torch.empty((rows, top), dtype=torch.int64, device=dev)
+    ws_ptr, ws_bytes, _keep = _workspace(
+        workspace, lambda: L.lib().cdx_token_logprobs_workspace_size(rows, vocab, top), dev)
+    L.call("cdx_token_logprobs", logits.data_ptr(), ld, rows, vocab, code, temperature, tptr, lp.data_ptr(),
+           stats.data_ptr(), h.data_ptr() if entropy else None, top, tl.data_ptr() if top else None,
+           ti.data_ptr() if top else None, ws_ptr, ws_bytes, _stream())
+    return TokenLogprobs(lp, stats, h, tl, ti)
+
+
+def token_logprobs_workspace_bytes(rows: int, vocab: int, top: int = 0) -> int:
+    return int(L.lib().cdx_token_logprobs_workspace_size(rows, vocab, top))
+
+
+def token_logprobs_backward(grad_logprob, logits, targets, stats, *, entropy=None, grad_entropy=None,
+                            temperature=1.0, out=None):
+    """Gradient of the logits (their shape and type) from those of logprob and, given the entropy that
+    token_logprobs returned, of the entropy (float32, one a row; either may be None).  Rows whose gradients
+    are 0 become zeros whatever they hold.  `out` may be the logits themselves."""
+    code, rows, vocab, ld = _logits(logits)
+    tptr = _per_row(targets, "targets", rows, torch.int64, logits)
+    sptr = _per_row(stats, "stats", 2 * rows, torch.float32, logits)
+    gptr = hptr = eptr = None
+    if grad_logprob is not None:
+        gptr = _per_row(grad_logprob, "grad_logprob", rows, torch.float32, logits)
+    if grad_entropy is not None:
+        if entropy is None:
+            raise ValueError("token_logprobs_backward: grad_entropy needs entropy")
+        hptr = _per_row(grad_entropy, "grad_entropy", rows, torch.float32, logits)
+        eptr = _per_row(entropy, "entropy", rows, torch.float32, logits)
+    grad, ldg = _grad_like(out, logits, ld)
+    L.call("cdx_token_logprobs_backward", gptr, logits.data_ptr(), ld, rows, vocab, code, temperature, tptr,
+           sptr, eptr, hptr, grad.data_ptr(), ldg, _stream())
+    return grad
+
+
+def distill_loss(logits, index, teacher, *, temperature=1.0, weight=None, out=None, workspace=None):
+    """The loss of each row of logits against a teacher's top logits, float32 [rows]: with q =
+    softmax(teacher / temperature) over the row's entries and l = log softmax(logits / temperature)
+    over the vocabulary, sum q (log q - l[index]).  index (int64 or int32) and teacher (float32,
+    float16 or bfloat16) are [rows, count], count up to 1024; entries of negative index do not count,
+    and a row without any has loss 0.  With `weight` (float32, one a row), (loss, gradient of
+    sum(weight * loss) with respect to the logits, in their type): one pass of a training step whose
+    rows' weights are known.  `out` (the gradient) may be the logits themselves.  `workspace`
+    (distill_loss_workspace_bytes) makes the call allocate its results only."""
+    code, rows, vocab, ld = _logits(logits)
+    for t, name in ((index, "index"), (teacher, "teacher")):
+        if not isinstance(t, torch.Tensor) or t.device != logits.device:
+            raise ValueError(f"{name} must be a tensor on {logits.device}")
+    if index.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"index must be int64 or int32, got {index.dtype}")
+    tcode = _float_code(teacher, "teacher")
+    irows, count, ldi = _rows(index, "index")
+    trows, tcount, ldt = _rows(teacher, "teacher")
+    if irows != rows or trows != rows or count != tcount:
+        raise ValueError(f"index and teacher must be [{rows}, count]")
+    loss = torch.empty((rows,), dtype=torch.float32, device=logits.device)
+    grad, gptr, ldg, wptr = None, None, vocab, None
+    if weight is not None:
+        wptr = _per_row(weight, "weight", rows, torch.float32, logits)
+        grad, ldg = _grad_like(out, logits, ld)
+        gptr = grad.data_ptr()
+    elif out is not None:
+        raise ValueError("distill_loss: a gradient needs weight")
+    ws_ptr, ws_bytes, _keep = _workspace(
+        workspace, lambda: L.lib().cdx_distill_loss_workspace_size(rows, vocab, count), logits.device)
+    L.call("cdx_distill_loss", logits.data_ptr(), ld, rows, vocab, code, temperature, index.data_ptr(), ldi,
+           index.element_size(), teacher.data_ptr(), ldt, tcode, count, loss.data_ptr(), wptr, gptr, ldg,
+           ws_ptr, ws_bytes, _stream())
+    return loss if weight is None else (loss, grad)
+
+
+def distill_loss_workspace_bytes(rows: int, vocab: int, count: int) -> int:
+    return int(L.lib().cdx_distill_loss_workspace_size(rows, vocab, count))

@@ -641,6 +641,52 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
                           void* grad_weight, void* grad_bias, int dtype, int param_dtype,
                           void* workspace, size_t workspace_bytes, hipStream_t stream);
 
+/* ---- what reads a model's logits --------------------------------------------- */
+
+/* Rows of logits x [rows, vocab] in dtype (CDX_DTYPE_F32, _F16 or _BF16), vocab in [1, 2^31 - 2^20],
+ * at a temperature T in [1e-6, 1e6]: with m = max x and L = log sum exp((x - m) / T), log softmax is
+ * l = (x - m) / T - L.  Sums are fp32, in a fixed order: the same bits every time.
+ *
+ *   logprob[r] = l at targets[r] (0 for a negative target, NaN for one past the vocabulary),
+ *   stats[r] = {m, L} (what the backward pass reads),
+ *   entropy[r] = -sum exp(l) l (may be NULL),
+ *   top_index, top_logprob [rows][top]: the `top` (0 to 64) largest logits, the largest first and
+ *     the lowest index first among equals, with their l.
+ * Logits of -infinity have probability 0.  A row of -infinity alone has logprob -infinity, entropy 0 and
+ * no gradient.  A NaN or +infinity makes its row's numbers NaN; top_index is then some index in the
+ * vocabulary.  workspace: the query's bytes; NULL allocates stream-ordered.  No counterpart in the
+ * reference. */
+size_t cdx_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top);
+int cdx_token_logprobs(const void* logits, int64_t ldx, int64_t rows, int64_t vocab, int dtype,
+                       double temperature, const int64_t* targets, float* logprob, float* stats,
+                       float* entropy, int top, float* top_logprob, int64_t* top_index,
+                       void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* grad_logits[r][v] = (g ([v = target] - p) - h p (l + entropy[r])) / T, p = exp(l), g = grad_logprob[r]
+ * (0 for a negative target), h = grad_entropy[r]; either may be NULL (0), grad_entropy needs entropy.
+ * Rows of g = h = 0 become zeros whatever they hold.  grad_logits (dtype) may be the logits' own
+ * place (the same pointer and leading dimension). */
+int cdx_token_logprobs_backward(const float* grad_logprob, const void* logits, int64_t ldx, int64_t rows,
+                                int64_t vocab, int dtype, double temperature, const int64_t* targets,
+                                const float* stats, const float* entropy, const float* grad_entropy,
+                                void* grad_logits, int64_t ldg, hipStream_t stream);
+
+/* Distillation from `count` (0 to 1024) entries of a teacher in each row: token index[r][k] (4 or 8
+ * bytes each) with the teacher's logit teacher[r][k] (teacher_dtype).  q = softmax(teacher / T) over
+ * the row's entries, but for those of negative index (and those of -infinity have q = 0);
+ *   loss[r] = sum_k q_k (log q_k - l at index_k)     (0 where no entry counts),
+ *   grad_logits[r][v] = weight[r] / T (exp(l_v) - sum of q_k with index_k = v)
+ * (0 there, where weight[r] is 0, and in a row of logits that are all -infinity).  weight NULL: the loss alone, and
+ * grad_logits is not written.  An index may come more than once; one past the vocabulary makes its
+ * row's loss and gradient NaN.  grad_logits (dtype) may be the logits' own place.  workspace as
+ * above. */
+size_t cdx_distill_loss_workspace_size(int64_t rows, int64_t vocab, int count);
+int cdx_distill_loss(const void* logits, int64_t ldx, int64_t rows, int64_t vocab, int dtype,
+                     double temperature, const void* index, int64_t ldi, int index_bytes,
+                     const void* teacher, int64_t ldt, int teacher_dtype, int count, float* loss,
+                     const float* weight, void* grad_logits, int64_t ldg, void* workspace,
+                     size_t workspace_bytes, hipStream_t stream);
+
 /* ---- tensor runtime ----------------------------------------------------- */
 
 /* dst (contiguous) <- src viewed with `shape` / `src_strides` (elements,

@@ -64,32 +64,26 @@ void linear16_slope_kernel(const T* __restrict__ grad, int64_t ldg, const T* __r
     }
 }
 
-enum class Kernel { Any };
-struct Plan { Kernel kernel; int64_t tiles; int slices; int64_t chunk; };
-
 // (a layer without inputs still has its bias's column of tiles)
 int64_t tiles_of(int64_t M, int64_t N, int side) {
     return ceil_div(M, (int64_t)side) * (N > 0 ? ceil_div(N, (int64_t)side) : 1);
 }
 
-Plan plan_of(Linear16Kind, int64_t M, int64_t N, int64_t K, bool) {
-    const int64_t tiles = tiles_of(M, N, 64);
+Plan plan_of(Linear16Kind, int64_t M, int64_t N, int64_t K, bool aligned) {
+    Kernel kernel = Kernel::Any;
+    int side = 64;
+    // (without columns of B there is nothing to load straight into LDS)
+    if (aligned && K >= kStep && N > 0) {
+        kernel = Kernel::Ring;
+        if (tiles_of(M, N, 256) >= 200) kernel = Kernel::Turns, side = 256;
+        else if (tiles_of(M, N, 128) >= 256) kernel = Kernel::Tile128, side = 128;
+    }
+    const int64_t tiles = tiles_of(M, N, side);
     int64_t s = tiles >= 256 ? 1 : 512 / tiles;
     if (s > K / 512) s = K / 512;
     if (s < 1 || N == 0) s = 1;
     const int64_t chunk = ceil_div(ceil_div(K, s), (int64_t)kStep) * kStep;
-    return {Kernel::Any, tiles, K > 0 ? (int)ceil_div(K, chunk) : 1, chunk > 0 ? chunk : kStep};
-}
-
-template <class T, bool CA, bool CB>
-int run(const Params& p, const Plan& pl, hipStream_t stream) {
-    const dim3 grid((unsigned)pl.tiles, (unsigned)pl.slices);
-    hipLaunchKernelGGL((linear16_any_kernel<T, CA, CB, 64, 64, 2, 2>), grid, dim3(256), 0, stream, p);
-    return hip_error(hipGetLastError(), "linear16 kernel launch");
-}
-
-template <class F> int with_16(int dtype, F f) {
-    return dtype == CDX_DTYPE_BF16 ? f(bf16{}) : f(f16{});
+    return {kernel, tiles, K > 0 ? (int)ceil_div(K, chunk) : 1, chunk > 0 ? chunk : kStep};
 }
 
 unsigned wide_grid(int64_t threads) {
@@ -114,7 +108,7 @@ size_t linear16_workspace(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bo
 
 const char* linear16_kernel_name(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned,
                                  int* slices) {
-    static const char* const names[] = {"any"};
+    static const char* const names[] = {"any", "ring", "tile 128", "turns"};
     const Plan pl = plan_of(kind, M, N, K, aligned);
     *slices = pl.slices;
     return names[(int)pl.kernel];
@@ -142,12 +136,12 @@ int launch_linear16(Linear16Kind kind, const Linear16Product& g, bool out_f32, v
         part.out.sums = sums;
         if (col_y) col_part = part.col_sums = sums + (int64_t)pl.slices * g.M * g.N;
     }
+    const int st = kind == Linear16Kind::Forward ? run_forward(g.dtype, part, pl, stream)
+                   : kind == Linear16Kind::Input ? run_input(g.dtype, part, pl, stream)
+                                                 : run_weight(g.dtype, part, pl, stream);
+    if (st || pl.slices == 1) return st;
     return with_16(g.dtype, [&](auto t) {
         using T = decltype(t);
-        int st = kind == Linear16Kind::Forward ? run<T, false, false>(part, pl, stream)
-                 : kind == Linear16Kind::Input ? run<T, false, true>(part, pl, stream)
-                                               : run<T, true, true>(part, pl, stream);
-        if (st || pl.slices == 1) return st;
         const dim3 grid(wide_grid(g.M * ceil_div(g.N, (int64_t)8) + (col_y ? g.M : 0)));
         if (kind == Linear16Kind::Forward)
             hipLaunchKernelGGL((linear16_sum_kernel<T, true>), grid, dim3(256), 0, stream, p, sums, col_part, pl.slices);

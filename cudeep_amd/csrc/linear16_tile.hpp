@@ -272,37 +272,56 @@ __device__ __forceinline__ void store_tile(const Params& p, uint8_t* buf, int64_
 
 // ---- the product -------------------------------------------------------------------------------
 
-// A step's products: halves of 32 k, a wave's FM fragments of A held, those of B one at a time.
-template <class T, bool CA, bool CB, int BM, int BN, int WM, int WN, bool SUMS> struct Wave {
+// A wave's products of a step, in halves of 32 k.  SUMS: the column sums of A as well, its product with
+// ones, which the WN waves that hold the same fragments of A share.
+template <class T, bool CA, bool CB, int BM, int BN, int WM, int WN> struct Wave {
     static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
+    static constexpr bool SUMS = CA && CB;
+    static constexpr int FS = (FM + WN - 1) / WN;   // fragments whose sums a wave forms
     floatx4 acc[FN][FM] = {};
-    floatx4 ones[SUMS ? FM : 1] = {};   // sum_k A(m, k), in every row: the product with ones
-    int wm, wn;
+    floatx4 ones[SUMS ? FS : 1] = {};
+    shortx8 fa[FM], fb[FN];
+    const int wm, wn;
+    const bool sums;
     Reader<CA, BM, FM> ra;
     Reader<CB, BN, FN> rb;
-    bool sums;
     __device__ __forceinline__ Wave(int lane, int wave, bool sums_)
-        : wm(wave % WM), wn(wave / WM), ra(lane, wave % WM * FM), rb(lane, wave / WM * FN), sums(sums_) {}
-    __device__ __forceinline__ void step(const uint8_t* ta, const uint8_t* tb) {
+        : wm(wave % WM), wn(wave / WM), sums(sums_), ra(lane, wave % WM * FM), rb(lane, wave / WM * FN) {}
+    template <int H> __device__ __forceinline__ void read(const uint8_t* tile) {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            shortx8 xa[FM];
+        for (int i = 0; i < FN; ++i) fb[i] = rb(tile + BM * 128, i, H);
 #pragma unroll
-            for (int j = 0; j < FM; ++j) xa[j] = ra(ta, j, h);
+        for (int j = 0; j < FM; ++j) fa[j] = ra(tile, j, H);
+    }
+    __device__ __forceinline__ void multiply() {
 #pragma unroll
-            for (int i = 0; i < FN; ++i) {
-                const shortx8 xb = rb(tb, i, h);
+        for (int i = 0; i < FN; ++i)
 #pragma unroll
-                for (int j = 0; j < FM; ++j) acc[i][j] = mfma<T>(xb, xa[j], acc[i][j]);
-            }
-            if constexpr (SUMS) {
-                if (sums) {
-                    const short one = std::is_same_v<T, bf16> ? 0x3f80 : 0x3c00;
-                    const shortx8 v = {one, one, one, one, one, one, one, one};
+            for (int j = 0; j < FM; ++j) acc[i][j] = mfma<T>(fb[i], fa[j], acc[i][j]);
+        if constexpr (SUMS) {
+            if (sums) {
+                const short one = std::is_same_v<T, bf16> ? 0x3f80 : 0x3c00;
+                const shortx8 v = {one, one, one, one, one, one, one, one};
 #pragma unroll
-                    for (int j = 0; j < FM; ++j) ones[j] = mfma<T>(v, xa[j], ones[j]);
+                for (int q = 0; q < WN; ++q) {
+                    if (wn != q) continue;
+#pragma unroll
+                    for (int f = 0; f < FS; ++f)
+                        if (q * FS + f < FM) ones[f] = mfma<T>(v, fa[q * FS + f], ones[f]);
                 }
             }
+        }
+    }
+    // The sums of column m0 + 16 j + lane of A, in every row of the product.
+    __device__ __forceinline__ void store_sums(const Params& p, int64_t m0, int lane) const {
+        if (!sums || lane >= 16) return;
+#pragma unroll
+        for (int f = 0; f < FS; ++f) {
+            const int j = wn * FS + f;
+            const int64_t m = m0 + 16 * (wm * FM + j) + lane;
+            if (j >= FM || m >= p.M) continue;
+            if (p.col_sums) p.col_sums[(int64_t)blockIdx.y * p.M + m] = ones[f][0];
+            else static_cast<T*>(p.col_y)[m] = (T)ones[f][0];
         }
     }
 };
@@ -319,18 +338,16 @@ template <int BM, int BN> __device__ __forceinline__ void tile_of(const Params& 
     n0 = id / high * BN;
 }
 
-// The column sums of A that the waves of the first tile of B's hold.
-template <class T, class W>
-__device__ __forceinline__ void store_col_sums(const Params& p, const W& w, int64_t m0, int lane) {
-    if (!w.sums || (lane >> 4) != 0) return;
-#pragma unroll
-    for (int j = 0; j < W::FM; ++j) {
-        const int64_t m = m0 + 16 * (w.wm * W::FM + j) + (lane & 15);
-        if (m >= p.M) continue;
-        if (p.col_sums) p.col_sums[(int64_t)blockIdx.y * p.M + m] = w.ones[j][0];
-        else static_cast<T*>(p.col_y)[m] = (T)w.ones[j][0];
+// The workgroup's k, and whether it forms the column sums of A.
+struct Slice {
+    int64_t k0, k1, whole;             // whole: steps without a ragged end
+    __device__ __forceinline__ explicit Slice(const Params& p) {
+        k0 = (int64_t)blockIdx.y * p.chunk;
+        k1 = k0 + p.chunk < p.K ? k0 + p.chunk : p.K;
+        whole = k1 > k0 ? (k1 - k0) / kStep : 0;
     }
-}
+};
+__device__ __forceinline__ bool forms_sums(const Params& p, int64_t n0) { return (p.col_sums || p.col_y) && n0 == 0; }
 
 // Operands of any alignment: every step through registers, the next one's loads in flight while one is
 // multiplied.
@@ -338,36 +355,230 @@ template <class T, bool CA, bool CB, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN)
 void linear16_any_kernel(Params p) {
     constexpr int NT = 64 * WM * WN;
-    constexpr bool SUMS = CA && CB;
     __shared__ __attribute__((aligned(1024))) uint8_t lds[(BM + BN) * 128];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int64_t m0, n0;
     tile_of<BM, BN>(p, m0, n0);
-    const int64_t k0 = (int64_t)blockIdx.y * p.chunk, k1 = k0 + p.chunk < p.K ? k0 + p.chunk : p.K;
+    const Slice sl(p);
     Loader<CA, BM, NT> la(p.a, p.lda, m0, p.M);
     Loader<CB, BN, NT> lb(p.b, p.ldb, n0, p.N);
-    Wave<T, CA, CB, BM, BN, WM, WN, SUMS> w(lane, wave, SUMS && (p.col_sums || p.col_y) && n0 == 0 && wave / WM == 0);
+    Wave<T, CA, CB, BM, BN, WM, WN> w(lane, wave, forms_sums(p, n0));
     typename Loader<CA, BM, NT>::Held ha;
     typename Loader<CB, BN, NT>::Held hb;
-    if (k0 < k1) {
-        la.load(k0, k1, ha);
-        lb.load(k0, k1, hb);
+    if (sl.k0 < sl.k1) {
+        la.load(sl.k0, sl.k1, ha);
+        lb.load(sl.k0, sl.k1, hb);
     }
-    for (int64_t k = k0; k < k1; k += kStep) {
+    for (int64_t k = sl.k0; k < sl.k1; k += kStep) {
         __syncthreads();
         la.store(ha, lds);
         lb.store(hb, lds + BM * 128);
         __syncthreads();
-        if (k + kStep < k1) {
-            la.load(k + kStep, k1, ha);
-            lb.load(k + kStep, k1, hb);
+        if (k + kStep < sl.k1) {
+            la.load(k + kStep, sl.k1, ha);
+            lb.load(k + kStep, sl.k1, hb);
         }
-        w.step(lds, lds + BM * 128);
+        w.template read<0>(lds);
+        w.multiply();
+        w.template read<1>(lds);
+        w.multiply();
     }
     constexpr int ROWS = (BM + BN) * 128 / (BN * 4) < BM ? (BM + BN) * 128 / (BN * 4) : BM;
     store_tile<T, !CA && !CB, BM, BN, WM, WN, ROWS>(p, lds, m0, n0, w.wm, w.wn, w.acc);
-    if constexpr (SUMS) store_col_sums<T>(p, w, m0, lane);
+    if constexpr (w.SUMS) w.store_sums(p, m0, lane);
 }
+
+// The ragged end of k through registers, and the results.
+template <class T, bool CA, bool CB, int BM, int BN, int WM, int WN, class W, class LA, class LB>
+__device__ __forceinline__ void finish_tile(const Params& p, const Slice& sl, W& w, const LA& la, const LB& lb,
+                                            uint8_t* buf, int64_t m0, int64_t n0, int lane) {
+    if (sl.k0 + sl.whole * kStep < sl.k1) {
+        typename LA::Held ha;
+        typename LB::Held hb;
+        la.load(sl.k0 + sl.whole * kStep, sl.k1, ha);
+        lb.load(sl.k0 + sl.whole * kStep, sl.k1, hb);
+        __syncthreads();
+        la.store(ha, buf);
+        lb.store(hb, buf + BM * 128);
+        __syncthreads();
+        w.template read<0>(buf);
+        w.multiply();
+        w.template read<1>(buf);
+        w.multiply();
+    }
+    constexpr int ROWS = (BM + BN) * 128 / (BN * 4) < BM ? (BM + BN) * 128 / (BN * 4) : BM;
+    store_tile<T, !CA && !CB, BM, BN, WM, WN, ROWS>(p, buf, m0, n0, w.wm, w.wn, w.acc);
+    if constexpr (W::SUMS) w.store_sums(p, m0, lane);
+}
+
+// Aligned operands, whole steps straight into LDS, D buffers of their own names (which tells the compiler
+// that a step's reads need not wait for the later steps' loads): D - 1 steps are in flight, one
+// barrier a step.
+template <class T, bool CA, bool CB, int BM, int BN, int WM, int WN, int D>
+__global__ __launch_bounds__(64 * WM * WN, 2)
+void linear16_tile_kernel(Params p) {
+    constexpr int NT = 64 * WM * WN, SIZE = (BM + BN) * 128;
+    static_assert(D == 2 || D == 4, "two or four buffers");
+    __shared__ __attribute__((aligned(1024))) uint8_t r0[SIZE];
+    __shared__ __attribute__((aligned(1024))) uint8_t r1[SIZE];
+    __shared__ __attribute__((aligned(1024))) uint8_t r2[D == 4 ? SIZE : 16];
+    __shared__ __attribute__((aligned(1024))) uint8_t r3[D == 4 ? SIZE : 16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int64_t m0, n0;
+    tile_of<BM, BN>(p, m0, n0);
+    const Slice sl(p);
+    const int64_t whole = sl.whole;
+    Loader<CA, BM, NT> la(p.a, p.lda, m0, p.M);
+    Loader<CB, BN, NT> lb(p.b, p.ldb, n0, p.N);
+    constexpr int LOADS = Loader<CA, BM, NT>::LOADS + Loader<CB, BN, NT>::LOADS;
+    Wave<T, CA, CB, BM, BN, WM, WN> w(lane, wave, forms_sums(p, n0));
+    auto fetch = [&](int64_t s, uint8_t* buf) {
+        // (past the last step that one again, which nobody reads: the waits count loads)
+        s = s < whole ? s : whole - 1;
+        la.fetch(sl.k0 + s * kStep, buf, wave);
+        lb.fetch(sl.k0 + s * kStep, buf + BM * 128, wave);
+    };
+    auto step = [&](int64_t s, const uint8_t* now, uint8_t* last) {
+        constexpr int N = (D - 2) * LOADS;
+        // vmcnt(N) lgkmcnt(0): this step's rows are in LDS, and the last step's are read
+        __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);
+        asm volatile("s_barrier" ::: "memory");
+        fetch(s + D - 1, last);
+        __builtin_amdgcn_sched_barrier(0);   // (the compiler would issue the loads between the last products)
+        w.template read<0>(now);
+        w.multiply();
+        w.template read<1>(now);
+        w.multiply();
+    };
+    if (whole > 0) {
+        fetch(0, r0);
+        if constexpr (D == 4) {
+            fetch(1, r1);
+            fetch(2, r2);
+        }
+        int64_t s = 0;
+#pragma unroll 1
+        for (; s + D <= whole; s += D) {
+            step(s, r0, D == 4 ? r3 : r1);
+            step(s + 1, r1, r0);
+            if constexpr (D == 4) {
+                step(s + 2, r2, r1);
+                step(s + 3, r3, r2);
+            }
+        }
+        if (s < whole) step(s, r0, D == 4 ? r3 : r1);
+        if constexpr (D == 4) {
+            if (s + 1 < whole) step(s + 1, r1, r0);
+            if (s + 2 < whole) step(s + 2, r2, r1);
+        }
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070);   // nothing is on its way to LDS
+    finish_tile<T, CA, CB, BM, BN, WM, WN>(p, sl, w, la, lb, r0, m0, n0, lane);
+}
+
+// The same with eight waves in two groups (a wave of each on every SIMD) that take turns: while one
+// group's operands come out of LDS, the other multiplies, a barrier between the phases.  A step is four phases
+// (read, multiply, read, multiply); the second group is a phase behind.  The next step's loads are
+// issued in the first phase, when the step before is read to its end by both groups, and waited for before
+// the barrier that ends the step for the first group.
+template <class T, bool CA, bool CB>
+__global__ __launch_bounds__(512, 2)
+void linear16_turns_kernel(Params p) {
+    constexpr int BM = 256, BN = 256, WM = 2, WN = 4, NT = 512, SIZE = (BM + BN) * 128;
+    __shared__ __attribute__((aligned(1024))) uint8_t r0[SIZE];
+    __shared__ __attribute__((aligned(1024))) uint8_t r1[SIZE];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int64_t m0, n0;
+    tile_of<BM, BN>(p, m0, n0);
+    const Slice sl(p);
+    const int64_t whole = sl.whole;
+    Loader<CA, BM, NT> la(p.a, p.lda, m0, p.M);
+    Loader<CB, BN, NT> lb(p.b, p.ldb, n0, p.N);
+    Wave<T, CA, CB, BM, BN, WM, WN> w(lane, wave, forms_sums(p, n0));
+    const bool second = wave >= 4;
+    auto fetch = [&](int64_t s, uint8_t* buf) {
+        s = s < whole ? s : whole - 1;   // (nobody reads it then)
+        la.fetch(sl.k0 + s * kStep, buf, wave);
+        lb.fetch(sl.k0 + s * kStep, buf + BM * 128, wave);
+    };
+    auto barrier = [&]() {
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    auto multiply = [&]() {
+        __builtin_amdgcn_s_setprio(1);
+        w.multiply();
+        __builtin_amdgcn_s_setprio(0);
+    };
+    auto step = [&](int64_t s, uint8_t* now, uint8_t* next) {
+        w.template read<0>(now);
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(s + 1, next);
+        barrier();
+        multiply();
+        barrier();
+        w.template read<1>(now);
+        // lgkmcnt(0): what was read is there before the other group may write over it; vmcnt(0)
+        if (second) __builtin_amdgcn_s_waitcnt(0x0070);
+        else __builtin_amdgcn_s_waitcnt(0xc07f);
+        barrier();
+        multiply();
+        if (!second) __builtin_amdgcn_s_waitcnt(0x0f70);   // vmcnt(0)
+        barrier();
+    };
+    if (whole > 0) {
+        fetch(0, r0);
+        __builtin_amdgcn_s_waitcnt(0x0070);
+        barrier();
+        if (second) barrier();
+        int64_t s = 0;
+#pragma unroll 1
+        for (; s + 2 <= whole; s += 2) {
+            step(s, r0, r1);
+            step(s + 1, r1, r0);
+        }
+        if (s < whole) step(s, r0, r1);
+        if (!second) barrier();
+    }
+    __builtin_amdgcn_s_waitcnt(0x0070);   // nothing is on its way to LDS
+    __syncthreads();
+    finish_tile<T, CA, CB, BM, BN, WM, WN>(p, sl, w, la, lb, r0, m0, n0, lane);
+}
+
+// ---- launches ------------------------------------------------------------------------------------
+
+enum class Kernel { Any, Ring, Tile128, Turns };
+struct Plan { Kernel kernel; int64_t tiles; int slices; int64_t chunk; };
+
+template <class F> int with_16(int dtype, F f) {
+    return dtype == CDX_DTYPE_BF16 ? f(bf16{}) : f(f16{});
+}
+
+template <class T, bool CA, bool CB>
+int run(const Params& p, const Plan& pl, hipStream_t stream) {
+    const dim3 grid((unsigned)pl.tiles, (unsigned)pl.slices);
+    switch (pl.kernel) {
+        case Kernel::Turns:
+            hipLaunchKernelGGL((linear16_turns_kernel<T, CA, CB>), grid, dim3(512), 0, stream, p);
+            break;
+        case Kernel::Tile128:
+            hipLaunchKernelGGL((linear16_tile_kernel<T, CA, CB, 128, 128, 2, 2, 2>), grid, dim3(256), 0, stream, p);
+            break;
+        case Kernel::Ring:
+            hipLaunchKernelGGL((linear16_tile_kernel<T, CA, CB, 64, 64, 2, 2, 4>), grid, dim3(256), 0, stream, p);
+            break;
+        case Kernel::Any:
+            hipLaunchKernelGGL((linear16_any_kernel<T, CA, CB, 64, 64, 2, 2>), grid, dim3(256), 0, stream, p);
+            break;
+    }
+    return hip_error(hipGetLastError(), "linear16 kernel launch");
+}
+
+// The products of one kind each (files of their own, which compile at the same time).
+int run_forward(int dtype, const Params& p, const Plan& pl, hipStream_t stream);
+int run_input(int dtype, const Params& p, const Plan& pl, hipStream_t stream);
+int run_weight(int dtype, const Params& p, const Plan& pl, hipStream_t stream);
 
 }  // namespace l16
 }  // namespace cdx

@@ -1,0 +1,12 @@
+// The product dw = dz^T x of a Linear layer in 16 bits: the kernels of linear16_tile.hpp.
+#include "linear16_tile.hpp"
+
+namespace cdx {
+namespace l16 {
+
+int run_weight(int dtype, const Params& p, const Plan& pl, hipStream_t stream) {
+    return with_16(dtype, [&](auto t) { return run<decltype(t), true, true>(p, pl, stream); });
+}
+
+}  // namespace l16
+}  // namespace cdx

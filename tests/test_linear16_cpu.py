@@ -75,3 +75,9 @@ def test_wrappers_refuse_host_tensors():
     for f in (lambda: ops.linear16(x, w), lambda: ops.linear16_backward(x, x, w), lambda: ops.linear16([1], w)):
         with pytest.raises((ValueError, TypeError)):
             f()
+
+
+def test_a_layer_without_inputs_takes_the_kernel_that_reads_none():
+    from tests.routes16 import linear16_kernel
+    for M, K in ((24, 130), (4096, 8192), (8, 64)):
+        assert linear16_kernel("weight", M, 0, K) == ("any", 1)

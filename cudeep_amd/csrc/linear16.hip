@@ -39,7 +39,7 @@ void linear16_sum_kernel(Params p, const float* __restrict__ part, const float* 
         } else if constexpr (EPI) {
             float bias[8];
             load_bias<T>(p.out, n, count, bias);
-            with_epilogue(p.out.act, [&](auto act) { finish8<T, decltype(act)::value>(p.out, m, n, count, v, bias); });
+            with_epilogue(p.out.act, [&](auto act) { finish<T, decltype(act)::value>(p.out, m, n, count, v, bias); });
         } else {
             store_n<8>(static_cast<T*>(p.out.y) + m * p.out.ldy + n, count, v);
         }
@@ -69,21 +69,41 @@ int64_t tiles_of(int64_t M, int64_t N, int side) {
     return ceil_div(M, (int64_t)side) * (N > 0 ? ceil_div(N, (int64_t)side) : 1);
 }
 
-Plan plan_of(Linear16Kind, int64_t M, int64_t N, int64_t K, bool aligned) {
-    Kernel kernel = Kernel::Any;
-    int side = 64;
-    // (without columns of B there is nothing to load straight into LDS)
-    if (aligned && K >= kStep && N > 0) {
-        kernel = Kernel::Ring;
-        if (tiles_of(M, N, 256) >= 200) kernel = Kernel::Turns, side = 256;
-        else if (tiles_of(M, N, 128) >= 256) kernel = Kernel::Tile128, side = 128;
-    }
+Plan make_plan(Kernel kernel, int64_t M, int64_t N, int64_t K, int side, int64_t slices) {
     const int64_t tiles = tiles_of(M, N, side);
-    int64_t s = tiles >= 256 ? 1 : 512 / tiles;
-    if (s > K / 512) s = K / 512;
-    if (s < 1 || N == 0) s = 1;
-    const int64_t chunk = ceil_div(ceil_div(K, s), (int64_t)kStep) * kStep;
+    const int64_t chunk = ceil_div(ceil_div(K, slices), (int64_t)kStep) * kStep;
     return {kernel, tiles, K > 0 ? (int)ceil_div(K, chunk) : 1, chunk > 0 ? chunk : kStep};
+}
+
+Plan direct_plan(int64_t M, int64_t N, int mt) {
+    return {Kernel::Direct, ceil_div(M, (int64_t)(16 * mt)) * ceil_div(N, (int64_t)16), 1, kStep, mt};
+}
+
+Plan plan_of(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned) {
+    aligned = aligned && K >= kStep && N > 0;
+    if (kind == Linear16Kind::Forward && K > 0 && M <= (aligned ? 128 : 64)) {
+        const int64_t tiles_m = ceil_div(M, (int64_t)16), tiles_n = ceil_div(N, (int64_t)16);
+        int mt = 1;
+        while (mt < 4 && ceil_div(tiles_m, (int64_t)mt) * tiles_n > 256 && mt < tiles_m) mt *= 2;
+        if (!aligned || (mt <= 2 && K <= 8192 && ceil_div(tiles_m, (int64_t)mt) * tiles_n <= (M <= 16 ? 512 : 256)))
+            return direct_plan(M, N, mt);
+    }
+    int64_t slices = 1;
+    auto cut = [&](int64_t tiles, int64_t least) {   // slices for a workgroup a CU, of `least` k and more
+        const int64_t s = tiles > 0 ? 256 / tiles : 1;
+        return s > K / least ? (K / least > 1 ? K / least : 1) : s > 1 ? s : 1;
+    };
+    // (without columns of B there is nothing to load straight into LDS)
+    if (!aligned) {
+        if (N > 0) slices = cut(tiles_of(M, N, 64), 1024);
+        return make_plan(Kernel::Any, M, N, K, 64, slices);
+    }
+    const int64_t t256 = tiles_of(M, N, 256), t128 = tiles_of(M, N, 128), t64 = tiles_of(M, N, 64);
+    const int64_t long_k = K / 4096 < 256 ? K / 4096 : 256;
+    if (t256 >= 200 || t256 * long_k >= 256) return make_plan(Kernel::Turns, M, N, K, 256, cut(t256, 4096));
+    if (t128 > 256) return make_plan(Kernel::Tile128, M, N, K, 128, 1);
+    if (t128 >= 140 || t128 * long_k >= 256) return make_plan(Kernel::Ring128, M, N, K, 128, cut(t128, 4096));
+    return make_plan(Kernel::Ring64, M, N, K, 64, cut(t64, 1024));
 }
 
 unsigned wide_grid(int64_t threads) {
@@ -91,35 +111,8 @@ unsigned wide_grid(int64_t threads) {
     return (unsigned)(g < 65536 ? g : 65536);
 }
 
-}  // namespace
-
-size_t linear16_workspace(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool col_sums) {
-    if (M == 0 || N == 0) return 0;
-    // (alignment may choose the kernel: the larger of both)
-    size_t most = 0;
-    for (int aligned = 0; aligned < 2; ++aligned) {
-        const Plan pl = plan_of(kind, M, N, K, aligned);
-        const size_t need = pl.slices > 1
-            ? (size_t)pl.slices * ((size_t)M * (size_t)N + (col_sums ? (size_t)M : 0)) * 4 : 0;
-        most = need > most ? need : most;
-    }
-    return most;
-}
-
-const char* linear16_kernel_name(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned,
-                                 int* slices) {
-    static const char* const names[] = {"any", "ring", "tile 128", "turns"};
-    const Plan pl = plan_of(kind, M, N, K, aligned);
-    *slices = pl.slices;
-    return names[(int)pl.kernel];
-}
-
-int launch_linear16(Linear16Kind kind, const Linear16Product& g, bool out_f32, void* col_y, void* ws,
-                    hipStream_t stream) {
-    const bool ca = kind == Linear16Kind::Weight, cb = kind != Linear16Kind::Forward;
-    const bool aligned = g.lda % 8 == 0 && g.ldb % 8 == 0 && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 &&
-                         g.lda <= kMaxLd && g.ldb <= kMaxLd && (!ca || g.M % 8 == 0) && (!cb || g.N % 8 == 0);
-    const Plan pl = plan_of(kind, g.M, g.N, g.K, aligned);
+int launch_plan(Linear16Kind kind, const Linear16Product& g, const Plan& pl, bool out_f32, void* col_y, void* ws,
+                hipStream_t stream) {
     if (!grid_fits(pl.tiles, 512)) return set_error(CDX_ERR_UNSUPPORTED, "linear16: too many output tiles");
     Params p{static_cast<const uint16_t*>(g.a), static_cast<const uint16_t*>(g.b), g.M, g.N, g.K, g.lda,
              g.ldb, pl.chunk, g.out, nullptr, nullptr};
@@ -149,6 +142,37 @@ int launch_linear16(Linear16Kind kind, const Linear16Product& g, bool out_f32, v
             hipLaunchKernelGGL((linear16_sum_kernel<T, false>), grid, dim3(256), 0, stream, p, sums, col_part, pl.slices);
         return hip_error(hipGetLastError(), "linear16_sum_kernel launch");
     });
+}
+
+}  // namespace
+
+size_t linear16_workspace(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool col_sums) {
+    if (M == 0 || N == 0) return 0;
+    // (alignment may choose the kernel: the larger of both)
+    size_t most = 0;
+    for (int aligned = 0; aligned < 2; ++aligned) {
+        const Plan pl = plan_of(kind, M, N, K, aligned);
+        const size_t need = pl.slices > 1
+            ? (size_t)pl.slices * ((size_t)M * (size_t)N + (col_sums ? (size_t)M : 0)) * 4 : 0;
+        most = need > most ? need : most;
+    }
+    return most;
+}
+
+const char* linear16_kernel_name(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned,
+                                 int* slices) {
+    static const char* const names[] = {"any", "ring 64", "ring 128", "tile 128", "turns", "direct"};
+    const Plan pl = plan_of(kind, M, N, K, aligned);
+    *slices = pl.slices;
+    return names[(int)pl.kernel];
+}
+
+int launch_linear16(Linear16Kind kind, const Linear16Product& g, bool out_f32, void* col_y, void* ws,
+                    hipStream_t stream) {
+    const bool ca = kind == Linear16Kind::Weight, cb = kind != Linear16Kind::Forward;
+    const bool aligned = g.lda % 8 == 0 && g.ldb % 8 == 0 && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 &&
+                         g.lda <= kMaxLd && g.ldb <= kMaxLd && (!ca || g.M % 8 == 0) && (!cb || g.N % 8 == 0);
+    return launch_plan(kind, g, plan_of(kind, g.M, g.N, g.K, aligned), out_f32, col_y, ws, stream);
 }
 
 int launch_linear16_slope(const void* grad, int64_t ldg, const void* z, int64_t ldz, void* dz,

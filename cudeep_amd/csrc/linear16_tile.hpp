@@ -45,6 +45,25 @@ __device__ __forceinline__ floatx4 mfma(shortx8 b, shortx8 a, floatx4 c) {
                                                       __builtin_bit_cast(f16x8, a), c, 0, 0, 0);
 }
 
+// The same with the sum kept in its registers: the compiler's own form gives each product a new place for
+// its result, which 32 of them a wave do not leave room for.  What reads the sums otherwise has to call
+// settle_sums first.
+template <class T> __device__ __forceinline__ void mfma_in_place(shortx8 b, shortx8 a, floatx4& c) {
+    if constexpr (std::is_same_v<T, bf16>)
+        asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+v"(c) : "v"(b), "v"(a));
+    else
+        asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+v"(c) : "v"(b), "v"(a));
+}
+
+// Waits until the last products are written (a result is there 19 wait states after its instruction, at most).
+template <int N, int M> __device__ __forceinline__ void settle_sums(floatx4 (&c)[N][M]) {
+    asm volatile("s_nop 15\n\ts_nop 15");
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+#pragma unroll
+        for (int j = 0; j < M; ++j) asm volatile("" : "+v"(c[i][j]));   // (reads come behind it)
+}
+
 // ---- an operand's tile of EXT rows (or columns) and one step in LDS ---------------------------
 
 // What the 32-byte units of a row of k are exchanged by: rows 0 to 3 and 8 to 11 (4 to 7 and 12 to 15),
@@ -65,33 +84,34 @@ template <bool COLS, int EXT> __device__ __forceinline__ void piece_source(int a
     }
 }
 
-// A wave's F operands of the instruction, from the tile's 16 rows (columns) number `first` on: a lane
-// has eight k (8 g + 0..7 of the step's half h) of row `l16`.
+// A wave's F operands of the instruction, from the tile's 16 rows (columns) number `first` (a multiple of
+// F) on: a lane has eight k (8 g + 0..7 of the step's half H) of row `l16`.
 template <bool COLS, int EXT, int F> struct Reader {
-    int at[COLS ? F : 2];
+    int at;
     __device__ __forceinline__ Reader(int lane, int first) {
         const int l16 = lane & 15, g = lane >> 4;
         if constexpr (COLS) {
             const int row = 8 * g + (l16 >> 2);
-#pragma unroll
-            for (int i = 0; i < F; ++i) {
-                const int u = first + i, swap = unit_swap<EXT>(row);   // (the swap leaves u's high bits)
-                at[i] = row * (2 * EXT) + 32 * (u ^ swap) + 8 * (l16 & 3);
-            }
+            at = row * (2 * EXT) + 32 * (first ^ unit_swap<EXT>(row)) + 8 * (l16 & 3);
         } else {
-            at[0] = first * 2048 + l16 * 128 + (g ^ (l16 >> 1)) * 16;
-            at[1] = at[0] ^ 64;
+            at = first * 2048 + l16 * 128 + (g ^ (l16 >> 1)) * 16;
         }
     }
-    __device__ __forceinline__ shortx8 operator()(const uint8_t* tile, int i, int h) const {
-        if constexpr (COLS) {
-            typedef __attribute__((address_space(3))) shortx4* P3;
-            const uint8_t* p = tile + h * (64 * EXT) + at[i];
-            const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P3)p);
-            const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P3)(p + 8 * EXT));
-            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-        } else {
-            return *reinterpret_cast<const shortx8*>(tile + i * 2048 + at[h]);
+    template <int H> __device__ __forceinline__ void read(const uint8_t* tile, shortx8 (&f)[F]) const {
+        int base = at;
+        // (addresses are formed where they are used: kept over the loop, they would not fit the registers)
+        if constexpr (COLS) asm volatile("" : "+v"(base));
+#pragma unroll
+        for (int i = 0; i < F; ++i) {
+            if constexpr (COLS) {
+                typedef __attribute__((address_space(3))) shortx4* P3;
+                const uint8_t* p = tile + H * (64 * EXT) + (base ^ (32 * i));
+                const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P3)p);
+                const shortx4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P3)(p + 8 * EXT));
+                f[i] = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+            } else {
+                f[i] = *reinterpret_cast<const shortx8*>(tile + i * 2048 + (base ^ (64 * H)));
+            }
         }
     }
 };
@@ -164,31 +184,31 @@ template <bool COLS, int EXT, int NT> struct Loader {
 
 // ---- results ---------------------------------------------------------------------------------
 
-// Eight sums of row m from column n on (the first `count` exist) through bias, activation and residual.
-template <class T, int ACT>
-__device__ __forceinline__ void finish8(const Linear16Out& o, int64_t m, int64_t n, int count,
-                                        float (&v)[8], const float (&bias)[8]) {
+// W sums of row m from column n on (the first `count` exist) through bias, activation and residual.
+template <class T, int ACT, int W>
+__device__ __forceinline__ void finish(const Linear16Out& o, int64_t m, int64_t n, int count,
+                                       float (&v)[W], const float (&bias)[W]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] += bias[j];
-    if (o.z) store_n<8>(static_cast<T*>(o.z) + m * o.ldz + n, count, v);
-    float r[8] = {};
-    if (o.residual) load_n<8>(static_cast<const T*>(o.residual) + m * o.ldr + n, count, r);
+    for (int j = 0; j < W; ++j) v[j] += bias[j];
+    if (o.z) store_n<W>(static_cast<T*>(o.z) + m * o.ldz + n, count, v);
+    float r[W] = {};
+    if (o.residual) load_n<W>(static_cast<const T*>(o.residual) + m * o.ldr + n, count, r);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = act_value<T, ACT>(v[j], 0.0f);
+    for (int j = 0; j < W; ++j) v[j] = act_value<T, ACT>(v[j], 0.0f);
     if (o.residual) {   // (adding a zero would turn -0 into 0)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] += r[j];
+        for (int j = 0; j < W; ++j) v[j] += r[j];
     }
-    store_n<8>(static_cast<T*>(o.y) + m * o.ldy + n, count, v);
+    store_n<W>(static_cast<T*>(o.y) + m * o.ldy + n, count, v);
 }
 
-template <class T>
-__device__ __forceinline__ void load_bias(const Linear16Out& o, int64_t n, int count, float (&b)[8]) {
+template <class T, int W>
+__device__ __forceinline__ void load_bias(const Linear16Out& o, int64_t n, int count, float (&b)[W]) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) b[j] = 0.0f;
+    for (int j = 0; j < W; ++j) b[j] = 0.0f;
     if (!o.bias || count <= 0) return;
-    if (o.bias_f32) load_n<8>(static_cast<const float*>(o.bias) + n, count, b);
-    else load_n<8>(static_cast<const T*>(o.bias) + n, count, b);
+    if (o.bias_f32) load_n<W>(static_cast<const float*>(o.bias) + n, count, b);
+    else load_n<W>(static_cast<const T*>(o.bias) + n, count, b);
 }
 
 // Calls f with the epilogue's code as a constant.
@@ -260,7 +280,7 @@ __device__ __forceinline__ void store_tile(const Params& p, uint8_t* buf, int64_
             each([&](int64_t m, float (&v)[8]) { store_n<8>(sums + m * p.N + n, count, v); });
         } else if constexpr (EPI) {
             with_epilogue(p.out.act, [&](auto act) {
-                each([&](int64_t m, float (&v)[8]) { finish8<T, decltype(act)::value>(p.out, m, n, count, v, bias); });
+                each([&](int64_t m, float (&v)[8]) { finish<T, decltype(act)::value>(p.out, m, n, count, v, bias); });
             });
         } else {
             each([&](int64_t m, float (&v)[8]) {
@@ -272,56 +292,75 @@ __device__ __forceinline__ void store_tile(const Params& p, uint8_t* buf, int64_
 
 // ---- the product -------------------------------------------------------------------------------
 
-// A wave's products of a step, in halves of 32 k.  SUMS: the column sums of A as well, its product with
-// ones, which the WN waves that hold the same fragments of A share.
-template <class T, bool CA, bool CB, int BM, int BN, int WM, int WN> struct Wave {
+// A wave's products of a step, in halves of 32 k.  SUMS: the column sums of A as well, a lane's eight k of
+// its column at a time (the vector unit has nothing else to do).  The workgroups of all tiles of B, and the WN waves that hold the same fragments of A, share the
+// fragments, so that none has much more to do than the others (8192 x 4096 x 4096 with all sums in the
+// first tile's workgroups 233 us, without any 216).
+template <class T, bool CA, bool CB, int BM, int BN, int WM, int WN, bool IN_PLACE = false> struct Wave {
     static constexpr int FM = BM / WM / 16, FN = BN / WN / 16;
     static constexpr bool SUMS = CA && CB;
     static constexpr int FS = (FM + WN - 1) / WN;   // fragments whose sums a wave forms
     floatx4 acc[FN][FM] = {};
-    floatx4 ones[SUMS ? FS : 1] = {};
+    float sums[SUMS ? FS : 1] = {};
     shortx8 fa[FM], fb[FN];
     const int wm, wn;
-    const bool sums;
+    int mine = 0;                                   // bit f: the sums of fragment wn FS + f are this wave's
     Reader<CA, BM, FM> ra;
     Reader<CB, BN, FN> rb;
-    __device__ __forceinline__ Wave(int lane, int wave, bool sums_)
-        : wm(wave % WM), wn(wave / WM), sums(sums_), ra(lane, wave % WM * FM), rb(lane, wave / WM * FN) {}
+    __device__ __forceinline__ Wave(const Params& p, int lane, int wave, int64_t n0)
+        : wm(wave % WM), wn(wave / WM), ra(lane, wave % WM * FM), rb(lane, wave / WM * FN) {
+        if constexpr (SUMS) {
+            if (!p.col_sums && !p.col_y) return;
+            const int64_t tiles = p.N > BN ? ceil_div(p.N, (int64_t)BN) : 1;
+            const int every = tiles < 1024 ? (int)tiles : 1024, at = (int)(n0 / BN);
+#pragma unroll
+            for (int f = 0; f < FS; ++f)
+                if (wn * FS + f < FM && (f * WM * WN + wave) % every == at) mine |= 1 << f;
+        }
+    }
     template <int H> __device__ __forceinline__ void read(const uint8_t* tile) {
-#pragma unroll
-        for (int i = 0; i < FN; ++i) fb[i] = rb(tile + BM * 128, i, H);
-#pragma unroll
-        for (int j = 0; j < FM; ++j) fa[j] = ra(tile, j, H);
+        rb.template read<H>(tile + BM * 128, fb);
+        ra.template read<H>(tile, fa);
     }
     __device__ __forceinline__ void multiply() {
 #pragma unroll
-        for (int i = 0; i < FN; ++i)
+        for (int i = 0; i < FN; ++i) {
 #pragma unroll
-            for (int j = 0; j < FM; ++j) acc[i][j] = mfma<T>(fb[i], fa[j], acc[i][j]);
-        if constexpr (SUMS) {
-            if (sums) {
-                const short one = std::is_same_v<T, bf16> ? 0x3f80 : 0x3c00;
-                const shortx8 v = {one, one, one, one, one, one, one, one};
-#pragma unroll
-                for (int q = 0; q < WN; ++q) {
-                    if (wn != q) continue;
-#pragma unroll
-                    for (int f = 0; f < FS; ++f)
-                        if (q * FS + f < FM) ones[f] = mfma<T>(v, fa[q * FS + f], ones[f]);
-                }
+            for (int j = 0; j < FM; ++j) {
+                if constexpr (IN_PLACE) mfma_in_place<T>(fb[i], fa[j], acc[i][j]);
+                else acc[i][j] = mfma<T>(fb[i], fa[j], acc[i][j]);
             }
+            if constexpr (SUMS)
+                if (i == 0 && mine) add_sums();
         }
     }
-    // The sums of column m0 + 16 j + lane of A, in every row of the product.
+    __device__ __forceinline__ void add_sums() {
+#pragma unroll
+        for (int j = 0; j < FM; ++j) {
+            if (wn != j / FS || !(mine & (1 << j % FS))) continue;
+            T e[8];
+            __builtin_memcpy(e, &fa[j], 16);
+            float s = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += (float)e[k];
+            sums[j % FS] += s;
+        }
+    }
+    __device__ __forceinline__ void settle() {
+        if constexpr (IN_PLACE) settle_sums(acc);
+    }
+    // A column's sum lies in the four lanes that share it.
     __device__ __forceinline__ void store_sums(const Params& p, int64_t m0, int lane) const {
-        if (!sums || lane >= 16) return;
 #pragma unroll
         for (int f = 0; f < FS; ++f) {
-            const int j = wn * FS + f;
-            const int64_t m = m0 + 16 * (wm * FM + j) + lane;
-            if (j >= FM || m >= p.M) continue;
-            if (p.col_sums) p.col_sums[(int64_t)blockIdx.y * p.M + m] = ones[f][0];
-            else static_cast<T*>(p.col_y)[m] = (T)ones[f][0];
+            if (!(mine & (1 << f))) continue;
+            float v = sums[f];
+            v += __shfl_xor(v, 16);
+            v += __shfl_xor(v, 32);
+            const int64_t m = m0 + 16 * (wm * FM + wn * FS + f) + (lane & 15);
+            if (lane >= 16 || m >= p.M) continue;
+            if (p.col_sums) p.col_sums[(int64_t)blockIdx.y * p.M + m] = v;
+            else static_cast<T*>(p.col_y)[m] = (T)v;
         }
     }
 };
@@ -338,7 +377,7 @@ template <int BM, int BN> __device__ __forceinline__ void tile_of(const Params& 
     n0 = id / high * BN;
 }
 
-// The workgroup's k, and whether it forms the column sums of A.
+// The workgroup's k.
 struct Slice {
     int64_t k0, k1, whole;             // whole: steps without a ragged end
     __device__ __forceinline__ explicit Slice(const Params& p) {
@@ -347,7 +386,6 @@ struct Slice {
         whole = k1 > k0 ? (k1 - k0) / kStep : 0;
     }
 };
-__device__ __forceinline__ bool forms_sums(const Params& p, int64_t n0) { return (p.col_sums || p.col_y) && n0 == 0; }
 
 // Operands of any alignment: every step through registers, the next one's loads in flight while one is
 // multiplied.
@@ -362,7 +400,7 @@ void linear16_any_kernel(Params p) {
     const Slice sl(p);
     Loader<CA, BM, NT> la(p.a, p.lda, m0, p.M);
     Loader<CB, BN, NT> lb(p.b, p.ldb, n0, p.N);
-    Wave<T, CA, CB, BM, BN, WM, WN> w(lane, wave, forms_sums(p, n0));
+    Wave<T, CA, CB, BM, BN, WM, WN> w(p, lane, wave, n0);
     typename Loader<CA, BM, NT>::Held ha;
     typename Loader<CB, BN, NT>::Held hb;
     if (sl.k0 < sl.k1) {
@@ -406,6 +444,7 @@ __device__ __forceinline__ void finish_tile(const Params& p, const Slice& sl, W&
         w.template read<1>(buf);
         w.multiply();
     }
+    w.settle();
     constexpr int ROWS = (BM + BN) * 128 / (BN * 4) < BM ? (BM + BN) * 128 / (BN * 4) : BM;
     store_tile<T, !CA && !CB, BM, BN, WM, WN, ROWS>(p, buf, m0, n0, w.wm, w.wn, w.acc);
     if constexpr (W::SUMS) w.store_sums(p, m0, lane);
@@ -431,7 +470,7 @@ void linear16_tile_kernel(Params p) {
     Loader<CA, BM, NT> la(p.a, p.lda, m0, p.M);
     Loader<CB, BN, NT> lb(p.b, p.ldb, n0, p.N);
     constexpr int LOADS = Loader<CA, BM, NT>::LOADS + Loader<CB, BN, NT>::LOADS;
-    Wave<T, CA, CB, BM, BN, WM, WN> w(lane, wave, forms_sums(p, n0));
+    Wave<T, CA, CB, BM, BN, WM, WN> w(p, lane, wave, n0);
     auto fetch = [&](int64_t s, uint8_t* buf) {
         // (past the last step that one again, which nobody reads: the waits count loads)
         s = s < whole ? s : whole - 1;
@@ -494,7 +533,7 @@ void linear16_turns_kernel(Params p) {
     const int64_t whole = sl.whole;
     Loader<CA, BM, NT> la(p.a, p.lda, m0, p.M);
     Loader<CB, BN, NT> lb(p.b, p.ldb, n0, p.N);
-    Wave<T, CA, CB, BM, BN, WM, WN> w(lane, wave, forms_sums(p, n0));
+    Wave<T, CA, CB, BM, BN, WM, WN, true> w(p, lane, wave, n0);
     const bool second = wave >= 4;
     auto fetch = [&](int64_t s, uint8_t* buf) {
         s = s < whole ? s : whole - 1;   // (nobody reads it then)
@@ -508,6 +547,7 @@ void linear16_turns_kernel(Params p) {
     };
     auto multiply = [&]() {
         __builtin_amdgcn_s_setprio(1);
+        asm volatile("s_nop 1");   // (an operand that was moved rather than read is there)
         w.multiply();
         __builtin_amdgcn_s_setprio(0);
     };
@@ -546,10 +586,96 @@ void linear16_turns_kernel(Params p) {
     finish_tile<T, CA, CB, BM, BN, WM, WN>(p, sl, w, la, lb, r0, m0, n0, lane);
 }
 
+// Few rows of x (both operands' rows hold k): operands from global memory straight into registers, any
+// alignment, the inner size split over eight waves in chunks of 64, whose sums meet in LDS in the order
+// of the waves.  A workgroup takes 16 columns and 16 MT rows; a wave has the weights of U chunks in
+// flight.
+constexpr int kDirectWaves = 8;
+
+template <class T, int MT>
+__global__ __launch_bounds__(64 * kDirectWaves)
+void linear16_direct_kernel(Params p) {
+    constexpr int NW = kDirectWaves, U = 8 / MT;
+    __shared__ floatx4 red[NW][MT][64];
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t tiles_n = ceil_div(p.N, (int64_t)16);
+    const int64_t n0 = blockIdx.x % tiles_n * 16, m0 = blockIdx.x / tiles_n * (16 * MT);
+    // a lane's row of each operand tile (rows past the last read it again)
+    const uint16_t* b = p.b + (n0 + l16 < p.N ? n0 + l16 : p.N - 1) * p.ldb + 8 * g;
+    const uint16_t* a[MT];
+#pragma unroll
+    for (int j = 0; j < MT; ++j) {
+        const int64_t m = m0 + 16 * j + l16;
+        a[j] = p.a + (m < p.M ? m : p.M - 1) * p.lda + 8 * g;
+    }
+    auto piece = [&](const uint16_t* s, int64_t k) {   // eight k from k + 8 g on, zeros past K
+        const int64_t left = p.K - k - 8 * g;
+        if (left >= 8) return load16(s + k);
+        uint16_t t[8] = {};
+#pragma unroll
+        for (int j = 0; j < 7; ++j)
+            if (j < left) t[j] = s[k + j];
+        u32x4 v;
+        __builtin_memcpy(&v, t, 16);
+        return v;
+    };
+    floatx4 acc[MT] = {};
+    auto multiply = [&](const u32x4 (&w)[2], const u32x4 (&x)[MT][2]) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+                acc[j] = mfma<T>(__builtin_bit_cast(shortx8, w[h]), __builtin_bit_cast(shortx8, x[j][h]), acc[j]);
+    };
+    const int64_t whole = p.K / 64, chunks = ceil_div(p.K, (int64_t)64);
+    int64_t c = wave;
+    for (; c + (U - 1) * NW < whole; c += U * NW) {
+        u32x4 w[U][2], x[U][MT][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) w[u][h] = load16(b + (c + u * NW) * 64 + 32 * h);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) x[u][j][h] = load16(a[j] + (c + u * NW) * 64 + 32 * h);
+        __builtin_amdgcn_sched_barrier(0);   // (all of them on their way before the first is used)
+#pragma unroll
+        for (int u = 0; u < U; ++u) multiply(w[u], x[u]);
+    }
+#pragma unroll 1
+    for (; c < chunks; c += NW) {
+        u32x4 w[2], x[MT][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            w[h] = piece(b, c * 64 + 32 * h);
+#pragma unroll
+            for (int j = 0; j < MT; ++j) x[j][h] = piece(a[j], c * 64 + 32 * h);
+        }
+        multiply(w, x);
+    }
+#pragma unroll
+    for (int j = 0; j < MT; ++j) red[wave][j][lane] = acc[j];
+    __syncthreads();
+    if (wave >= MT) return;
+    floatx4 sum = red[0][wave][lane];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) sum += red[w][wave][lane];
+    const int64_t m = m0 + 16 * wave + l16, n = n0 + 4 * g, left = p.N - n;
+    const int count = left < 0 ? 0 : left > 4 ? 4 : (int)left;
+    if (m >= p.M || count == 0) return;
+    float bias[4], v[4] = {sum[0], sum[1], sum[2], sum[3]};
+    load_bias<T>(p.out, n, count, bias);
+    with_epilogue(p.out.act, [&](auto act) { finish<T, decltype(act)::value>(p.out, m, n, count, v, bias); });
+}
+
 // ---- launches ------------------------------------------------------------------------------------
 
-enum class Kernel { Any, Ring, Tile128, Turns };
-struct Plan { Kernel kernel; int64_t tiles; int slices; int64_t chunk; };
+enum class Kernel { Any, Ring64, Ring128, Tile128, Turns, Direct };
+struct Plan { Kernel kernel; int64_t tiles; int slices; int64_t chunk; int mt = 1; };   // mt: Direct's MT
 
 template <class F> int with_16(int dtype, F f) {
     return dtype == CDX_DTYPE_BF16 ? f(bf16{}) : f(f16{});
@@ -565,11 +691,22 @@ int run(const Params& p, const Plan& pl, hipStream_t stream) {
         case Kernel::Tile128:
             hipLaunchKernelGGL((linear16_tile_kernel<T, CA, CB, 128, 128, 2, 2, 2>), grid, dim3(256), 0, stream, p);
             break;
-        case Kernel::Ring:
+        case Kernel::Ring128:
+            hipLaunchKernelGGL((linear16_tile_kernel<T, CA, CB, 128, 128, 2, 4, 4>), grid, dim3(512), 0, stream, p);
+            break;
+        case Kernel::Ring64:
             hipLaunchKernelGGL((linear16_tile_kernel<T, CA, CB, 64, 64, 2, 2, 4>), grid, dim3(256), 0, stream, p);
             break;
         case Kernel::Any:
             hipLaunchKernelGGL((linear16_any_kernel<T, CA, CB, 64, 64, 2, 2>), grid, dim3(256), 0, stream, p);
+            break;
+        case Kernel::Direct:
+            if constexpr (!CA && !CB) {
+                const dim3 threads(64 * kDirectWaves);
+                if (pl.mt == 1) hipLaunchKernelGGL((linear16_direct_kernel<T, 1>), grid, threads, 0, stream, p);
+                else if (pl.mt == 2) hipLaunchKernelGGL((linear16_direct_kernel<T, 2>), grid, threads, 0, stream, p);
+                else hipLaunchKernelGGL((linear16_direct_kernel<T, 4>), grid, threads, 0, stream, p);
+            }
             break;
     }
     return hip_error(hipGetLastError(), "linear16 kernel launch");

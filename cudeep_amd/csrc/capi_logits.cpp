@@ -10,8 +10,6 @@ using namespace cdx::checks;
 
 namespace {
 
-static_assert(sizeof(cdx::RowStats) == 2 * sizeof(float), "two floats a row");
-
 int check_logits(const char* fn, const void* x, int64_t ldx, int64_t rows, int64_t vocab, int dtype,
                  double temperature) {
     if (bad_dim(rows)) return bad(fn, "rows must be in [0, 2^40]");
@@ -38,7 +36,7 @@ extern "C" {
 
 size_t cdx_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top) {
     if (bad_dim(rows) || vocab < 1 || vocab > cdx::kMaxVocab || top < 0 || top > cdx::kMaxTop) return 0;
-    return cdx::token_logprobs_workspace(rows, vocab, CDX_DTYPE_F32, top);
+    return cdx::token_logprobs_workspace(rows, vocab, top);
 }
 
 int cdx_token_logprobs(const void* logits, int64_t ldx, int64_t rows, int64_t vocab, int dtype,
@@ -53,7 +51,7 @@ int cdx_token_logprobs(const void* logits, int64_t ldx, int64_t rows, int64_t vo
     if (!targets || !logprob || !stats) return bad(fn, "targets, logprob or stats is NULL");
     if (top > 0 && (!top_logprob || !top_index)) return bad(fn, "top_logprob or top_index is NULL");
     cdx::TokenLogprobArgs a{logit_rows(logits, ldx, rows, vocab, dtype, temperature), targets, logprob,
-                            reinterpret_cast<cdx::RowStats*>(stats), entropy, top, top_logprob, top_index};
+                            stats, entropy, top, top_logprob, top_index};
     return with_workspace(fn, cdx_token_logprobs_workspace_size(rows, vocab, top), workspace, workspace_bytes,
                           stream, [&](void* ws) { return cdx::launch_token_logprobs(a, ws, stream); });
 }
@@ -69,13 +67,13 @@ int cdx_token_logprobs_backward(const float* grad_logprob, const void* logits, i
     if (!targets || !stats) return bad(fn, "targets or stats is NULL");
     if (grad_entropy && !entropy) return bad(fn, "grad_entropy needs entropy");
     return cdx::launch_token_logprobs_backward(logit_rows(logits, ldx, rows, vocab, dtype, temperature), targets,
-                                               reinterpret_cast<const cdx::RowStats*>(stats), grad_logprob,
+                                               stats, grad_logprob,
                                                entropy, grad_entropy, grad_logits, ldg, stream);
 }
 
 size_t cdx_distill_loss_workspace_size(int64_t rows, int64_t vocab, int count) {
     if (bad_dim(rows) || vocab < 1 || vocab > cdx::kMaxVocab || count < 0 || count > cdx::kMaxEntries) return 0;
-    return cdx::distill_workspace(rows, vocab, CDX_DTYPE_F32, count, true);
+    return cdx::distill_workspace(rows, vocab, CDX_DTYPE_F32, count);
 }
 
 int cdx_distill_loss(const void* logits, int64_t ldx, int64_t rows, int64_t vocab, int dtype,
@@ -104,6 +102,6 @@ int cdx_distill_loss(const void* logits, int64_t ldx, int64_t rows, int64_t voca
 
 // Internal: how many workgroups share a row (op 0: log probabilities with `top` alternatives; 1: distillation).
 extern "C" int cdxi_logits_parts(int op, int64_t rows, int64_t vocab, int top) {
-    return op ? cdx::distill_parts(rows, vocab, CDX_DTYPE_F32, true)
-              : cdx::token_logprobs_parts(rows, vocab, CDX_DTYPE_F32, top);
+    return op ? cdx::distill_parts(rows, vocab, CDX_DTYPE_F32)
+              : cdx::token_logprobs_parts(rows, vocab, top);
 }

@@ -25,6 +25,31 @@ constexpr int kUnroll = 4;           // 16-byte pieces of a thread in flight
 
 template <class T> constexpr int kVec = 16 / (int)sizeof(T);
 
+// A whole piece read for the last time, or written, past the caches (STREAM): what they hold of the rows
+// that are read again stays there.  4096 x 65536 in bf16, loss and gradient: 226 us, 247 with ordinary loads
+// and stores; 2048 x 131072 237 and 272.  Gradients that the caches can hold are left there for
+// the product that reads them (streams).
+typedef u32x4 __attribute__((aligned(1))) u32x4_any;
+template <bool STREAM> __device__ __forceinline__ u32x4 load_piece(const void* p) {
+    if constexpr (STREAM) return __builtin_nontemporal_load(static_cast<const u32x4_any*>(p));
+    else return load16(p);
+}
+template <bool STREAM, class T> __device__ __forceinline__ void store_piece(T* p, const float (&v)[kVec<T>]) {
+    if constexpr (STREAM) {
+        T e[kVec<T>];
+#pragma unroll
+        for (int j = 0; j < kVec<T>; ++j) e[j] = round_to<T>(v[j]);
+        u32x4 w;
+        __builtin_memcpy(&w, e, 16);
+        __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(p));
+    } else {
+        store_n<kVec<T>>(p, kVec<T>, v);
+    }
+}
+inline bool streams(int64_t rows, int64_t vocab, int dtype) {
+    return (double)rows * (double)vocab * (dtype == CDX_DTYPE_F32 ? 4 : 2) >= 256e6;
+}
+
 // The sums of some of a row's elements: m their maximum, s = sum e, t = sum e (x - m), e = exp((x - m) / T).
 struct Part { float m, s, t; };
 
@@ -61,85 +86,113 @@ template <bool ENT, int N> __device__ __forceinline__ float take(Part& a, const 
     return most;
 }
 
-// The join over a workgroup of NT threads, in all of them.
+// The join over a workgroup of NT threads, in all of them: the waves' maxima and sums by lane rotations, the
+// waves' parts by those of 16 lanes.
 template <bool ENT, int NT> __device__ __forceinline__ Part join_all(Part a, float c, Part* red) {
-#pragma unroll
-    for (int k = 1; k < 64; k *= 2) {
-        const Part b{__shfl_xor(a.m, k), __shfl_xor(a.s, k), ENT ? __shfl_xor(a.t, k) : 0.0f};
-        a = (threadIdx.x & k) ? join<ENT>(b, a, c) : join<ENT>(a, b, c);
-    }
-    __syncthreads();
+    rescale<ENT>(a, max64(a.m), c);
+    a.s = sum64(a.s);
+    if constexpr (ENT) a.t = sum64(a.t);
+    __syncthreads();   // (the last call's readers are done)
     if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = a;
     __syncthreads();
-    a = red[0];
-#pragma unroll
-    for (int w = 1; w < NT / 64; ++w) a = join<ENT>(a, red[w], c);
+    const int w = threadIdx.x & 15;
+    a = w < NT / 64 ? red[w] : Part{kLowest, 0.0f, 0.0f};
+    rescale<ENT>(a, max16(a.m), c);
+    a.s = sum16(a.s);
+    if constexpr (ENT) a.t = sum16(a.t);
     return a;
 }
 
-// kUnroll pieces of a thread as loaded: piece u begins at element `at` + u * NT * kVec; elements from
-// `end` on read as -infinity.
-template <class T, int NT> struct Pieces {
-    static constexpr int N = kUnroll * kVec<T>, STRIDE = NT * kVec<T>;
-    u32x4 u[kUnroll];
-    __device__ __forceinline__ void load(const T* x, int at) {
+// U pieces of 16 bytes of a thread as loaded: piece i is wanted from element `at` + i NT kVec on.  Where that
+// would pass `end`, the row's last kVec elements are loaded instead and the wanted ones of them kept
+// (mask), so that all loads are on their way together.
+template <class T, int NT, int U> struct Pieces {
+    static constexpr int V = kVec<T>, N = U * V, STRIDE = NT * V, ROUND = NT * N;
+    u32x4 u[U];
+    __device__ __forceinline__ void load(const T* x, int at, int end) {
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i) u[i] = load16(x + at + i * STRIDE);
+        for (int i = 0; i < U; ++i) {
+            const int from = at + i * STRIDE;
+            u[i] = load16(x + (from < end - V ? from : end - V));
+        }
+    }
+    __device__ __forceinline__ void get(int i, float (&v)[V]) const {
+        T e[V];
+        __builtin_memcpy(e, &u[i], 16);
+#pragma unroll
+        for (int j = 0; j < V; ++j) v[j] = (float)e[j];
     }
     __device__ __forceinline__ void get(float (&v)[N]) const {
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i) {
-            T e[kVec<T>];
-            __builtin_memcpy(e, &u[i], 16);
+        for (int i = 0; i < U; ++i) {
+            float w[V];
+            get(i, w);
 #pragma unroll
-            for (int j = 0; j < kVec<T>; ++j) v[i * kVec<T> + j] = (float)e[j];
+            for (int j = 0; j < V; ++j) v[i * V + j] = w[j];
         }
     }
-    __device__ __forceinline__ static void get_checked(const T* x, int at, int end, float (&v)[N]) {
+    // -infinity in the place of the elements of piece i that belong to the piece before, or to none.
+    __device__ __forceinline__ static void mask(int i, int at, int end, float (&v)[V]) {
+        const int from = at + i * STRIDE, off = from - (end - V);   // the wanted ones begin at `off`
 #pragma unroll
-        for (int i = 0; i < kUnroll; ++i) {
-            const int from = at + i * STRIDE, n = end - from;
-            float w[kVec<T>];
-            load_n<kVec<T>>(x + (n > 0 ? from : 0), n, w, -__builtin_inff());
+        for (int j = 0; j < V; ++j) v[j] = j < off ? -__builtin_inff() : v[j];
+    }
+    __device__ __forceinline__ static void mask(int at, int end, float (&v)[N]) {
 #pragma unroll
-            for (int j = 0; j < kVec<T>; ++j) v[i * kVec<T> + j] = w[j];
+        for (int i = 0; i < U; ++i) {
+            float w[V];
+#pragma unroll
+            for (int j = 0; j < V; ++j) w[j] = v[i * V + j];
+            mask(i, at, end, w);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[i * V + j] = w[j];
         }
     }
 };
 
-// The sums of elements begin .. end - 1, and, with TOP, the thread's largest value and the round it first
-// lies in (-infinity and 0 where nothing is larger).
-template <class T, int NT, bool ENT, bool TOP>
-__device__ __forceinline__ Part scan(const T* x, int begin, int end, float c, float& best, int& round) {
-    using P = Pieces<T, NT>;
-    constexpr int ROUND = NT * P::N;
+// A thread's largest value (-infinity where nothing is larger), the round that it first lies in and that
+// round's pieces.
+template <class T, int NT> struct Best { float value = -__builtin_inff(); int round = 0; Pieces<T, NT, kUnroll> held; };
+struct NoBest {};
+
+// The sums of elements begin .. end - 1, and, with a Best, that.
+template <class T, int NT, bool ENT, class B>
+__device__ __forceinline__ Part scan(const T* x, int begin, int end, float c, B& best) {
+    using P = Pieces<T, NT, kUnroll>;
     Part a{kLowest, 0.0f, 0.0f};
-    const int whole = (end - begin) / ROUND;
-    const int at = begin + (int)threadIdx.x * kVec<T>;
     float v[P::N];
-    best = -__builtin_inff();
-    round = 0;
+    P now, next;
     auto use = [&](int r) {
         const float most = take<ENT>(a, v, c);
-        if constexpr (TOP) {
-            round = most > best ? r : round;
-            best = fmaxf(best, most);
+        if constexpr (!std::is_same_v<B, NoBest>) {
+            if (r == 0) best.held = now;
+            if (most > best.value) {   // (seldom after the first rounds)
+                best.value = most;
+                best.round = r;
+                best.held = now;
+            }
         }
     };
-    if (whole > 0) {
-        P now, next;
-        now.load(x, at);
-        for (int r = 0; r < whole; ++r) {
-            if (r + 1 < whole) next.load(x, at + (r + 1) * ROUND);
-            now.get(v);
-            use(r);
-            now = next;
+    if (end - begin < P::V) {   // (less than one piece)
+#pragma unroll
+        for (int j = 0; j < P::N; ++j) {
+            const int i = begin + j;
+            v[j] = threadIdx.x == 0 && j < P::V && i < end ? (float)x[i] : -__builtin_inff();
         }
+        take<ENT>(a, v, c);
+        return a;
     }
-    if (begin + whole * ROUND < end) {
-        P::get_checked(x, at + whole * ROUND, end, v);
-        use(whole);
+    const int rounds = (end - begin + P::ROUND - 1) / P::ROUND, at = begin + (int)threadIdx.x * P::V;
+    now.load(x, at, end);
+    for (int r = 0; r + 1 < rounds; ++r) {
+        next.load(x, at + (r + 1) * P::ROUND, end);
+        now.get(v);
+        use(r);
+        now = next;
     }
+    now.get(v);
+    P::mask(at + (rounds - 1) * P::ROUND, end, v);
+    use(rounds - 1);
     return a;
 }
 
@@ -160,111 +213,126 @@ __device__ __forceinline__ float key_value(u64 k) {
     return __builtin_bit_cast(float, u ^ (u >> 31 ? 0x80000000u : 0xffffffffu));
 }
 
-constexpr int kTopThreads = 256;
-constexpr int kRoundKeys = kTopThreads * 8;             // at most, of one round of pieces
-constexpr int kTopBuffer = kRoundKeys + 512;
+constexpr int kGroups = 256;             // groups of neighbouring threads whose largest element is known, at most
+constexpr int kSpare = 512;              // keys kept from one round of pieces to the next, at most
 
-struct TopShared {
-    u64 keys[kTopBuffer];
-    u64 best[kTopThreads];
+template <int NT> struct TopShared {
+    static constexpr int ROUND = NT * 8, MOST = ROUND + kSpare;   // keys of one round of pieces, at most
+    alignas(16) u64 keys[MOST];
+    alignas(16) u64 best[kGroups];
     u64 threshold;
-    int count, chosen, who[kMaxTop];
+    int count, who[kMaxTop];
 };
 
-// Leaves the `k` largest of the first `count` keys in their order at the front (all threads call it).
-// A key's place is the number of larger ones; keys differ, so that places do.
-__device__ __forceinline__ int keep_largest(u64* keys, int count, int k) {
-    constexpr int MOST = (kTopBuffer + kTopThreads - 1) / kTopThreads;
-    u64 mine[MOST];
-    int place[MOST];
-    int n = 0;
-    for (int i = threadIdx.x; i < count; i += kTopThreads, ++n) {
-        const u64 key = keys[i];
-        int larger = 0;
-        for (int j = 0; j < count; ++j) larger += keys[j] > key;
-        // (a static index: the arrays stay in registers)
+// How many of `count` keys (from a 16-byte address on) are larger.
+__device__ __forceinline__ int larger_ones(const u64* keys, int count, u64 key) {
+    typedef u64 u64x2 __attribute__((ext_vector_type(2)));
+    int n = 0, j = 0;
+#pragma unroll 1
+    for (; j + 16 <= count; j += 16) {   // (eight reads on their way together)
+        u64x2 k[8];
 #pragma unroll
-        for (int s = 0; s < MOST; ++s)
-            if (s == n) { mine[s] = key; place[s] = larger; }
+        for (int i = 0; i < 8; ++i) k[i] = *reinterpret_cast<const u64x2*>(keys + j + 2 * i);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n += (k[i][0] > key) + (k[i][1] > key);
+    }
+#pragma unroll 4
+    for (; j < count; ++j) n += keys[j] > key;
+    return n;
+}
+
+// Leaves the `k` largest of the first `count` keys, at most MOST, in their order at the front (all NT threads
+// call it).  A key's place is the number of larger ones; keys differ, so that places do.
+template <int NT, int MOST> __device__ __forceinline__ int keep_largest(u64* keys, int count, int k) {
+    constexpr int EACH = (MOST + NT - 1) / NT;
+    u64 mine[EACH];
+    int place[EACH];
+#pragma unroll
+    for (int s = 0; s < EACH; ++s) {
+        const int i = threadIdx.x + s * NT;
+        place[s] = k;
+        if (i < count) {
+            mine[s] = keys[i];
+            place[s] = larger_ones(keys, count, mine[s]);
+        }
     }
     __syncthreads();
 #pragma unroll
-    for (int s = 0; s < MOST; ++s)
-        if (s < n && place[s] < k) keys[place[s]] = mine[s];
+    for (int s = 0; s < EACH; ++s)
+        if (place[s] < k) keys[place[s]] = mine[s];
     __syncthreads();
     return count < k ? count : k;
 }
 
-// The k-th largest of the threads' keys (0 where fewer are there), by halving: the first wave holds all of
-// them, four a lane.
-__device__ __forceinline__ u64 kth_largest(const u64* best, int k) {
-    const int lane = threadIdx.x & 63;
-    u64 v[kTopThreads / 64];
-#pragma unroll
-    for (int i = 0; i < kTopThreads / 64; ++i) v[i] = best[lane + 64 * i];
-    u64 at = 0;
-    for (int bit = 63; bit >= 0; --bit) {
-        const u64 up = at | 1ull << bit;
-        int n = 0;
-#pragma unroll
-        for (int i = 0; i < kTopThreads / 64; ++i) n += __popcll(__ballot(v[i] >= up));
-        if (n >= k) at = up;
-        if (n == k) break;
-    }
-    return at;
-}
-
-// The k largest of elements begin .. end - 1 at the front of sh.keys; how many there are.  `best`, `round`:
-// the scan's.  Each thread's largest element is known; the k-th largest of those is a bound that the k
-// largest elements of all reach, and they lie with the k threads whose own reach it: only those
-// threads' elements are looked at again.
-template <class T>
-__device__ __forceinline__ int largest(const T* x, int begin, int end, int k, float best, int round, TopShared& sh) {
-    using P = Pieces<T, kTopThreads>;
-    constexpr int V = kVec<T>;
+// The k largest of elements begin .. end - 1 at the front of sh.keys; how many there are.  Each group's
+// largest element is known (`best`: the scan's); the k-th largest of those is a bound that the k
+// largest elements of all reach, and they lie with the k groups whose own reach it: only those
+// groups' elements are looked at again.
+template <class T, int NT>
+__device__ __forceinline__ int largest(const T* x, int begin, int end, int k, const Best<T, NT>& best, TopShared<NT>& sh) {
+    using P = Pieces<T, NT, kUnroll>;
+    using S = TopShared<NT>;
+    constexpr int V = P::V;
     const int tid = threadIdx.x;
+    const int pieces = (end - begin + P::STRIDE - 1) / P::STRIDE;   // of a thread
+    // threads of a group: more for short rows and few wanted, where comparing the groups costs more than
+    // looking at more elements (8192 rows of 4000, 5 of each: 256 groups 71 us, as below 41)
+    int G = NT / kGroups;
+    while (NT / G > 64 && NT / G >= 4 * k && (int64_t)k * pieces * 2 * G <= NT) G *= 2;
     u64 mine = 0;
-    // the first element of its round with that value
-    const int at = begin + tid * V + round * (kTopThreads * P::N);
-    if (at < end) {
-        float v[P::N];
-        P::get_checked(x, at, end, v);
-#pragma unroll
-        for (int j = P::N - 1; j >= 0; --j) {
-            const int index = at + j / V * P::STRIDE + j % V;
-            // (NaN alone: the first there is)
-            if (index < end && (v[j] == best || (j == 0 && mine == 0))) mine = key_of(v[j], index);
+    const int at = begin + tid * V + best.round * P::ROUND;
+    if (end - begin < V) {
+        for (int i = begin; tid == 0 && i < end; ++i) {
+            const u64 key = key_of((float)x[i], i);
+            mine = key > mine ? key : mine;
         }
+    } else if (at < end) {
+        // the first element of its round with that value (NaN alone: the first there is)
+#pragma unroll
+        for (int i = kUnroll - 1; i >= 0; --i) {
+            const int from = at + i * P::STRIDE, first = from < end - V ? from : end - V;
+            float v[V];
+            best.held.get(i, v);
+#pragma unroll
+            for (int j = V - 1; j >= 0; --j)
+                if (first + j >= from && v[j] == best.value) mine = key_of(v[j], first + j);
+        }
+        if (mine == 0) mine = key_of(__builtin_nanf(""), at);
     }
-    sh.best[tid] = mine;
-    if (tid == 0) sh.count = sh.chosen = 0;
+    for (int g = 1; g < G; g *= 2) {
+        const u64 other = __shfl_xor(mine, g);
+        mine = other > mine ? other : mine;
+    }
+    const int part = tid & (G - 1), groups = NT / G;
+    if (part == 0) sh.best[tid / G] = mine;
+    if (tid < kMaxTop) sh.who[tid] = -1;
+    if (tid == 0) sh.count = 0, sh.threshold = 0;
     __syncthreads();
-    if (tid < 64) {
-        const u64 t = kth_largest(sh.best, k);
-        if (tid == 0) sh.threshold = t;
+    // a group's place among them, each of its threads with a part of the comparisons
+    int place = larger_ones(sh.best + part * (groups / G), groups / G, mine);
+    for (int g = 1; g < G; g *= 2) place += __shfl_xor(place, g);
+    if (part == 0 && mine && place < k) {
+        sh.who[place] = tid;
+        if (place == k - 1) sh.threshold = mine;
     }
     __syncthreads();
-    u64 threshold = sh.threshold;
-    if (mine && mine >= threshold) {
-        const int i = atomicAdd(&sh.chosen, 1);
-        if (i < kMaxTop) sh.who[i] = tid;
-    }
-    __syncthreads();
-    const int chosen = sh.chosen < kMaxTop ? sh.chosen : kMaxTop;
-    const int pieces = (int)(((int64_t)(end - begin) + kTopThreads * V - 1) / (kTopThreads * V));
-    const int64_t items = (int64_t)chosen * pieces;
-    for (int64_t first = 0; first < items; first += kTopThreads) {
-        const int count = sh.count;
-        __syncthreads();   // everybody has read the count
-        if (count > kTopBuffer - kRoundKeys) {
-            const int left = keep_largest(sh.keys, count, k);
-            if (left == k) threshold = sh.keys[k - 1] > threshold ? sh.keys[k - 1] : threshold;
-            if (tid == 0) sh.count = left;
-            __syncthreads();
+    u64 threshold = sh.threshold;   // (0 where fewer than k groups have elements)
+    const int64_t items = (int64_t)k * pieces * G;
+    for (int64_t first = 0; first < items; first += NT) {
+        if (first > 0) {
+            const int count = sh.count;
+            __syncthreads();   // everybody has read the count
+            if (count > kSpare) {
+                const int left = keep_largest<NT, S::MOST>(sh.keys, count, k);
+                if (left == k) threshold = sh.keys[k - 1] > threshold ? sh.keys[k - 1] : threshold;
+                if (tid == 0) sh.count = left;
+                __syncthreads();
+            }
         }
         const int64_t i = first + tid;
         if (i < items) {
-            const int from = begin + ((int)(i % pieces) * kTopThreads + sh.who[i / pieces]) * V, n = end - from;
+            const int q = (int)(i / G), who = sh.who[q / pieces];
+            const int from = begin + q % pieces * P::STRIDE + (who + (int)(i & (G - 1))) * V, n = who < 0 ? 0 : end - from;
             if (n > 0) {
                 float v[V];
                 load_n<V>(x + from, n, v);
@@ -273,14 +341,14 @@ __device__ __forceinline__ int largest(const T* x, int begin, int end, int k, fl
                     const u64 key = key_of(v[j], from + j);
                     if (j < n && key >= threshold) {
                         const int slot = atomicAdd(&sh.count, 1);
-                        if (slot < kTopBuffer) sh.keys[slot] = key;
+                        if (slot < S::MOST) sh.keys[slot] = key;
                     }
                 }
             }
         }
         __syncthreads();
     }
-    return keep_largest(sh.keys, sh.count < kTopBuffer ? sh.count : kTopBuffer, k);
+    return keep_largest<NT, S::MOST>(sh.keys, sh.count < S::MOST ? sh.count : S::MOST, k);
 }
 
 // ---- log probabilities --------------------------------------------------------------------------
@@ -288,7 +356,7 @@ __device__ __forceinline__ int largest(const T* x, int begin, int end, int k, fl
 struct LogprobParams {
     LogitRows r;
     const int64_t* targets;
-    float* logprob; RowStats* stats; float* entropy;
+    float* logprob; float* stats; float* entropy;
     int top; float* top_logprob; int64_t* top_index;
     int parts, length;                 // a row's parts, elements each
     Part* part; u64* keys;             // [rows][parts], [rows][parts][top]
@@ -310,30 +378,30 @@ template <class T> __device__ __forceinline__ void finish_row(const LogprobParam
     if (t >= p.r.vocab) lp = __builtin_nanf("");
     else if (t >= 0) lp = log_softmax((float)static_cast<const T*>(p.r.x)[row * p.r.ldx + t], s, p.r.inv_t);
     p.logprob[row] = lp;
-    p.stats[row] = s;
+    p.stats[row] = s.m;
+    p.stats[p.r.rows + row] = s.l;
     if (p.entropy) p.entropy[row] = entropy_of(a, s.l, p.r.inv_t);
 }
 
 // A workgroup a row, or a part of one.
-template <class T, bool ENT, bool TOP>
-__global__ __launch_bounds__(kTopThreads)
+template <class T, int NT, bool ENT, bool TOP>
+__global__ __launch_bounds__(NT)
 void logprob_kernel(LogprobParams p) {
-    __shared__ Part red[kTopThreads / 64];
-    __shared__ std::conditional_t<TOP, TopShared, char> sh;
+    __shared__ Part red[NT / 64];
+    __shared__ std::conditional_t<TOP, TopShared<NT>, char> sh;
     const int64_t row = blockIdx.x / p.parts;
     const int part = (int)(blockIdx.x % p.parts);
     const T* x = static_cast<const T*>(p.r.x) + row * p.r.ldx;
     const int begin = part * p.length;
     const int end = p.r.vocab - begin < p.length ? (int)p.r.vocab : begin + p.length;
     const float c = p.r.inv_t * kLog2e;
-    float best;
-    int round;
-    Part a = scan<T, kTopThreads, ENT, TOP>(x, begin, end, c, best, round);
-    a = join_all<ENT, kTopThreads>(a, c, red);
+    std::conditional_t<TOP, Best<T, NT>, NoBest> best;
+    Part a = scan<T, NT, ENT>(x, begin, end, c, best);
+    a = join_all<ENT, NT>(a, c, red);
     if (p.parts > 1) {
         if (threadIdx.x == 0) p.part[row * p.parts + part] = a;
         if constexpr (TOP) {
-            const int n = largest(x, begin, end, p.top, best, round, sh);
+            const int n = largest<T, NT>(x, begin, end, p.top, best, sh);
             if ((int)threadIdx.x < p.top)
                 p.keys[(row * p.parts + part) * p.top + threadIdx.x] = (int)threadIdx.x < n ? sh.keys[threadIdx.x] : 0;
         }
@@ -342,7 +410,7 @@ void logprob_kernel(LogprobParams p) {
     const RowStats s{a.m, logf(a.s)};
     if (threadIdx.x == 0) finish_row<T>(p, row, a, s);
     if constexpr (TOP) {
-        largest(x, begin, end, p.top, best, round, sh);
+        largest<T, NT>(x, begin, end, p.top, best, sh);
         if ((int)threadIdx.x < p.top) {
             const u64 key = sh.keys[threadIdx.x];
             p.top_logprob[row * p.top + threadIdx.x] = log_softmax(key_value(key), s, p.r.inv_t);
@@ -351,28 +419,30 @@ void logprob_kernel(LogprobParams p) {
     }
 }
 
+constexpr int kJoinThreads = 256, kJoinKeys = 1024;   // (logprob_plan: parts * top is no more)
+
 // A row's parts together.
 template <class T, bool ENT, bool TOP>
-__global__ __launch_bounds__(kTopThreads)
+__global__ __launch_bounds__(kJoinThreads)
 void logprob_join_kernel(LogprobParams p) {
-    __shared__ Part red[kTopThreads / 64];
-    __shared__ u64 keys[TOP ? kTopBuffer : 1];
+    __shared__ Part red[kJoinThreads / 64];
+    __shared__ __attribute__((aligned(16))) u64 keys[TOP ? kJoinKeys : 1];
     const int64_t row = blockIdx.x;
     const float c = p.r.inv_t * kLog2e;
     Part a{kLowest, 0.0f, 0.0f};
-    for (int i = threadIdx.x; i < p.parts; i += kTopThreads) a = join<ENT>(a, p.part[row * p.parts + i], c);
-    a = join_all<ENT, kTopThreads>(a, c, red);
+    for (int i = threadIdx.x; i < p.parts; i += kJoinThreads) a = join<ENT>(a, p.part[row * p.parts + i], c);
+    a = join_all<ENT, kJoinThreads>(a, c, red);
     const RowStats s{a.m, logf(a.s)};
     if (threadIdx.x == 0) finish_row<T>(p, row, a, s);
     if constexpr (TOP) {
-        const int count = p.parts * p.top;   // at most kTopBuffer
-        for (int i = threadIdx.x; i < count; i += kTopThreads) keys[i] = p.keys[row * count + i];
+        const int count = p.parts * p.top;
+        for (int i = threadIdx.x; i < count; i += kJoinThreads) keys[i] = p.keys[row * count + i];
         __syncthreads();
         // (parts of fewer elements than `top` leave zeros, which are below every key)
-        for (int i = threadIdx.x; i < count; i += kTopThreads)
+        for (int i = threadIdx.x; i < count; i += kJoinThreads)
             if (keys[i] == 0) keys[i] = i;   // small, and all different
         __syncthreads();
-        keep_largest(keys, count, p.top);
+        keep_largest<kJoinThreads, kJoinKeys>(keys, count, p.top);
         if ((int)threadIdx.x < p.top) {
             const u64 key = keys[threadIdx.x];
             p.top_logprob[row * p.top + threadIdx.x] = log_softmax(key_value(key), s, p.r.inv_t);
@@ -385,9 +455,9 @@ void logprob_join_kernel(LogprobParams p) {
 constexpr int kBackwardThreads = 256;
 template <class T> constexpr int kBackward = kBackwardThreads * kUnroll * kVec<T>;
 
-template <class T>
+template <class T, bool STREAM>
 __global__ __launch_bounds__(kBackwardThreads)
-void logprob_backward_kernel(LogitRows r, const int64_t* __restrict__ targets, const RowStats* __restrict__ stats,
+void logprob_backward_kernel(LogitRows r, const int64_t* __restrict__ targets, const float* __restrict__ stats,
                              const float* __restrict__ g_lp, const float* __restrict__ entropy,
                              const float* __restrict__ g_h, T* grad, int64_t ldg, int parts) {
     constexpr int V = kVec<T>;
@@ -395,7 +465,7 @@ void logprob_backward_kernel(LogitRows r, const int64_t* __restrict__ targets, c
     const int64_t first = (int64_t)(blockIdx.x % parts) * kBackward<T>;
     const T* x = static_cast<const T*>(r.x) + row * r.ldx;
     T* out = grad + row * ldg;
-    const RowStats s = stats[row];
+    const RowStats s{stats[row], stats[r.rows + row]};
     const int64_t t = targets[row];
     float g = g_lp ? g_lp[row] : 0.0f;
     if (t < 0) g = 0.0f;
@@ -404,33 +474,55 @@ void logprob_backward_kernel(LogitRows r, const int64_t* __restrict__ targets, c
     // -g p - h p (l + H) = -p (h l + (h H + g))
     const float hs = h * r.inv_t, gs = g * r.inv_t, both = h != 0.0f ? (h * entropy[row] + g) * r.inv_t : gs;
     const bool none = (g == 0.0f && h == 0.0f) || s.l == -__builtin_inff();
+    auto gradient = [&](float (&v)[V], int64_t at) {
+        if (none) {
 #pragma unroll
-    for (int i = 0; i < kUnroll; ++i) {
-        const int64_t at = first + ((int64_t)i * kBackwardThreads + threadIdx.x) * V;
-        const int64_t left = r.vocab - at;
-        const int n = left < 0 ? 0 : left > V ? V : (int)left;
-        if (n == 0) break;
-        float v[V] = {};
-        if (!none) {
-            load_n<V>(x + at, n, v);
-#pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float l = (v[j] - s.m) * r.inv_t - s.l, p = __builtin_amdgcn_exp2f(l * kLog2e);
-                v[j] = -p * (hs * fmaxf(l, kFar) + both);
-            }
-            if (t >= at && t < at + V) {
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (t == at + j) v[j] += gs;
-            }
+            for (int j = 0; j < V; ++j) v[j] = 0.0f;
+            return;
         }
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+            const float l = (v[j] - s.m) * r.inv_t - s.l, p = __builtin_amdgcn_exp2f(l * kLog2e);
+            v[j] = -p * (hs * fmaxf(l, kFar) + both);
+        }
+        if (t >= at && t < at + V) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (t == at + j) v[j] += gs;
+        }
+    };
+    const int64_t at0 = first + (int64_t)threadIdx.x * V;
+    constexpr int64_t STRIDE = (int64_t)kBackwardThreads * V;
+    if (at0 + (kUnroll - 1) * STRIDE + V <= r.vocab) {
+        u32x4 u[kUnroll];
+        if (!none) {   // (a row without a gradient is not read)
+#pragma unroll
+            for (int i = 0; i < kUnroll; ++i) u[i] = load_piece<STREAM>(x + at0 + i * STRIDE);
+        }
+#pragma unroll
+        for (int i = 0; i < kUnroll; ++i) {
+            T e[V];
+            float v[V];
+            __builtin_memcpy(e, &u[i], 16);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = (float)e[j];
+            gradient(v, at0 + i * STRIDE);
+            store_piece<STREAM>(out + at0 + i * STRIDE, v);
+        }
+        return;
+    }
+    for (int64_t at = at0; at < r.vocab && at < first + kBackward<T>; at += STRIDE) {
+        const int n = r.vocab - at < V ? (int)(r.vocab - at) : V;
+        float v[V] = {};
+        if (!none) load_n<V>(x + at, n, v);
+        gradient(v, at);
         store_n<V>(out + at, n, v);
     }
 }
 
 // ---- distillation ---------------------------------------------------------------------------------
 
-constexpr int kDistillThreads = 1024;
+constexpr int kDistillThreads = 512;   // of a row's parts
 
 struct DistillParams {
     DistillArgs a;
@@ -502,58 +594,92 @@ __device__ __forceinline__ bool entries_loss(const DistillArgs& a, int64_t row, 
     return sum != 0.0f;
 }
 
-// The gradient of elements begin .. end - 1; all threads call it, with the row's entries in LDS.
-template <class T, int NT>
-__device__ __forceinline__ void distill_grad(const DistillArgs& a, int64_t row, int begin, int end, RowStats s,
-                                             bool some, float loss, const Entries& e) {
-    constexpr int V = kVec<T>;
-    const T* x = static_cast<const T*>(a.r.x) + row * a.r.ldx;
-    T* out = static_cast<T*>(a.grad) + row * a.ldg;
+// What a row's gradient needs: 0 everywhere (none), else f (exp(l) - q).
+struct GradRow { RowStats s; float f, inv_t; bool none; };
+
+__device__ __forceinline__ GradRow grad_row(const DistillArgs& a, int64_t row, RowStats s, bool some, float loss) {
     const float w = a.weight[row];
-    const bool none = !some || w == 0.0f || s.l == -__builtin_inff();
     // (an index past the vocabulary shows in every element)
-    const float f = loss != loss ? loss : w * a.r.inv_t;
-    for (int at = begin + (int)threadIdx.x * V; at < end; at += NT * V) {
-        const int n = end - at;
-        float v[V] = {};
-        if (!none) {
-            load_n<V>(x + at, n, v);
+    return {s, loss != loss ? loss : w * a.r.inv_t, a.r.inv_t, !some || w == 0.0f || s.l == -__builtin_inff()};
+}
+
+template <int V> __device__ __forceinline__ void grad_values(const GradRow& g, float (&v)[V]) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = f * __builtin_amdgcn_exp2f(((v[j] - s.m) * a.r.inv_t - s.l) * kLog2e);
-        }
-        store_n<V>(out + at, n, v);
-    }
-    if (none) return;
-    __syncthreads();   // the entries' places are written above and once more below
+    for (int j = 0; j < V; ++j)
+        v[j] = g.none ? 0.0f : g.f * __builtin_amdgcn_exp2f(((v[j] - g.s.m) * g.inv_t - g.s.l) * kLog2e);
+}
+
+// Once the rest of the row is written, its entries that lie in begin .. end - 1, once more.
+template <class T, int NT>
+__device__ __forceinline__ void grad_entries(const DistillArgs& a, T* out, int begin, int end, const GradRow& g, const Entries& e) {
+    if (g.none) return;
+    __syncthreads();
     for (int k = threadIdx.x; k < a.count; k += NT) {
         const int i = e.index[k];
         if (i < begin || i >= end) continue;
         float q = 0.0f;   // of all entries of this index: each of them stores the same
         for (int j = 0; j < a.count; ++j) q += e.index[j] == i ? e.q[j] : 0.0f;
-        out[i] = (T)(f * (__builtin_amdgcn_exp2f(((e.x[k] - s.m) * a.r.inv_t - s.l) * kLog2e) - q));
+        out[i] = (T)(g.f * (__builtin_amdgcn_exp2f(((e.x[k] - g.s.m) * g.inv_t - g.s.l) * kLog2e) - q));
     }
 }
 
-// A workgroup a row: sums, entries, and the gradient, for which the row is read again.
-template <class T, bool GRAD>
-__global__ __launch_bounds__(kDistillThreads)
-void distill_kernel(DistillParams p) {
-    constexpr int NT = kDistillThreads;
-    __shared__ Part red[NT / 64];
-    __shared__ float redf[NT / 64];
-    __shared__ Entries e;
-    const DistillArgs& a = p.a;
-    const int64_t row = blockIdx.x;
+// The gradient of elements begin .. end - 1, which are read again; all threads call it, with the row's entries
+// in LDS.
+template <class T, int NT, bool STREAM>
+__device__ __forceinline__ void distill_grad(const DistillArgs& a, int64_t row, int begin, int end, const GradRow& g, const Entries& e) {
+    constexpr int V = kVec<T>, U = kUnroll;
     const T* x = static_cast<const T*>(a.r.x) + row * a.r.ldx;
-    const float c = a.r.inv_t * kLog2e;
+    T* out = static_cast<T*>(a.grad) + row * a.ldg;
+    int at = begin + (int)threadIdx.x * V;
+    for (; at + ((U - 1) * NT + 1) * V <= end; at += U * NT * V) {
+        u32x4 u[U];
+#pragma unroll
+        for (int i = 0; i < U; ++i) u[i] = load_piece<STREAM>(x + at + i * NT * V);
+#pragma unroll
+        for (int i = 0; i < U; ++i) {
+            T t[V];
+            float v[V];
+            __builtin_memcpy(t, &u[i], 16);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[j] = (float)t[j];
+            grad_values(g, v);
+            store_piece<STREAM>(out + at + i * NT * V, v);
+        }
+    }
+    for (; at < end; at += NT * V) {
+        const int n = end - at;
+        float v[V] = {};
+        if (!g.none) load_n<V>(x + at, n, v);
+        grad_values(g, v);
+        store_n<V>(out + at, n, v);
+    }
+    grad_entries<T, NT>(a, out, begin, end, g, e);
+}
+
+// The indices of a row's entries, and the logits there.
+template <class T, int NT>
+__device__ __forceinline__ void load_entries(const DistillArgs& a, int64_t row, const T* x, Entries& e) {
     for (int k = threadIdx.x; k < a.count; k += NT) {
         const int i = entry_index(a, row, k);
         e.index[k] = i;
         e.x[k] = i >= 0 && i < a.r.vocab ? (float)x[i] : 0.0f;
     }
-    float best;
-    int round;
-    Part s = scan<T, NT, false, false>(x, 0, (int)a.r.vocab, c, best, round);
+}
+
+// A workgroup a row: sums, entries, and the gradient, for which the row is read again (most of it out of
+// the caches).
+template <class T, int NT, bool GRAD, bool STREAM>
+__global__ __launch_bounds__(NT)
+void distill_kernel(DistillArgs a) {
+    __shared__ Part red[NT / 64];
+    __shared__ float redf[NT / 64];
+    __shared__ Entries e;
+    const int64_t row = blockIdx.x;
+    const T* x = static_cast<const T*>(a.r.x) + row * a.r.ldx;
+    const float c = a.r.inv_t * kLog2e;
+    load_entries<T, NT>(a, row, x, e);
+    NoBest none;
+    Part s = scan<T, NT, false>(x, 0, (int)a.r.vocab, c, none);
     s = join_all<false, NT>(s, c, red);
     const RowStats st{s.m, logf(s.s)};
     float loss;
@@ -561,7 +687,7 @@ void distill_kernel(DistillParams p) {
     if (threadIdx.x == 0) a.loss[row] = loss;
     if constexpr (GRAD) {
         __syncthreads();
-        distill_grad<T, NT>(a, row, 0, (int)a.r.vocab, st, some, loss, e);
+        distill_grad<T, NT, STREAM>(a, row, 0, (int)a.r.vocab, grad_row(a, row, st, some, loss), e);
     }
 }
 
@@ -583,9 +709,8 @@ void distill_part_kernel(DistillParams p) {
         if (i >= begin && i < end) p.found[row * a.count + k] = (float)x[i];
     }
     const float c = a.r.inv_t * kLog2e;
-    float best;
-    int round;
-    Part s = scan<T, NT, false, false>(x, begin, end, c, best, round);
+    NoBest none;
+    Part s = scan<T, NT, false>(x, begin, end, c, none);
     s = join_all<false, NT>(s, c, red);
     if (threadIdx.x == 0) p.part[row * p.parts + part] = s;
 }
@@ -619,7 +744,7 @@ void distill_join_kernel(DistillParams p) {
         const int begin = part * p.length;
         const int end = a.r.vocab - begin < p.length ? (int)a.r.vocab : begin + p.length;
         __syncthreads();
-        distill_grad<T, NT>(a, row, begin, end, st, some, loss, e);
+        distill_grad<T, NT, false>(a, row, begin, end, grad_row(a, row, st, some, loss), e);
     }
 }
 
@@ -638,23 +763,39 @@ Cut cut_of(int64_t rows, int64_t vocab, int64_t groups, int64_t least, int64_t m
     return {(int)ceil_div(vocab, length), (int)length};
 }
 
-Cut logprob_cut(int64_t rows, int64_t vocab, int top) {
-    return cut_of(rows, vocab, 1024, 4096, top > 0 ? 1024 / top : 256);
+struct LogprobPlan { Cut cut; int threads; };
+
+LogprobPlan logprob_plan(int64_t rows, int64_t vocab, int top) {
+    Cut c{1, (int)vocab};
+    if (rows < 128 && vocab > 65536) c = cut_of(rows, vocab, 512, 16384, top > 0 ? kJoinKeys / top : 256);
+    if (rows < 512) return {c, 512};
+    return {c, top == 0 && vocab > 40000 ? 1024 : 256};
 }
-Cut distill_cut(int64_t rows, int64_t vocab) { return cut_of(rows, vocab, 256, 8192, 256); }
+struct DistillPlan { Cut cut; int threads; };
+
+DistillPlan distill_plan(int64_t rows, int64_t vocab, int dtype) {
+    if (rows < 128 && vocab > 65536) return {cut_of(rows, vocab, 512, 16384, 256), kDistillThreads};
+    const int64_t bytes = vocab * (dtype == CDX_DTYPE_F32 ? 4 : 2);
+    return {{1, (int)vocab}, rows < 512 ? 512 : bytes >= 128000 ? 1024 : bytes >= 48000 ? 512 : 256};
+}
 
 size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 template <class T>
-int run_logprob(const LogprobParams& p, hipStream_t stream) {
+int run_logprob(const LogprobParams& p, int threads, hipStream_t stream) {
     const int64_t groups = p.r.rows * p.parts;
-    if (!grid_fits(groups, kTopThreads)) return set_error(CDX_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+    if (!grid_fits(groups, 1024)) return set_error(CDX_ERR_UNSUPPORTED, "token_logprobs: too many rows");
     auto go = [&](auto ent, auto top) {
         constexpr bool ENT = decltype(ent)::value, TOP = decltype(top)::value;
-        hipLaunchKernelGGL((logprob_kernel<T, ENT, TOP>), dim3((unsigned)groups), dim3(kTopThreads), 0, stream, p);
+        if (threads == 1024)
+            hipLaunchKernelGGL((logprob_kernel<T, 1024, ENT, TOP>), dim3((unsigned)groups), dim3(1024), 0, stream, p);
+        else if (threads == 512)
+            hipLaunchKernelGGL((logprob_kernel<T, 512, ENT, TOP>), dim3((unsigned)groups), dim3(512), 0, stream, p);
+        else
+            hipLaunchKernelGGL((logprob_kernel<T, 256, ENT, TOP>), dim3((unsigned)groups), dim3(256), 0, stream, p);
         int st = hip_error(hipGetLastError(), "logprob_kernel launch");
         if (st || p.parts == 1) return st;
-        hipLaunchKernelGGL((logprob_join_kernel<T, ENT, TOP>), dim3((unsigned)p.r.rows), dim3(kTopThreads), 0, stream, p);
+        hipLaunchKernelGGL((logprob_join_kernel<T, ENT, TOP>), dim3((unsigned)p.r.rows), dim3(kJoinThreads), 0, stream, p);
         return hip_error(hipGetLastError(), "logprob_join_kernel launch");
     };
     std::true_type yes;
@@ -663,31 +804,68 @@ int run_logprob(const LogprobParams& p, hipStream_t stream) {
     return p.top ? go(no, yes) : go(no, no);
 }
 
+template <class T>
+int run_distill(const DistillParams& p, const DistillPlan& pl, hipStream_t stream) {
+    const DistillArgs& a = p.a;
+    const dim3 rows((unsigned)a.r.rows), all((unsigned)(a.r.rows * p.parts)), threads(kDistillThreads);
+    if (p.parts == 1) {
+        auto go = [&](auto threads, auto grad, auto stream_past) {
+            constexpr int NT = decltype(threads)::value;
+            hipLaunchKernelGGL((distill_kernel<T, NT, decltype(grad)::value, decltype(stream_past)::value>), rows, dim3(NT), 0, stream, a);
+        };
+        const bool past = streams(a.r.rows, a.r.vocab, a.r.dtype);
+        auto kind = [&](auto threads) {
+            if (!a.weight) go(threads, std::false_type{}, std::false_type{});
+            else if (past) go(threads, std::true_type{}, std::true_type{});
+            else go(threads, std::true_type{}, std::false_type{});
+        };
+        if (pl.threads == 1024) kind(std::integral_constant<int, 1024>{});
+        else if (pl.threads == 512) kind(std::integral_constant<int, 512>{});
+        else kind(std::integral_constant<int, 256>{});
+        return hip_error(hipGetLastError(), "distill_kernel launch");
+    }
+    hipLaunchKernelGGL(distill_part_kernel<T>, all, threads, 0, stream, p);
+    const int st = hip_error(hipGetLastError(), "distill_part_kernel launch");
+    if (st) return st;
+    if (a.weight) hipLaunchKernelGGL((distill_join_kernel<T, true>), all, threads, 0, stream, p);
+    else hipLaunchKernelGGL((distill_join_kernel<T, false>), rows, threads, 0, stream, p);
+    return hip_error(hipGetLastError(), "distill_join_kernel launch");
+}
+
+int launch_distill_plan(const DistillArgs& a, const DistillPlan& pl, void* ws, hipStream_t stream) {
+    DistillParams p{a, pl.cut.parts, pl.cut.length, static_cast<Part*>(ws), nullptr};
+    if (!grid_fits(a.r.rows * p.parts, 1024)) return set_error(CDX_ERR_UNSUPPORTED, "distill_loss: too many rows");
+    if (p.parts > 1)
+        p.found = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + round256((size_t)a.r.rows * p.parts * sizeof(Part)));
+    return with_dtype(a.r.dtype, [&](auto t) { return run_distill<decltype(t)>(p, pl, stream); });
+}
+
+int launch_logprob_plan(const TokenLogprobArgs& a, const LogprobPlan& pl, void* ws, hipStream_t stream) {
+    LogprobParams p{a.r, a.targets, a.logprob, a.stats, a.entropy, a.top, a.top_logprob, a.top_index, pl.cut.parts,
+                    pl.cut.length, static_cast<Part*>(ws), nullptr};
+    if (pl.cut.parts > 1)
+        p.keys = reinterpret_cast<u64*>(static_cast<uint8_t*>(ws) + round256((size_t)a.r.rows * pl.cut.parts * sizeof(Part)));
+    return with_dtype(a.r.dtype, [&](auto t) { return run_logprob<decltype(t)>(p, pl.threads, stream); });
+}
+
 }  // namespace
 
-size_t token_logprobs_workspace(int64_t rows, int64_t vocab, int dtype, int top) {
-    (void)dtype;
+size_t token_logprobs_workspace(int64_t rows, int64_t vocab, int top) {
     if (rows == 0) return 0;
-    const Cut c = logprob_cut(rows, vocab, top);
+    const Cut c = logprob_plan(rows, vocab, top).cut;
     if (c.parts == 1) return 0;
     return round256((size_t)rows * c.parts * sizeof(Part)) + (size_t)rows * c.parts * top * sizeof(u64);
 }
 
-int token_logprobs_parts(int64_t rows, int64_t vocab, int dtype, int top) {
-    (void)dtype;
-    return logprob_cut(rows, vocab, top).parts;
+int token_logprobs_parts(int64_t rows, int64_t vocab, int top) {
+    return logprob_plan(rows, vocab, top).cut.parts;
 }
 
 int launch_token_logprobs(const TokenLogprobArgs& a, void* ws, hipStream_t stream) {
-    const Cut c = logprob_cut(a.r.rows, a.r.vocab, a.top);
-    LogprobParams p{a.r, a.targets, a.logprob, a.stats, a.entropy, a.top, a.top_logprob, a.top_index, c.parts,
-                    c.length, static_cast<Part*>(ws), nullptr};
-    if (c.parts > 1)
-        p.keys = reinterpret_cast<u64*>(static_cast<uint8_t*>(ws) + round256((size_t)a.r.rows * c.parts * sizeof(Part)));
-    return with_dtype(a.r.dtype, [&](auto t) { return run_logprob<decltype(t)>(p, stream); });
+    return launch_logprob_plan(a, logprob_plan(a.r.rows, a.r.vocab, a.top), ws, stream);
 }
 
-int launch_token_logprobs_backward(const LogitRows& r, const int64_t* targets, const RowStats* stats,
+int launch_token_logprobs_backward(const LogitRows& r, const int64_t* targets, const float* stats,
                                    const float* g, const float* entropy, const float* gh, void* grad,
                                    int64_t ldg, hipStream_t stream) {
     return with_dtype(r.dtype, [&](auto t) {
@@ -695,47 +873,30 @@ int launch_token_logprobs_backward(const LogitRows& r, const int64_t* targets, c
         const int64_t parts = ceil_div(r.vocab, (int64_t)kBackward<T>);
         if (!grid_fits(r.rows * parts, kBackwardThreads))
             return set_error(CDX_ERR_UNSUPPORTED, "token_logprobs_backward: too many elements");
-        hipLaunchKernelGGL(logprob_backward_kernel<T>, dim3((unsigned)(r.rows * parts)), dim3(kBackwardThreads), 0,
-                           stream, r, targets, stats, g, entropy, gh, static_cast<T*>(grad), ldg, (int)parts);
+        const dim3 grid((unsigned)(r.rows * parts)), threads(kBackwardThreads);
+        if (streams(r.rows, r.vocab, r.dtype))
+            hipLaunchKernelGGL((logprob_backward_kernel<T, true>), grid, threads, 0, stream, r, targets, stats, g,
+                               entropy, gh, static_cast<T*>(grad), ldg, (int)parts);
+        else
+            hipLaunchKernelGGL((logprob_backward_kernel<T, false>), grid, threads, 0, stream, r, targets, stats, g,
+                               entropy, gh, static_cast<T*>(grad), ldg, (int)parts);
         return hip_error(hipGetLastError(), "logprob_backward_kernel launch");
     });
 }
 
-size_t distill_workspace(int64_t rows, int64_t vocab, int dtype, int count, bool grad) {
-    (void)dtype; (void)grad;
+size_t distill_workspace(int64_t rows, int64_t vocab, int dtype, int count) {
     if (rows == 0) return 0;
-    const Cut c = distill_cut(rows, vocab);
+    const Cut c = distill_plan(rows, vocab, dtype).cut;
     if (c.parts == 1) return 0;
     return round256((size_t)rows * c.parts * sizeof(Part)) + (size_t)rows * count * sizeof(float);
 }
 
-int distill_parts(int64_t rows, int64_t vocab, int dtype, bool grad) {
-    (void)dtype; (void)grad;
-    return distill_cut(rows, vocab).parts;
+int distill_parts(int64_t rows, int64_t vocab, int dtype) {
+    return distill_plan(rows, vocab, dtype).cut.parts;
 }
 
 int launch_distill(const DistillArgs& a, void* ws, hipStream_t stream) {
-    const Cut c = distill_cut(a.r.rows, a.r.vocab);
-    DistillParams p{a, c.parts, c.length, static_cast<Part*>(ws), nullptr};
-    const int64_t groups = a.r.rows * c.parts;
-    if (!grid_fits(groups, kDistillThreads)) return set_error(CDX_ERR_UNSUPPORTED, "distill_loss: too many rows");
-    const dim3 rows((unsigned)a.r.rows), all((unsigned)groups), threads(kDistillThreads);
-    if (c.parts > 1)
-        p.found = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + round256((size_t)a.r.rows * c.parts * sizeof(Part)));
-    return with_dtype(a.r.dtype, [&](auto t) {
-        using T = decltype(t);
-        if (c.parts == 1) {
-            if (a.weight) hipLaunchKernelGGL((distill_kernel<T, true>), rows, threads, 0, stream, p);
-            else hipLaunchKernelGGL((distill_kernel<T, false>), rows, threads, 0, stream, p);
-            return hip_error(hipGetLastError(), "distill_kernel launch");
-        }
-        hipLaunchKernelGGL(distill_part_kernel<T>, all, threads, 0, stream, p);
-        const int st = hip_error(hipGetLastError(), "distill_part_kernel launch");
-        if (st) return st;
-        if (a.weight) hipLaunchKernelGGL((distill_join_kernel<T, true>), all, threads, 0, stream, p);
-        else hipLaunchKernelGGL((distill_join_kernel<T, false>), rows, threads, 0, stream, p);
-        return hip_error(hipGetLastError(), "distill_join_kernel launch");
-    });
+    return launch_distill_plan(a, distill_plan(a.r.rows, a.r.vocab, a.r.dtype), ws, stream);
 }
 
 }  // namespace cdx

@@ -23,16 +23,16 @@ struct RowStats { float m, l; };
 struct TokenLogprobArgs {
     LogitRows r;
     const int64_t* targets;
-    float* logprob; RowStats* stats;
+    float* logprob; float* stats;        // stats: m of all rows, then L
     float* entropy;                    // may be null
     int top; float* top_logprob; int64_t* top_index;
 };
-size_t token_logprobs_workspace(int64_t rows, int64_t vocab, int dtype, int top);
+size_t token_logprobs_workspace(int64_t rows, int64_t vocab, int top);
 int launch_token_logprobs(const TokenLogprobArgs& a, void* ws, hipStream_t stream);
 
 // grad: may be the logits' own place.  g (null: none): the log probabilities' gradients; gh (null: none):
 // the entropies'.
-int launch_token_logprobs_backward(const LogitRows& r, const int64_t* targets, const RowStats* stats,
+int launch_token_logprobs_backward(const LogitRows& r, const int64_t* targets, const float* stats,
                                    const float* g, const float* entropy, const float* gh, void* grad,
                                    int64_t ldg, hipStream_t stream);
 
@@ -45,11 +45,11 @@ struct DistillArgs {
     const float* weight;               // null: no gradient
     void* grad; int64_t ldg;
 };
-size_t distill_workspace(int64_t rows, int64_t vocab, int dtype, int count, bool grad);
+size_t distill_workspace(int64_t rows, int64_t vocab, int dtype, int count);
 int launch_distill(const DistillArgs& a, void* ws, hipStream_t stream);
 
 // How many workgroups share a row (for tests that aim at one way or the other).
-int token_logprobs_parts(int64_t rows, int64_t vocab, int dtype, int top);
-int distill_parts(int64_t rows, int64_t vocab, int dtype, bool grad);
+int token_logprobs_parts(int64_t rows, int64_t vocab, int top);
+int distill_parts(int64_t rows, int64_t vocab, int dtype);
 
 }  // namespace cdx

@@ -1111,7 +1111,8 @@ def linear16_backward_workspace_bytes(M: int, N: int, K: int, epilogue=L.EPI_NON
 
 class TokenLogprobs(NamedTuple):
     """What token_logprobs returns, float32 [rows] each but for the alternatives ([rows, top]; index
-    int64) and `stats` [rows, 2], which the backward pass takes."""
+    int64) and `stats` (the largest logit of each row, then the logarithm of its sum, then what the
+    other fields show), which the backward pass takes."""
     logprob: torch.Tensor
     stats: torch.Tensor
     entropy: torch.Tensor | None = None
@@ -1127,11 +1128,15 @@ def _logits(logits):
     return code, rows, vocab, ld
 
 
-def _per_row(t, name, rows, dtype, like):
-    """Pointer of a checked contiguous vector of a value a row."""
+def _same_device(t, name, dtype, like):
     _need(t, name, dtype)
     if t.device != like.device:
         raise ValueError(f"{name} is on {t.device}, not on {like.device}")
+
+
+def _per_row(t, name, rows, dtype, like):
+    """Pointer of a checked contiguous vector of a value a row."""
+    _same_device(t, name, dtype, like)
     if t.numel() != rows or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous tensor of {rows} elements")
     return t.data_ptr()
@@ -1156,13 +1161,15 @@ def token_logprobs(logits, targets, *, temperature=1.0, entropy=False, top=0, wo
     code, rows, vocab, ld = _logits(logits)
     tptr = _per_row(targets, "targets", rows, torch.int64, logits)
     dev = logits.device
-    lp = torch.empty((rows,), dtype=torch.float32, device=dev)
-    stats = torch.empty((rows, 2), dtype=torch.float32, device=dev)
-    h = torch.empty_like(lp) if entropy else None
+    # one tensor seen as its rows: half the time of one a result
+    stats = logits.new_empty((4 if entropy else 3, rows), dtype=torch.float32)
+    parts = stats.unbind()
+    lp = parts[2]
+    h = parts[3] if entropy else None
     tl = ti = None
     if top:
-        tl = torch.empty((rows, top), dtype=torch.float32, device=dev)
-        ti = torch.empty((rows, top), dtype=torch.int64, device=dev)
+        tl = logits.new_empty((rows, top), dtype=torch.float32)
+        ti = targets.new_empty((rows, top))
     ws_ptr, ws_bytes, _keep = _workspace(
         workspace, lambda: L.lib().cdx_token_logprobs_workspace_size(rows, vocab, top), dev)
     L.call("cdx_token_logprobs", logits.data_ptr(), ld, rows, vocab, code, temperature, tptr, lp.data_ptr(),
@@ -1182,7 +1189,9 @@ def token_logprobs_backward(grad_logprob, logits, targets, stats, *, entropy=Non
     are 0 become zeros whatever they hold.  `out` may be the logits themselves."""
     code, rows, vocab, ld = _logits(logits)
     tptr = _per_row(targets, "targets", rows, torch.int64, logits)
-    sptr = _per_row(stats, "stats", 2 * rows, torch.float32, logits)
+    _same_device(stats, "stats", torch.float32, logits)
+    if stats.dim() != 2 or stats.shape[0] < 2 or stats.shape[1] != rows or not stats.is_contiguous():
+        raise ValueError("stats must be what token_logprobs returned")
     gptr = hptr = eptr = None
     if grad_logprob is not None:
         gptr = _per_row(grad_logprob, "grad_logprob", rows, torch.float32, logits)
@@ -1193,7 +1202,7 @@ def token_logprobs_backward(grad_logprob, logits, targets, stats, *, entropy=Non
         eptr = _per_row(entropy, "entropy", rows, torch.float32, logits)
     grad, ldg = _grad_like(out, logits, ld)
     L.call("cdx_token_logprobs_backward", gptr, logits.data_ptr(), ld, rows, vocab, code, temperature, tptr,
-           sptr, eptr, hptr, grad.data_ptr(), ldg, _stream())
+           stats.data_ptr(), eptr, hptr, grad.data_ptr(), ldg, _stream())
     return grad
 
 
@@ -1217,7 +1226,7 @@ def distill_loss(logits, index, teacher, *, temperature=1.0, weight=None, out=No
     trows, tcount, ldt = _rows(teacher, "teacher")
     if irows != rows or trows != rows or count != tcount:
         raise ValueError(f"index and teacher must be [{rows}, count]")
-    loss = torch.empty((rows,), dtype=torch.float32, device=logits.device)
+    loss = logits.new_empty((rows,), dtype=torch.float32)
     grad, gptr, ldg, wptr = None, None, vocab, None
     if weight is not None:
         wptr = _per_row(weight, "weight", rows, torch.float32, logits)

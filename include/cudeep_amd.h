@@ -648,7 +648,7 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
  * l = (x - m) / T - L.  Sums are fp32, in a fixed order: the same bits every time.
  *
  *   logprob[r] = l at targets[r] (0 for a negative target, NaN for one past the vocabulary),
- *   stats[r] = {m, L} (what the backward pass reads),
+ *   stats[r] = m, stats[rows + r] = L (what the backward pass reads),
  *   entropy[r] = -sum exp(l) l (may be NULL),
  *   top_index, top_logprob [rows][top]: the `top` (0 to 64) largest logits, the largest first and
  *     the lowest index first among equals, with their l.

@@ -233,7 +233,9 @@ def test_nan_and_infinity_stay_in_their_rows(rows):
     x[1, 77], x[3, 8999], x[5] = float("nan"), INF, float("nan")
     r = ops.token_logprobs(x, t, entropy=True, top=5)
     for a, b in zip(r, clean):
-        assert torch.equal(a[~bad], b[~bad])
+        if a is not r.stats:
+            assert torch.equal(a[~bad], b[~bad])
+    assert torch.equal(r.stats[:, ~bad], clean.stats[:, ~bad])
     assert torch.isnan(r.logprob[bad]).all() and torch.isnan(r.entropy[bad]).all() and torch.isnan(r.top_logprob[bad]).all()
     assert ((r.top_index >= 0) & (r.top_index < 9000)).all()
     dx = ops.token_logprobs_backward(g, x, t, r.stats)
@@ -493,7 +495,7 @@ def test_offsets_past_32_bits():
     idx[-3:] = _ints(0, vocab, (3, 4), 3)
     val, w = torch.randn(rows, 4, device="cuda"), torch.ones(rows, device="cuda")
     r = ops.token_logprobs(x, t, entropy=True, top=3)
-    e = _check_logprobs(x[-3:], t[-3:], 1.0, ops.TokenLogprobs(*(a[-3:] for a in r)), 3)
+    e = _check_logprobs(x[-3:], t[-3:], 1.0, ops.TokenLogprobs(r.logprob[-3:], r.stats[:, -3:], *(a[-3:] for a in r[2:])), 3)
     dx = ops.token_logprobs_backward(w, x, t, r.stats, entropy=r.entropy, grad_entropy=w)
     _check_backward(x[-3:], t[-3:], e, w[-3:], w[-3:], dx[-3:])
     loss, grad = ops.distill_loss(x, idx, val, weight=w, out=dx)
@@ -521,7 +523,8 @@ def test_refusals():
     for T in (0.0, -1.0, float("nan"), float("inf"), 1e-7, 1e7):
         refused(lambda: ops.token_logprobs(x, t, temperature=T), RuntimeError)
         refused(lambda: ops.distill_loss(x, idx, val, temperature=T), RuntimeError)
-    refused(lambda: ops.token_logprobs_backward(w, x, t, r.stats[:3]), ValueError)
+    refused(lambda: ops.token_logprobs_backward(w, x, t, r.stats[:1]), ValueError)
+    refused(lambda: ops.token_logprobs_backward(w, x, t, r.stats[:, :3]), ValueError)
     refused(lambda: ops.token_logprobs_backward(w.double(), x, t, r.stats), TypeError)
     refused(lambda: ops.token_logprobs_backward(w, x, t, r.stats, grad_entropy=w), ValueError)
     refused(lambda: ops.token_logprobs_backward(w, x, t, r.stats, out=x.half()), TypeError)

@@ -42,10 +42,10 @@ def test_token_logprobs_arguments():
     none[2] = 0
     assert _status("cdx_token_logprobs", *none) == L.CDX_OK
     small = list(good)
-    small[1] = small[3] = 100000
+    small[1] = small[3] = 1 << 21
     small[13], small[14] = _at(7), 4
     assert _status("cdx_token_logprobs", *small) == L.CDX_ERR_WORKSPACE
-    assert _status("cdx_token_logprobs_workspace_size", 1, 100000, 5) > 0
+    assert _status("cdx_token_logprobs_workspace_size", 1, 1 << 21, 5) > 0
     assert _status("cdx_token_logprobs_workspace_size", 8192, 100000, 5) == 0
     assert _status("cdx_token_logprobs_workspace_size", 1, 100000, 65) == 0
 
@@ -71,7 +71,7 @@ def test_distill_arguments():
     none[2] = 0
     assert _status("cdx_distill_loss", *none) == L.CDX_OK
     small = list(good)
-    small[1] = small[3] = small[16] = 100000
+    small[1] = small[3] = small[16] = 1 << 21
     small[17], small[18] = _at(7), 4
     assert _status("cdx_distill_loss", *small) == L.CDX_ERR_WORKSPACE
     assert _status("cdx_distill_loss_workspace_size", 8192, 100000, 5) == 0

@@ -11,6 +11,9 @@
 // would lose |m| / T 2^-24.  The running maximum begins at the lowest finite value, so that masked
 // logits (-infinity, or a type's lowest value) never meet infinity - infinity; a row of -infinity
 // alone has S = 0, and L = -infinity says so.
+//
+// Gradients of 64 MB and more are written, and their logits read for the last time, past the caches: what
+// those hold of rows that are read again stays there.
 #include "logits.hpp"
 
 namespace cdx {
@@ -24,31 +27,6 @@ constexpr float kFar = -1e30f;       // a difference so large that its exponenti
 constexpr int kUnroll = 4;           // 16-byte pieces of a thread in flight
 
 template <class T> constexpr int kVec = 16 / (int)sizeof(T);
-
-// A whole piece read for the last time, or written, past the caches (STREAM): what they hold of the rows
-// that are read again stays there.  4096 x 65536 in bf16, loss and gradient: 226 us, 247 with ordinary loads
-// and stores; 2048 x 131072 237 and 272.  Gradients that the caches can hold are left there for
-// the product that reads them (streams).
-typedef u32x4 __attribute__((aligned(1))) u32x4_any;
-template <bool STREAM> __device__ __forceinline__ u32x4 load_piece(const void* p) {
-    if constexpr (STREAM) return __builtin_nontemporal_load(static_cast<const u32x4_any*>(p));
-    else return load16(p);
-}
-template <bool STREAM, class T> __device__ __forceinline__ void store_piece(T* p, const float (&v)[kVec<T>]) {
-    if constexpr (STREAM) {
-        T e[kVec<T>];
-#pragma unroll
-        for (int j = 0; j < kVec<T>; ++j) e[j] = round_to<T>(v[j]);
-        u32x4 w;
-        __builtin_memcpy(&w, e, 16);
-        __builtin_nontemporal_store(w, reinterpret_cast<u32x4_any*>(p));
-    } else {
-        store_n<kVec<T>>(p, kVec<T>, v);
-    }
-}
-inline bool streams(int64_t rows, int64_t vocab, int dtype) {
-    return (double)rows * (double)vocab * (dtype == CDX_DTYPE_F32 ? 4 : 2) >= 256e6;
-}
 
 // The sums of some of a row's elements: m their maximum, s = sum e, t = sum e (x - m), e = exp((x - m) / T).
 struct Part { float m, s, t; };
@@ -497,7 +475,7 @@ void logprob_backward_kernel(LogitRows r, const int64_t* __restrict__ targets, c
         u32x4 u[kUnroll];
         if (!none) {   // (a row without a gradient is not read)
 #pragma unroll
-            for (int i = 0; i < kUnroll; ++i) u[i] = load_piece<STREAM>(x + at0 + i * STRIDE);
+            for (int i = 0; i < kUnroll; ++i) u[i] = load16_as<STREAM>(x + at0 + i * STRIDE);
         }
 #pragma unroll
         for (int i = 0; i < kUnroll; ++i) {
@@ -507,7 +485,7 @@ void logprob_backward_kernel(LogitRows r, const int64_t* __restrict__ targets, c
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = (float)e[j];
             gradient(v, at0 + i * STRIDE);
-            store_piece<STREAM>(out + at0 + i * STRIDE, v);
+            store16_as<STREAM, T>(out + at0 + i * STRIDE, v);
         }
         return;
     }
@@ -634,7 +612,7 @@ __device__ __forceinline__ void distill_grad(const DistillArgs& a, int64_t row, 
     for (; at + ((U - 1) * NT + 1) * V <= end; at += U * NT * V) {
         u32x4 u[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) u[i] = load_piece<STREAM>(x + at + i * NT * V);
+        for (int i = 0; i < U; ++i) u[i] = load16_as<STREAM>(x + at + i * NT * V);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             T t[V];
@@ -643,7 +621,7 @@ __device__ __forceinline__ void distill_grad(const DistillArgs& a, int64_t row, 
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = (float)t[j];
             grad_values(g, v);
-            store_piece<STREAM>(out + at + i * NT * V, v);
+            store16_as<STREAM, T>(out + at + i * NT * V, v);
         }
     }
     for (; at < end; at += NT * V) {
@@ -813,7 +791,7 @@ int run_distill(const DistillParams& p, const DistillPlan& pl, hipStream_t strea
             constexpr int NT = decltype(threads)::value;
             hipLaunchKernelGGL((distill_kernel<T, NT, decltype(grad)::value, decltype(stream_past)::value>), rows, dim3(NT), 0, stream, a);
         };
-        const bool past = streams(a.r.rows, a.r.vocab, a.r.dtype);
+        const bool past = past_caches(a.r.rows, a.r.vocab, a.r.dtype);
         auto kind = [&](auto threads) {
             if (!a.weight) go(threads, std::false_type{}, std::false_type{});
             else if (past) go(threads, std::true_type{}, std::true_type{});
@@ -874,7 +852,7 @@ int launch_token_logprobs_backward(const LogitRows& r, const int64_t* targets, c
         if (!grid_fits(r.rows * parts, kBackwardThreads))
             return set_error(CDX_ERR_UNSUPPORTED, "token_logprobs_backward: too many elements");
         const dim3 grid((unsigned)(r.rows * parts)), threads(kBackwardThreads);
-        if (streams(r.rows, r.vocab, r.dtype))
+        if (past_caches(r.rows, r.vocab, r.dtype))
             hipLaunchKernelGGL((logprob_backward_kernel<T, true>), grid, threads, 0, stream, r, targets, stats, g,
                                entropy, gh, static_cast<T*>(grad), ldg, (int)parts);
         else

@@ -102,22 +102,24 @@ Plan plan_of(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned) {
         if (!aligned || (mt <= 2 && K <= 8192 && ceil_div(tiles_m, (int64_t)mt) * tiles_n <= (M <= 16 ? 512 : 256)))
             return direct_plan(M, N, mt);
     }
-    int64_t slices = 1;
-    auto cut = [&](int64_t tiles, int64_t least) {   // slices for a workgroup a CU, of `least` k and more
-        const int64_t s = tiles > 0 ? 256 / tiles : 1;
+    // slices for about `groups` workgroups, of `least` k and more
+    auto cut = [&](int64_t tiles, int64_t groups, int64_t least) {
+        const int64_t s = groups / tiles;
         return s > K / least ? (K / least > 1 ? K / least : 1) : s > 1 ? s : 1;
     };
     // (without columns of B there is nothing to load straight into LDS)
     if (!aligned) {
-        if (N > 0) slices = cut(tiles_of(M, N, 64), 1024);
-        return make_plan(Kernel::Any, M, N, K, 64, slices);
+        if (N == 0) return make_plan(Kernel::Any, M, N, K, 64, 1);
+        const int64_t t128 = tiles_of(M, N, 128), t64 = tiles_of(M, N, 64);
+        if (t128 >= 80) return make_plan(Kernel::Any128, M, N, K, 128, t128 >= 200 ? 1 : cut(t128, 512, 384));
+        return make_plan(Kernel::Any, M, N, K, 64, t64 >= 200 ? 1 : cut(t64, 512, 384));
     }
     const int64_t t256 = tiles_of(M, N, 256), t128 = tiles_of(M, N, 128), t64 = tiles_of(M, N, 64);
     const int64_t long_k = K / 4096 < 256 ? K / 4096 : 256;
-    if (t256 >= 200 || t256 * long_k >= 256) return make_plan(Kernel::Turns, M, N, K, 256, cut(t256, 4096));
+    if (t256 >= 200 || t256 * long_k >= 256) return make_plan(Kernel::Turns, M, N, K, 256, cut(t256, 256, 4096));
     if (t128 > 256) return make_plan(Kernel::Tile128, M, N, K, 128, 1);
-    if (t128 >= 140 || t128 * long_k >= 256) return make_plan(Kernel::Ring128, M, N, K, 128, cut(t128, 4096));
-    return make_plan(Kernel::Ring64, M, N, K, 64, cut(t64, 1024));
+    if (t128 >= 140 || t128 * long_k >= 256) return make_plan(Kernel::Ring128, M, N, K, 128, cut(t128, 256, 4096));
+    return make_plan(Kernel::Ring64, M, N, K, 64, cut(t64, 256, 1024));
 }
 
 unsigned wide_grid(int64_t threads) {
@@ -175,7 +177,7 @@ size_t linear16_workspace(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bo
 
 const char* linear16_kernel_name(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned,
                                  int* slices) {
-    static const char* const names[] = {"any", "ring 64", "ring 128", "tile 128", "turns", "direct"};
+    static const char* const names[] = {"any", "any 128", "ring 64", "ring 128", "tile 128", "turns", "direct"};
     const Plan pl = plan_of(kind, M, N, K, aligned);
     *slices = pl.slices;
     return names[(int)pl.kernel];

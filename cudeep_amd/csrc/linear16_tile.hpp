@@ -387,13 +387,13 @@ struct Slice {
     }
 };
 
-// Operands of any alignment: every step through registers, the next one's loads in flight while one is
-// multiplied.
+// Operands of any alignment: every step through registers into the LDS buffer that is not being read, the
+// step after it on its way meanwhile; one barrier a step.
 template <class T, bool CA, bool CB, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN)
 void linear16_any_kernel(Params p) {
-    constexpr int NT = 64 * WM * WN;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds[(BM + BN) * 128];
+    constexpr int NT = 64 * WM * WN, SIZE = (BM + BN) * 128;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[2 * SIZE];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int64_t m0, n0;
     tile_of<BM, BN>(p, m0, n0);
@@ -403,25 +403,31 @@ void linear16_any_kernel(Params p) {
     Wave<T, CA, CB, BM, BN, WM, WN> w(p, lane, wave, n0);
     typename Loader<CA, BM, NT>::Held ha;
     typename Loader<CB, BN, NT>::Held hb;
-    if (sl.k0 < sl.k1) {
-        la.load(sl.k0, sl.k1, ha);
-        lb.load(sl.k0, sl.k1, hb);
-    }
-    for (int64_t k = sl.k0; k < sl.k1; k += kStep) {
-        __syncthreads();
-        la.store(ha, lds);
-        lb.store(hb, lds + BM * 128);
-        __syncthreads();
+    auto load = [&](int64_t k) {
+        if (k >= sl.k1) return;
+        la.load(k, sl.k1, ha);
+        lb.load(k, sl.k1, hb);
+    };
+    auto store = [&](uint8_t* buf) {
+        la.store(ha, buf);
+        lb.store(hb, buf + BM * 128);
+    };
+    load(sl.k0);
+    if (sl.k0 < sl.k1) store(lds);
+    load(sl.k0 + kStep);
+    int buf = 0;
+    for (int64_t k = sl.k0; k < sl.k1; k += kStep, buf ^= SIZE) {
+        __syncthreads();   // this step's rows are in LDS, and the last step's are read
         if (k + kStep < sl.k1) {
-            la.load(k + kStep, sl.k1, ha);
-            lb.load(k + kStep, sl.k1, hb);
+            store(lds + (buf ^ SIZE));
+            load(k + 2 * kStep);
         }
-        w.template read<0>(lds);
+        w.template read<0>(lds + buf);
         w.multiply();
-        w.template read<1>(lds);
+        w.template read<1>(lds + buf);
         w.multiply();
     }
-    constexpr int ROWS = (BM + BN) * 128 / (BN * 4) < BM ? (BM + BN) * 128 / (BN * 4) : BM;
+    constexpr int ROWS = 2 * SIZE / (BN * 4) < BM ? 2 * SIZE / (BN * 4) : BM;
     store_tile<T, !CA && !CB, BM, BN, WM, WN, ROWS>(p, lds, m0, n0, w.wm, w.wn, w.acc);
     if constexpr (w.SUMS) w.store_sums(p, m0, lane);
 }
@@ -674,7 +680,7 @@ void linear16_direct_kernel(Params p) {
 
 // ---- launches ------------------------------------------------------------------------------------
 
-enum class Kernel { Any, Ring64, Ring128, Tile128, Turns, Direct };
+enum class Kernel { Any, Any128, Ring64, Ring128, Tile128, Turns, Direct };
 struct Plan { Kernel kernel; int64_t tiles; int slices; int64_t chunk; int mt = 1; };   // mt: Direct's MT
 
 template <class F> int with_16(int dtype, F f) {
@@ -696,6 +702,9 @@ int run(const Params& p, const Plan& pl, hipStream_t stream) {
             break;
         case Kernel::Ring64:
             hipLaunchKernelGGL((linear16_tile_kernel<T, CA, CB, 64, 64, 2, 2, 4>), grid, dim3(256), 0, stream, p);
+            break;
+        case Kernel::Any128:
+            hipLaunchKernelGGL((linear16_any_kernel<T, CA, CB, 128, 128, 2, 4>), grid, dim3(512), 0, stream, p);
             break;
         case Kernel::Any:
             hipLaunchKernelGGL((linear16_any_kernel<T, CA, CB, 64, 64, 2, 2>), grid, dim3(256), 0, stream, p);

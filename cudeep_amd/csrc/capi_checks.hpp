@@ -61,6 +61,11 @@ inline int check_in_place(const char* fn, const char* what, const Span& out, con
     return bad(fn, (std::string(what) + " overlap without being the same").c_str());
 }
 
+// Scratch that holds 16-byte pieces.
+inline int check_workspace(const char* fn, const void* ws) {
+    return (uintptr_t)ws % 16 ? bad(fn, "workspace must be 16-byte aligned") : (int)CDX_OK;
+}
+
 // Runs f(scratch) with the caller's workspace or stream-ordered memory.
 template <class F>
 inline int with_workspace(const char* fn, size_t need, void* ws, size_t ws_bytes, hipStream_t stream, F f) {

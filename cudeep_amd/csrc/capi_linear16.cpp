@@ -26,6 +26,11 @@ int check_apart(const char* fn, const char* what, const Span& out, const Span& i
     return overlap(out, in) ? bad(fn, (std::string(what) + " overlap").c_str()) : (int)CDX_OK;
 }
 
+// Sizes that no checked call has (the queries come without one).
+bool no_layer(int64_t M, int64_t N, int64_t K) {
+    return bad_dim(M) || bad_dim(N) || bad_dim(K) || too_large(M, N) || too_large(M, K) || too_large(N, K);
+}
+
 // A vector's bytes as a row.
 Span vector_span(const void* p, int64_t n, int dtype) { return {p, n, 1, n, dtype}; }
 
@@ -39,7 +44,7 @@ size_t slope_bytes(int64_t M, int64_t N, int epilogue) {
 extern "C" {
 
 size_t cdx_linear16_workspace_size(int64_t M, int64_t N, int64_t K) {
-    if (bad_dim(M) || bad_dim(N) || bad_dim(K)) return 0;
+    if (no_layer(M, N, K)) return 0;
     return cdx::linear16_workspace(Linear16Kind::Forward, M, N, K, false);
 }
 
@@ -54,6 +59,7 @@ int cdx_linear16(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, co
     if (!st) st = check_matrix(fn, "y", y, ldy, M, N);
     if (!st && residual) st = check_matrix(fn, "residual", residual, ldr, M, N);
     if (!st && z) st = check_matrix(fn, "z", z, ldz, M, N);
+    if (!st) st = check_workspace(fn, workspace);
     if (st || M == 0 || N == 0) return st;
     const Span sx{x, ldx, M, K, dtype}, sw{weight, ldw, N, K, dtype}, sy{y, ldy, M, N, dtype};
     st = check_apart(fn, "y and x", sy, sx);
@@ -82,7 +88,7 @@ int cdx_linear16(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, co
 }
 
 size_t cdx_linear16_backward_workspace_size(int64_t M, int64_t N, int64_t K, int epilogue) {
-    if (bad_dim(M) || bad_dim(N) || bad_dim(K) || !gemm_epilogue(epilogue)) return 0;
+    if (no_layer(M, N, K) || !gemm_epilogue(epilogue)) return 0;
     const size_t dx = cdx::linear16_workspace(Linear16Kind::Input, M, K, N, false);
     const size_t dw = cdx::linear16_workspace(Linear16Kind::Weight, N, K, M, true);
     return slope_bytes(M, N, epilogue) + (dx > dw ? dx : dw);
@@ -101,6 +107,7 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
     if (!st && grad_x) st = check_matrix(fn, "weight", weight, ldw, N, K);
     if (!st && grad_x) st = check_matrix(fn, "grad_x", grad_x, ldgx, M, K);
     if (!st && grad_weight) st = check_matrix(fn, "grad_weight", grad_weight, K, N, K);
+    if (!st) st = check_workspace(fn, workspace);
     if (st) return st;
     if (grad_bias && !grad_weight && N > 0 && K > 0) return bad(fn, "grad_bias needs grad_weight");
     // grad_x is written first: everything that is read later has to be apart from it

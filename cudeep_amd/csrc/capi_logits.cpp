@@ -44,7 +44,8 @@ int cdx_token_logprobs(const void* logits, int64_t ldx, int64_t rows, int64_t vo
                        float* entropy, int top, float* top_logprob, int64_t* top_index,
                        void* workspace, size_t workspace_bytes, hipStream_t stream) {
     static const char fn[] = "cdx_token_logprobs";
-    const int st = check_logits(fn, logits, ldx, rows, vocab, dtype, temperature);
+    int st = check_logits(fn, logits, ldx, rows, vocab, dtype, temperature);
+    if (!st) st = check_workspace(fn, workspace);
     if (st) return st;
     if (top < 0 || top > cdx::kMaxTop || top > vocab) return bad(fn, "top must be in [0, min(64, vocab)]");
     if (rows == 0) return CDX_OK;
@@ -83,6 +84,7 @@ int cdx_distill_loss(const void* logits, int64_t ldx, int64_t rows, int64_t voca
                      size_t workspace_bytes, hipStream_t stream) {
     static const char fn[] = "cdx_distill_loss";
     int st = check_logits(fn, logits, ldx, rows, vocab, dtype, temperature);
+    if (!st) st = check_workspace(fn, workspace);
     if (st) return st;
     if (count < 0 || count > cdx::kMaxEntries) return bad(fn, "count must be in [0, 1024]");
     if (index_bytes != 4 && index_bytes != 8) return bad(fn, "index_bytes must be 4 or 8");

@@ -762,7 +762,7 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 template <class T>
 int run_logprob(const LogprobParams& p, int threads, hipStream_t stream) {
     const int64_t groups = p.r.rows * p.parts;
-    if (!grid_fits(groups, 1024)) return set_error(CDX_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+    if (!grid_fits(groups, threads)) return set_error(CDX_ERR_UNSUPPORTED, "token_logprobs: too many rows");
     auto go = [&](auto ent, auto top) {
         constexpr bool ENT = decltype(ent)::value, TOP = decltype(top)::value;
         if (threads == 1024)
@@ -812,7 +812,7 @@ int run_distill(const DistillParams& p, const DistillPlan& pl, hipStream_t strea
 
 int launch_distill_plan(const DistillArgs& a, const DistillPlan& pl, void* ws, hipStream_t stream) {
     DistillParams p{a, pl.cut.parts, pl.cut.length, static_cast<Part*>(ws), nullptr};
-    if (!grid_fits(a.r.rows * p.parts, 1024)) return set_error(CDX_ERR_UNSUPPORTED, "distill_loss: too many rows");
+    if (!grid_fits(a.r.rows * p.parts, pl.threads)) return set_error(CDX_ERR_UNSUPPORTED, "distill_loss: too many rows");
     if (p.parts > 1)
         p.found = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + round256((size_t)a.r.rows * p.parts * sizeof(Part)));
     return with_dtype(a.r.dtype, [&](auto t) { return run_distill<decltype(t)>(p, pl, stream); });

@@ -615,9 +615,10 @@ int cdx_linear_weight_grad_e4m3(const void* dz, int64_t lddz, int dtype,
  * backward pass takes, rounded to dtype; y comes from the unrounded one) may be NULL.  epilogue:
  * CDX_EPI_NONE to _SIGMOID, with the hardware's exponential and reciprocal.  y may be
  * residual itself (the same pointer and leading dimension); y and z must not overlap anything
- * else.  workspace: the query's bytes; NULL allocates stream-ordered.  Products of more tiles
- * than a launch holds (from 2^23 of 64 x 64 on) are CDX_ERR_UNSUPPORTED.  The same bits every
- * time.  No counterpart in the reference. */
+ * else.  workspace: the query's bytes, 16-byte aligned; NULL allocates stream-ordered.  Products
+ * of more tiles than a launch holds (2^23 of 128 x 128, or of 256 x 256 where operands are
+ * aligned, and 16 columns for few rows) are CDX_ERR_UNSUPPORTED.  The same bits every time.  No
+ * counterpart in the reference. */
 size_t cdx_linear16_workspace_size(int64_t M, int64_t N, int64_t K);
 int cdx_linear16(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
                  const void* weight, int64_t ldw, const void* bias, int bias_dtype,
@@ -654,8 +655,9 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
  *     the lowest index first among equals, with their l.
  * Logits of -infinity have probability 0.  A row of -infinity alone has logprob -infinity, entropy 0 and
  * no gradient.  A NaN or +infinity makes its row's numbers NaN; top_index is then some index in the
- * vocabulary.  workspace: the query's bytes; NULL allocates stream-ordered.  No counterpart in the
- * reference. */
+ * vocabulary.  workspace: the query's bytes, 16-byte aligned; NULL allocates stream-ordered.
+ * Rows, one workgroup each, are up to 2^24 - 1, and up to 2^22 - 1 of long ones (more are
+ * CDX_ERR_UNSUPPORTED).  No counterpart in the reference. */
 size_t cdx_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top);
 int cdx_token_logprobs(const void* logits, int64_t ldx, int64_t rows, int64_t vocab, int dtype,
                        double temperature, const int64_t* targets, float* logprob, float* stats,
@@ -678,8 +680,8 @@ int cdx_token_logprobs_backward(const float* grad_logprob, const void* logits, i
  *   grad_logits[r][v] = weight[r] / T (exp(l_v) - sum of q_k with index_k = v)
  * (0 there, where weight[r] is 0, and in a row of logits that are all -infinity).  weight NULL: the loss alone, and
  * grad_logits is not written.  An index may come more than once; one past the vocabulary makes its
- * row's loss and gradient NaN.  grad_logits (dtype) may be the logits' own place.  workspace as
- * above. */
+ * row's loss and gradient NaN.  grad_logits (dtype) may be the logits' own place.  Rows and
+ * workspace as above. */
 size_t cdx_distill_loss_workspace_size(int64_t rows, int64_t vocab, int count);
 int cdx_distill_loss(const void* logits, int64_t ldx, int64_t rows, int64_t vocab, int dtype,
                      double temperature, const void* index, int64_t ldi, int index_bytes,

@@ -323,6 +323,7 @@ template <class T, bool CA, bool CB, int BM, int BN, int WM, int WN, bool IN_PLA
         ra.template read<H>(tile, fa);
     }
     __device__ __forceinline__ void multiply() {
+        if constexpr (IN_PLACE) asm volatile("s_nop 1");   // (an operand that was moved rather than read is there)
 #pragma unroll
         for (int i = 0; i < FN; ++i) {
 #pragma unroll
@@ -553,7 +554,6 @@ void linear16_turns_kernel(Params p) {
     };
     auto multiply = [&]() {
         __builtin_amdgcn_s_setprio(1);
-        asm volatile("s_nop 1");   // (an operand that was moved rather than read is there)
         w.multiply();
         __builtin_amdgcn_s_setprio(0);
     };

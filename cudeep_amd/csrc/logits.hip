@@ -23,7 +23,8 @@ using namespace b8;
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLowest = -3.4028234663852886e38f;
-constexpr float kFar = -1e30f;       // a difference so large that its exponential is 0 at any temperature
+constexpr float kFar = -1e20f;       // a difference so large that its exponential is 0 at any temperature, and
+                                     // small enough that its products with sums and gradients are finite
 constexpr int kUnroll = 4;           // 16-byte pieces of a thread in flight
 
 template <class T> constexpr int kVec = 16 / (int)sizeof(T);

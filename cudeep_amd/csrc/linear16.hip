@@ -93,33 +93,56 @@ Plan direct_plan(int64_t M, int64_t N, int mt) {
     return {Kernel::Direct, ceil_div(M, (int64_t)(16 * mt)) * ceil_div(N, (int64_t)16), 1, kStep, mt};
 }
 
+// Which kernel, and how many slices of k (all figures us, bf16, M x N x K; "input", "weight": of those
+// products, else forward).  Slices are added by a launch of their own, so that they have to save more than
+// that and their sums' traffic: 8 of 64 x 64 tiles at most (256 x 256 x 16384 14.9, 16 of them 16.9), 16 of
+// 128 x 128 (weight 256 x 512 x 65536 48, 32 of them 56).
 Plan plan_of(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned) {
-    aligned = aligned && K >= kStep && N > 0;
-    if (kind == Linear16Kind::Forward && K > 0 && M <= (aligned ? 128 : 64)) {
+    aligned = aligned && K >= kStep && N > 0;   // (a whole step, and columns of B, to load straight into LDS)
+    // Few rows, whose weights are read once: one launch with k split inside the workgroups, while these are no
+    // more than the CUs (1 x 4096 x 4096 6.6, ring 64 in 4 slices 8.6; 128 x 1024 x 1024 5.0, ring 64 5.8; but
+    // 16 x 8192 x 4096 18.9, ring 64 13.9) and k is short (1 x 2048 x 8192 12.0, ring 64 in 8 slices 9.9).
+    // Operands of any alignment, which ring 64 does not take, up to 64 rows and half that k (33 x 4096 x 1001
+    // 9.6, any in 2 slices 11.7; 64 x 4096 x 4001 50, any in 8 slices 15.6; 65 x 4096 x 1001 15.9, any 13.0).
+    if (kind == Linear16Kind::Forward && K > 0 && M <= (aligned ? 128 : 64) && K <= (aligned ? 4096 : 2048)) {
         const int64_t tiles_m = ceil_div(M, (int64_t)16), tiles_n = ceil_div(N, (int64_t)16);
-        int mt = 1;
-        while (mt < 4 && ceil_div(tiles_m, (int64_t)mt) * tiles_n > 256 && mt < tiles_m) mt *= 2;
-        if (!aligned || (mt <= 2 && K <= 8192 && ceil_div(tiles_m, (int64_t)mt) * tiles_n <= (M <= 16 ? 512 : 256)))
-            return direct_plan(M, N, mt);
+        for (int mt = 1; mt <= (aligned ? 2 : 4); mt *= 2)
+            if (ceil_div(tiles_m, (int64_t)mt) * tiles_n <= 256) return direct_plan(M, N, mt);
     }
-    // slices for about `groups` workgroups, of `least` k and more
-    auto cut = [&](int64_t tiles, int64_t groups, int64_t least) {
-        const int64_t s = groups / tiles;
-        return s > K / least ? (K / least > 1 ? K / least : 1) : s > 1 ? s : 1;
+    // slices for about `groups` workgroups, of `least` k and more, `most` of them
+    auto cut = [&](int64_t tiles, int64_t groups, int64_t least, int64_t most) {
+        int64_t s = groups / tiles;
+        if (s > K / least) s = K / least;
+        if (s > most) s = most;
+        return s > 1 ? s : 1;
     };
-    // (without columns of B there is nothing to load straight into LDS)
+    const int64_t t256 = tiles_of(M, N, 256), t128 = tiles_of(M, N, 128), t64 = tiles_of(M, N, 64);
+    const int64_t long_k = K / 2048 < 256 ? K / 2048 : 256;
+    const int64_t narrow = M < N ? M : N;       // the smaller side
     if (!aligned) {
         if (N == 0) return make_plan(Kernel::Any, M, N, K, 64, 1);
-        const int64_t t128 = tiles_of(M, N, 128), t64 = tiles_of(M, N, 64);
-        if (t128 >= 80) return make_plan(Kernel::Any128, M, N, K, 128, t128 >= 200 ? 1 : cut(t128, 512, 384));
-        return make_plan(Kernel::Any, M, N, K, 64, t64 >= 200 ? 1 : cut(t64, 512, 384));
+        // 128 x 128 tiles, where they fill more than half of the CUs or k is long enough for slices (4096 x 4096 x
+        // 4001 183, 64 x 64 318; 2048 x 1280 x 1001 17.2, 64 x 64 19.7; 1336 x 1440 x 8001 in 3 slices 78, 64 x
+        // 64 96; but 640 x 2048 x 1001 16.5, 64 x 64 13.5), and half of a tile does not lie outside (400000 x 64 x
+        // 1024 199, 64 x 64 176)
+        if (narrow > 64 && (t128 >= 140 || t128 * long_k >= 256))
+            return make_plan(Kernel::Any128, M, N, K, 128, t128 >= 200 ? 1 : cut(t128, 512, 1024, 16));
+        return make_plan(Kernel::Any, M, N, K, 64, t64 >= 200 ? 1 : cut(t64, 512, 384, 8));
     }
-    const int64_t t256 = tiles_of(M, N, 256), t128 = tiles_of(M, N, 128), t64 = tiles_of(M, N, 64);
-    const int64_t long_k = K / 4096 < 256 ? K / 4096 : 256;
-    if (t256 >= 200 || t256 * long_k >= 256) return make_plan(Kernel::Turns, M, N, K, 256, cut(t256, 256, 4096));
+    // 256 x 256, for most of the CUs (2560 x 5120 x 1024 35.6, tile 128 38.8; 2560 x 4608 x 1024 37.5, tile 128
+    // 34.0), by slices too (weight 1024 x 1024 x 65536 in 16 155, ring 128 in 4 177), where half of a tile does not
+    // lie outside (128 x 128256 x 4096 255, tile 128 206; 192 x 65536 x 2048 74, tile 128 85)
+    if (narrow > 128 && (t256 >= 200 || t256 * (long_k / 2) >= 256))
+        return make_plan(Kernel::Turns, M, N, K, 256, cut(t256, 256, 4096, 256));
+    // 128 x 128 tiles: two workgroups a CU share it where there is more than one (2048 x 2176 x 2048 32.3, ring 128
+    // 36.7; 1 x 128256 x 4096 172, turns 246), else one has four buffers (2048 x 2048 x 2048 21.2, tile 128 26.4)
     if (t128 > 256) return make_plan(Kernel::Tile128, M, N, K, 128, 1);
-    if (t128 >= 140 || t128 * long_k >= 256) return make_plan(Kernel::Ring128, M, N, K, 128, cut(t128, 256, 4096));
-    return make_plan(Kernel::Ring64, M, N, K, 64, cut(t64, 256, 1024));
+    // and 64 x 64 tiles where those leave CUs idle (1408 x 1536 x 2048, 132 tiles of 128, 21.2, ring 128 19.0; 1024 x
+    // 1536 x 2048, 96, 13.4, ring 128 18.7), unless k is long (1152 x 1152 x 8192 46, ring 128 in 3 slices 36;
+    // weight 256 x 512 x 65536 55, ring 128 in 16 slices 48; 1280 x 1280 x 4096 25.0, ring 128 in 2 slices 26.7)
+    if (t128 > 128 || t128 * long_k >= 256)
+        return make_plan(Kernel::Ring128, M, N, K, 128, cut(t128, 256, 2048, 16));
+    return make_plan(Kernel::Ring64, M, N, K, 64, cut(t64, 256, 1024, 8));
 }
 
 unsigned wide_grid(int64_t threads) {

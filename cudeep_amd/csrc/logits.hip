@@ -744,17 +744,32 @@ Cut cut_of(int64_t rows, int64_t vocab, int64_t groups, int64_t least, int64_t m
 
 struct LogprobPlan { Cut cut; int threads; };
 
-LogprobPlan logprob_plan(int64_t rows, int64_t vocab, int top) {
+int64_t row_bytes(int64_t vocab, int dtype) { return vocab * (dtype == CDX_DTYPE_F32 ? 4 : 2); }
+
+// Few long rows are cut, which a second launch joins (1 x 131072 with 5 alternatives, bf16, in 8 parts 11.6 us,
+// whole 16.5; 16 x 131072 6.2, whole 10.9; 1 x 65536 11.1 in 4, whole 11.5; 128 x 131072 17.6, whole 18.0).
+// Threads of a row: 512 while a CU has one row (1 x 65536 with 5 alternatives 11.5 us, 256 threads 16.0; 128
+// x 131072 18.0, 256 threads 20.8), else 256 (300 x 50001 10.7, 512 threads 12.7; 8192 x 4096 with 5
+// alternatives 55, 512 threads 123), and 1024 where rows are long and only their sums wanted (1024 x 50001 in
+// fp32 37.4, 256 threads 39.0; 1024 x 131072 55, 256 threads 57; but 600 x 64000 19.1, 256 threads 17.6).
+// Parts do not depend on the type, which the workspace's query does not have.
+LogprobPlan logprob_plan(int64_t rows, int64_t vocab, int top, int dtype) {
     Cut c{1, (int)vocab};
     if (rows < 128 && vocab > 65536) c = cut_of(rows, vocab, 512, 16384, top > 0 ? kJoinKeys / top : 256);
-    if (rows < 512) return {c, 512};
-    return {c, top == 0 && vocab > 40000 ? 1024 : 256};
+    if (rows < 256) return {c, 512};
+    return {c, top == 0 && row_bytes(vocab, dtype) >= 150000 ? 1024 : 256};
 }
 struct DistillPlan { Cut cut; int threads; };
 
+// The same with the gradient: parts from 65536 on (64 x 65536 with 64 entries, bf16, in 4 parts 14.0 us, whole
+// 17.5; 64 x 131072 in 8 17.1, whole 25.4; 1 x 50001 in 4 13.4, whole 14.9, and without a gradient 16 x 32000
+// in 2 8.0, whole 5.5).  Threads: a row that is read again should be in the caches still, and fewer rows are in
+// flight with more threads each, but the entries cost them the same: 256 for rows of less than 48 KB (4096 x
+// 8192, bf16, 31.9 us, 512 threads 51.9), 1024 from 128 KB on (513 x 50001 in fp32 50.9, 256 threads 54.2;
+// 2048 x 64000, bf16, 117, 512 threads 120).
 DistillPlan distill_plan(int64_t rows, int64_t vocab, int dtype) {
-    if (rows < 128 && vocab > 65536) return {cut_of(rows, vocab, 512, 16384, 256), kDistillThreads};
-    const int64_t bytes = vocab * (dtype == CDX_DTYPE_F32 ? 4 : 2);
+    if (rows < 128 && vocab >= 65536) return {cut_of(rows, vocab, 512, 16384, 256), kDistillThreads};
+    const int64_t bytes = row_bytes(vocab, dtype);
     return {{1, (int)vocab}, rows < 512 ? 512 : bytes >= 128000 ? 1024 : bytes >= 48000 ? 512 : 256};
 }
 
@@ -831,17 +846,17 @@ int launch_logprob_plan(const TokenLogprobArgs& a, const LogprobPlan& pl, void* 
 
 size_t token_logprobs_workspace(int64_t rows, int64_t vocab, int top) {
     if (rows == 0) return 0;
-    const Cut c = logprob_plan(rows, vocab, top).cut;
+    const Cut c = logprob_plan(rows, vocab, top, CDX_DTYPE_F32).cut;
     if (c.parts == 1) return 0;
     return round256((size_t)rows * c.parts * sizeof(Part)) + (size_t)rows * c.parts * top * sizeof(u64);
 }
 
 int token_logprobs_parts(int64_t rows, int64_t vocab, int top) {
-    return logprob_plan(rows, vocab, top).cut.parts;
+    return logprob_plan(rows, vocab, top, CDX_DTYPE_F32).cut.parts;
 }
 
 int launch_token_logprobs(const TokenLogprobArgs& a, void* ws, hipStream_t stream) {
-    return launch_logprob_plan(a, logprob_plan(a.r.rows, a.r.vocab, a.top), ws, stream);
+    return launch_logprob_plan(a, logprob_plan(a.r.rows, a.r.vocab, a.top, a.r.dtype), ws, stream);
 }
 
 int launch_token_logprobs_backward(const LogitRows& r, const int64_t* targets, const float* stats,

@@ -616,9 +616,8 @@ int cdx_linear_weight_grad_e4m3(const void* dz, int64_t lddz, int dtype,
  * CDX_EPI_NONE to _SIGMOID, with the hardware's exponential and reciprocal.  y may be
  * residual itself (the same pointer and leading dimension); y and z must not overlap anything
  * else.  workspace: the query's bytes, 16-byte aligned; NULL allocates stream-ordered.  Products
- * of more tiles than a launch holds (2^23 of 128 x 128, or of 256 x 256 where operands are
- * aligned, and 16 columns for few rows) are CDX_ERR_UNSUPPORTED.  The same bits every time.  No
- * counterpart in the reference. */
+ * of 2^23 output tiles and more (of 256 x 256, fewer rows or columns 128 x 128 or 64 x 64) are
+ * CDX_ERR_UNSUPPORTED.  The same bits every time.  No counterpart in the reference. */
 size_t cdx_linear16_workspace_size(int64_t M, int64_t N, int64_t K);
 int cdx_linear16(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
                  const void* weight, int64_t ldw, const void* bias, int bias_dtype,
@@ -656,7 +655,7 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
  * Logits of -infinity have probability 0.  A row of -infinity alone has logprob -infinity, entropy 0 and
  * no gradient.  A NaN or +infinity makes its row's numbers NaN; top_index is then some index in the
  * vocabulary.  workspace: the query's bytes, 16-byte aligned; NULL allocates stream-ordered.
- * Rows, one workgroup each, are up to 2^24 - 1, and up to 2^22 - 1 of long ones (more are
+ * Rows, one workgroup each, are up to 2^24 - 1, and up to 2^22 - 1 of 128 KB and more (else
  * CDX_ERR_UNSUPPORTED).  No counterpart in the reference. */
 size_t cdx_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top);
 int cdx_token_logprobs(const void* logits, int64_t ldx, int64_t rows, int64_t vocab, int dtype,

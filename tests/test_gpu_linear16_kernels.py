@@ -33,13 +33,14 @@ def _padded(t, aligned, value=float("nan")):
 
 # (kernel, whether slices are added, aligned, a product's M, N, K); K is no multiple of 64
 CASES = [("direct", False, True, 5, 304, 1000), ("direct", False, True, 30, 4040, 1096),
-         ("direct", False, True, 128, 520, 72), ("direct", False, False, 60, 5001, 333),
-         ("direct", False, False, 17, 4999, 65), ("ring 64", False, True, 296, 1000, 200),
+         ("direct", False, True, 128, 520, 72), ("direct", False, False, 60, 4001, 333),
+         ("direct", False, False, 17, 3999, 65), ("ring 64", False, True, 296, 1000, 200),
          ("ring 64", True, True, 136, 264, 4136), ("ring 128", False, True, 1400, 1608, 264),
          ("ring 128", True, True, 264, 520, 90120), ("tile 128", False, True, 2104, 2184, 200),
          ("turns", False, True, 3600, 3592, 200), ("turns", True, True, 1000, 1104, 53352),
-         ("any", False, False, 839, 953, 77), ("any", True, False, 299, 203, 1777),
-         ("any 128", False, False, 1801, 1807, 93), ("any 128", True, False, 1336, 1441, 1026)]
+         ("tile 128", False, True, 72, 33000, 136), ("tile 128", False, True, 33000, 128, 136),
+         ("any", False, False, 839, 953, 77), ("any", False, False, 50, 30001, 77), ("any", True, False, 299, 203, 1777),
+         ("any 128", False, False, 1801, 1807, 93), ("any 128", True, False, 1336, 1441, 4106)]
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f16"])

@@ -14,7 +14,7 @@ def _gpu():
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("size", [(511, 40009), (513, 40009), (513, 39999), (127, 70001), (128, 70001)])
+@pytest.mark.parametrize("size", [(255, 40009), (257, 75001), (511, 40009), (513, 40009), (513, 39999), (127, 70001), (128, 70001)])
 def test_logprobs_and_gradient(size, dtype):
     import torch
     from cudeep_amd import ops

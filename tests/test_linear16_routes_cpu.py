@@ -12,12 +12,16 @@ BF16 = 3
 
 
 @pytest.mark.parametrize("M,N,K,aligned,want", [
-    (1, 4096, 4096, True, "direct"), (16, 8192, 4096, True, "direct"), (16, 8208, 4096, True, "ring 64"),
-    (16, 32768, 64, True, "ring 128"), (1, 4096, 8200, True, "ring 64"), (32, 4096, 2048, True, "direct"),
-    (48, 4096, 2048, True, "ring 64"), (128, 1024, 1024, True, "direct"), (129, 1024, 1024, True, "ring 64"),
-    (64, 4096, 63, True, "direct"), (64, 30000, 4001, False, "direct"), (65, 4096, 4001, False, "any"),
-    (640, 2048, 64, False, "any 128"), (640, 1920, 64, False, "any"),
-    (1280, 1280, 1280, True, "ring 64"), (1400, 1600, 1280, True, "ring 128"), (2048, 2048, 2048, True, "ring 128"),
+    (1, 4096, 4096, True, "direct"), (1, 4096, 4104, True, "ring 64"), (16, 4112, 4096, True, "ring 64"),
+    (32, 4096, 2048, True, "direct"), (33, 4096, 2048, True, "ring 64"), (128, 1024, 1024, True, "direct"),
+    (129, 1024, 1024, True, "ring 64"), (64, 4096, 63, True, "direct"), (64, 4096, 2048, False, "direct"),
+    (64, 4096, 2049, False, "any"), (64, 4097, 333, False, "any"), (65, 4096, 333, False, "any"),
+    (65, 17920, 333, False, "any 128"), (64, 17920, 333, False, "any"), (65, 17792, 333, False, "any"),
+    (640, 1664, 8193, False, "any 128"), (640, 1664, 4001, False, "any"), (300, 700, 100001, False, "any 128"),
+    (16, 32768, 64, True, "ring 128"), (16, 40000, 64, True, "tile 128"), (1, 128256, 4096, True, "tile 128"),
+    (128, 128256, 4096, True, "tile 128"), (129, 128256, 4096, True, "turns"),
+    (1280, 1280, 1280, True, "ring 64"), (1024, 2048, 1280, True, "ring 64"), (1400, 1600, 1280, True, "ring 128"),
+    (1024, 1024, 8192, True, "ring 128"), (1024, 1024, 8128, True, "ring 64"), (2048, 2048, 2048, True, "ring 128"),
     (2048, 2176, 2048, True, "tile 128"), (2048, 2176, 63, True, "any 128"), (3584, 3584, 512, True, "tile 128"),
     (2560, 5120, 512, True, "turns"), (512, 512, 65536, True, "ring 128"), (1024, 1024, 65536, True, "turns"),
     (256, 256, 16384, True, "ring 64"),
@@ -30,8 +34,8 @@ def test_forward(M, N, K, aligned, want):
 
 
 @pytest.mark.parametrize("M,N,K,aligned,slices", [
-    (64, 4096, 4096, True, 4), (1024, 1024, 4096, True, 1), (256, 256, 16384, True, 16), (256, 784, 8192, True, 4),
-    (1024, 1024, 65536, True, 16), (512, 512, 65536, True, 16), (256, 784, 8192, False, 9), (1336, 1440, 8026, False, 3),
+    (64, 4096, 4096, True, 4), (1024, 1024, 4096, True, 1), (256, 256, 16384, True, 8), (256, 784, 8192, True, 4),
+    (1024, 1024, 65536, True, 16), (512, 512, 65536, True, 16), (256, 784, 8192, False, 8), (1336, 1440, 8026, False, 3), (256, 512, 65536, True, 16),
     (300, 1000, 200, True, 1),
 ])
 def test_slices(M, N, K, aligned, slices):
@@ -41,12 +45,10 @@ def test_slices(M, N, K, aligned, slices):
 
 
 def test_products_that_no_launch_holds():
-    for M, N in ((1 << 20, 1 << 20), (1, 1 << 28), (1 << 18, 1 << 22)):
+    """2^23 tiles and more, of 64 x 64 and of 128 x 128."""
+    for M, N in ((1 << 20, 1 << 20), (1, 1 << 30), (1 << 18, 1 << 22)):
         st = L.lib().cdx_linear16(M, N, 16, P, 16, P, 16, None, BF16, None, N, C, N, None, N, 0, BF16, None, 0, None)
-        if M * N <= 1 << 38:   # (larger ones fit 256 x 256 tiles only where K has a whole step)
-            assert st == L.CDX_ERR_UNSUPPORTED and b"tiles" in L.lib().cdx_last_error(), (M, N)
-        else:
-            assert st == L.CDX_ERR_UNSUPPORTED, (M, N)
+        assert st == L.CDX_ERR_UNSUPPORTED and b"tiles" in L.lib().cdx_last_error(), (M, N)
 
 
 def test_queries_of_sizes_that_nothing_has():
@@ -63,7 +65,7 @@ def test_logits_parts():
     f.restype, f.argtypes = ctypes.c_int, [ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int]
     for op, rows, vocab, top, want in [(0, 1, 65536, 5, 1), (0, 1, 131072, 5, 8), (0, 1, 131072, 64, 8),
                                        (0, 1, 400000, 64, 16), (0, 127, 131072, 0, 4), (0, 128, 131072, 0, 1),
-                                       (1, 16, 65536, 0, 1), (1, 16, 131072, 0, 8), (1, 128, 131072, 0, 1)]:
+                                       (1, 16, 65535, 0, 1), (1, 16, 65536, 0, 4), (1, 16, 131072, 0, 8), (1, 128, 131072, 0, 1)]:
         assert f(op, rows, vocab, top) == want, (op, rows, vocab, top)
 
 

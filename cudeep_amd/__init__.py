@@ -1,8 +1,8 @@
 """cudeep_amd -- MI355X (gfx950) implementation of cuDeep's dense-contraction
 hot path: FP32 MFMA SGEMM, TF32-mode (bf16x3) GEMM, fused bias/ReLU/GELU
 epilogues, im2col + Conv2d forward, and the Linear helpers, layer norm, 8-bit
-block-scaled products and 8-bit activation checkpoints, behind the C-ABI in
-include/cudeep_amd.h (libcudeep_amd.so)."""
+block-scaled products, 8-bit activation checkpoints, the 16-bit Linear and what
+reads a model's logits, behind the C-ABI in include/cudeep_amd.h (libcudeep_amd.so)."""
 from ._runtime import share_torch_hip_runtime
 
 # before any native library of this package is loaded

@@ -8,7 +8,7 @@ namespace {
 using namespace l16;
 
 // Sums of slices, added in their order, through the epilogue: a thread has eight n of a row.  Behind
-// them the column sums.
+// them the column sums.  Short and bound by its launch (256 x 784 in 4 slices 3.9 us).
 template <class T, bool EPI>
 __global__ __launch_bounds__(256)
 void linear16_sum_kernel(Params p, const float* __restrict__ part, const float* __restrict__ col_part,
@@ -46,7 +46,8 @@ void linear16_sum_kernel(Params p, const float* __restrict__ part, const float* 
     }
 }
 
-// dz = grad act'(z), eight columns a thread.  PAST: grad and z, which nobody reads again, pass the caches by
+// dz = grad act'(z), eight columns a thread, one pass that memory bounds (8192 x 4096 in bf16 36 us, 5.6 TB/s:
+// some of z is in the caches).  PAST: grad and z, which nobody reads again, pass the caches by
 // (block8.hpp), so that dz is there for the products: a training step of 8192 x 4096 x 4096 727 us, 741
 // without.
 template <class T, int ACT, bool PAST>

@@ -362,7 +362,10 @@ template <class T> __device__ __forceinline__ void finish_row(const LogprobParam
     if (p.entropy) p.entropy[row] = entropy_of(a, s.l, p.r.inv_t);
 }
 
-// A workgroup a row, or a part of one.
+// A workgroup a row, or a part of one: the row is read once, with the next round's loads on their way, and
+// memory bounds long batches (1021 x 50001 in fp32, with entropies, 37.3 us, 5.5 TB/s; 2048 x 131072 in
+// bf16 with entropies and 8 alternatives 111.6, 4.8 TB/s).  A single row of 32000 in fp32 with 5 alternatives
+// takes 8.0 us, most of them the chain of the alternatives.
 template <class T, int NT, bool ENT, bool TOP>
 __global__ __launch_bounds__(NT)
 void logprob_kernel(LogprobParams p) {
@@ -430,7 +433,9 @@ void logprob_join_kernel(LogprobParams p) {
     }
 }
 
-// The gradient, element by element: a workgroup takes kBackward elements of a row.
+// The gradient, element by element: a workgroup takes kBackward elements of a row.  Memory bounds it, 1021 x
+// 50001 in fp32 61.9 us, 6.6 TB/s read and written (62.1 with the rows in reverse, which begins with those
+// that were read last).
 constexpr int kBackwardThreads = 256;
 template <class T> constexpr int kBackward = kBackwardThreads * kUnroll * kVec<T>;
 
@@ -645,8 +650,9 @@ __device__ __forceinline__ void load_entries(const DistillArgs& a, int64_t row, 
     }
 }
 
-// A workgroup a row: sums, entries, and the gradient, for which the row is read again (most of it out of
-// the caches).
+// A workgroup a row: sums, entries, and the gradient, for which the row is read again.  Memory bounds it:
+// 4096 x 65536 in bf16 with 64 entries 232 us, in which 0.86 GB are read (0.54 are the logits) and 0.54
+// written.  Rows kept in registers for the second reading do not fit (spills, 875 us against 247).
 template <class T, int NT, bool GRAD, bool STREAM>
 __global__ __launch_bounds__(NT)
 void distill_kernel(DistillArgs a) {

@@ -80,12 +80,13 @@ void linear16_slope_kernel(const T* __restrict__ grad, int64_t ldg, const T* __r
 }
 
 // (a layer without inputs still has its bias's column of tiles)
-int64_t tiles_of(int64_t M, int64_t N, int side) {
-    return ceil_div(M, (int64_t)side) * (N > 0 ? ceil_div(N, (int64_t)side) : 1);
+int64_t tiles_of(int64_t M, int64_t N, int rows, int cols) {
+    return ceil_div(M, (int64_t)rows) * (N > 0 ? ceil_div(N, (int64_t)cols) : 1);
 }
+int64_t tiles_of(int64_t M, int64_t N, int side) { return tiles_of(M, N, side, side); }
 
 Plan make_plan(Kernel kernel, int64_t M, int64_t N, int64_t K, int side, int64_t slices) {
-    const int64_t tiles = tiles_of(M, N, side);
+    const int64_t tiles = kernel == Kernel::Tall ? tiles_of(M, N, 128, 64) : tiles_of(M, N, side);
     const int64_t chunk = ceil_div(ceil_div(K, slices), (int64_t)kStep) * kStep;
     return {kernel, tiles, K > 0 ? (int)ceil_div(K, chunk) : 1, chunk > 0 ? chunk : kStep};
 }
@@ -138,11 +139,15 @@ Plan plan_of(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned) {
     // 128 x 128 tiles: two workgroups a CU share it where there is more than one (2048 x 2176 x 2048 32.3, ring 128
     // 36.7; 1 x 128256 x 4096 172, turns 246), else one has four buffers (2048 x 2048 x 2048 21.2, tile 128 26.4)
     if (t128 > 256) return make_plan(Kernel::Tile128, M, N, K, 128, 1);
-    // and 64 x 64 tiles where those leave CUs idle (1408 x 1536 x 2048, 132 tiles of 128, 21.2, ring 128 19.0; 1024 x
-    // 1536 x 2048, 96, 13.4, ring 128 18.7), unless k is long (1152 x 1152 x 8192 46, ring 128 in 3 slices 36;
-    // weight 256 x 512 x 65536 55, ring 128 in 16 slices 48; 1280 x 1280 x 4096 25.0, ring 128 in 2 slices 26.7)
-    if (t128 > 128 || t128 * long_k >= 256)
+    // fewer of them, with a long k, in three slices and more (1152 x 1152 x 8192 36, ring 64 46; weight 256 x 512 x
+    // 65536 in 16 48, ring 64 55; but 2048 x 1024 x 4096 in 2 30.1, tall 24.2)
+    if (t128 <= 85 && t128 * long_k >= 256)
         return make_plan(Kernel::Ring128, M, N, K, 128, cut(t128, 256, 2048, 16));
+    // 128 x 64 where a CU would have more than one of 64 x 64 and has one of these (8192 x 256 x 784 10.4, ring 64
+    // 12.1; 2048 x 1024 x 4096 24.2, ring 64 26.1; 1280 x 1280 x 1280 10.3, ring 64 10.6; but 1024 x 1024 x 1024
+    // 8.3, ring 64 6.3, and 1408 x 1536 x 2048 24.5, ring 128 19.0)
+    if (t64 > 256 && tiles_of(M, N, 128, 64) <= 256) return make_plan(Kernel::Tall, M, N, K, 64, 1);
+    if (t64 > 256) return make_plan(Kernel::Ring128, M, N, K, 128, 1);
     return make_plan(Kernel::Ring64, M, N, K, 64, cut(t64, 256, 1024, 8));
 }
 
@@ -201,7 +206,7 @@ size_t linear16_workspace(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bo
 
 const char* linear16_kernel_name(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned,
                                  int* slices) {
-    static const char* const names[] = {"any", "any 128", "ring 64", "ring 128", "tile 128", "turns", "direct"};
+    static const char* const names[] = {"any", "any 128", "ring 64", "ring 128", "tile 128", "turns", "direct", "tall"};
     const Plan pl = plan_of(kind, M, N, K, aligned);
     *slices = pl.slices;
     return names[(int)pl.kernel];

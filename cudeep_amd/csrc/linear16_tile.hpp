@@ -458,7 +458,9 @@ __device__ __forceinline__ void finish_tile(const Params& p, const Slice& sl, W&
         w.multiply();
     }
     w.settle();
-    constexpr int ROWS = (BM + BN) * 128 / (BN * 4) < BM ? (BM + BN) * 128 / (BN * 4) : BM;
+    constexpr int FIT = (BM + BN) * 128 / (BN * 4);   // rows of sums that the buffer holds
+    constexpr int ROWS = FIT >= BM ? BM : FIT >= BM / 2 ? BM / 2 : BM / 4;
+    static_assert(ROWS <= FIT, "rows of sums fit the buffer");
     store_tile<T, !CA && !CB, BM, BN, WM, WN, ROWS>(p, buf, m0, n0, w.wm, w.wn, w.acc);
     if constexpr (W::SUMS) w.store_sums(p, m0, lane);
 }
@@ -467,7 +469,8 @@ __device__ __forceinline__ void finish_tile(const Params& p, const Slice& sl, W&
 // that a step's reads need not wait for the later steps' loads): D - 1 steps are in flight, one
 // barrier a step.  What bounds them, at 64 x 64 x 4 buffers: a step of four waves is short beside its barrier
 // and the loads' way (one workgroup a CU, 1280 x 1280 x 1280: 10.2 us, 0.5 us a step; eight buffers
-// are no faster); at 128 x 128: LDS reads, as many as matrix instructions have slots for (2048 x 2048 x
+// are no faster), for which a CU does better with one of 128 x 64 and eight waves than with two of 64 x 64 (8192 x
+// 256 x 784 10.4 us against 12.1); at 128 x 128: LDS reads, as many as matrix instructions have slots for (2048 x 2048 x
 // 2048 with eight waves and four buffers, alone on a CU, 21.2 us, 810 TFLOP/s; two workgroups a CU with two
 // buffers each hide each other's barriers, 2560 x 4608 x 1024 34 us, 710 TFLOP/s).
 template <class T, bool CA, bool CB, int BM, int BN, int WM, int WN, int D>
@@ -697,7 +700,7 @@ void linear16_direct_kernel(Params p) {
 
 // ---- launches ------------------------------------------------------------------------------------
 
-enum class Kernel { Any, Any128, Ring64, Ring128, Tile128, Turns, Direct };
+enum class Kernel { Any, Any128, Ring64, Ring128, Tile128, Turns, Direct, Tall };
 struct Plan { Kernel kernel; int64_t tiles; int slices; int64_t chunk; int mt = 1; };   // mt: Direct's MT
 
 template <class F> int with_16(int dtype, F f) {
@@ -719,6 +722,9 @@ int run(const Params& p, const Plan& pl, hipStream_t stream) {
             break;
         case Kernel::Ring64:
             hipLaunchKernelGGL((linear16_tile_kernel<T, CA, CB, 64, 64, 2, 2, 4>), grid, dim3(256), 0, stream, p);
+            break;
+        case Kernel::Tall:
+            hipLaunchKernelGGL((linear16_tile_kernel<T, CA, CB, 128, 64, 4, 2, 4>), grid, dim3(512), 0, stream, p);
             break;
         case Kernel::Any128:
             hipLaunchKernelGGL((linear16_any_kernel<T, CA, CB, 128, 128, 2, 4>), grid, dim3(512), 0, stream, p);

@@ -35,6 +35,7 @@ def _padded(t, aligned, value=float("nan")):
 CASES = [("direct", False, True, 5, 304, 1000), ("direct", False, True, 30, 4040, 1096),
          ("direct", False, True, 128, 520, 72), ("direct", False, False, 60, 4001, 333),
          ("direct", False, False, 17, 3999, 65), ("ring 64", False, True, 296, 1000, 200),
+         ("tall", False, True, 1304, 1288, 200), ("tall", False, True, 8200, 136, 4104),
          ("ring 64", True, True, 136, 264, 4136), ("ring 128", False, True, 1400, 1608, 264),
          ("ring 128", True, True, 264, 520, 90120), ("tile 128", False, True, 2104, 2184, 200),
          ("turns", False, True, 3600, 3592, 200), ("turns", True, True, 1000, 1104, 53352),

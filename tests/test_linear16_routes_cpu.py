@@ -20,7 +20,9 @@ BF16 = 3
     (640, 1664, 8193, False, "any 128"), (640, 1664, 4001, False, "any"), (300, 700, 100001, False, "any 128"),
     (16, 32768, 64, True, "ring 128"), (16, 40000, 64, True, "tile 128"), (1, 128256, 4096, True, "tile 128"),
     (128, 128256, 4096, True, "tile 128"), (129, 128256, 4096, True, "turns"),
-    (1280, 1280, 1280, True, "ring 64"), (1024, 2048, 1280, True, "ring 64"), (1400, 1600, 1280, True, "ring 128"),
+    (1024, 1024, 1280, True, "ring 64"), (1025, 1024, 1280, True, "tall"), (1024, 2048, 1280, True, "tall"),
+    (1025, 2048, 1280, True, "ring 128"), (2048, 1024, 4096, True, "tall"), (1152, 1152, 8192, True, "ring 128"),
+    (1152, 1152, 8128, True, "tall"), (1400, 1600, 1280, True, "ring 128"),
     (1024, 1024, 8192, True, "ring 128"), (1024, 1024, 8128, True, "ring 64"), (2048, 2048, 2048, True, "ring 128"),
     (2048, 2176, 2048, True, "tile 128"), (2048, 2176, 63, True, "any 128"), (3584, 3584, 512, True, "tile 128"),
     (2560, 5120, 512, True, "turns"), (512, 512, 65536, True, "ring 128"), (1024, 1024, 65536, True, "turns"),

@@ -97,16 +97,17 @@ Plan direct_plan(int64_t M, int64_t N, int mt) {
 
 // Which kernel, and how many slices of k (all figures us, bf16, M x N x K; "input", "weight": of those
 // products, else forward).  Slices are added by a launch of their own, so that they have to save more than
-// that and their sums' traffic: 8 of 64 x 64 tiles at most (256 x 256 x 16384 14.9, 16 of them 16.9), 16 of
-// 128 x 128 (weight 256 x 512 x 65536 48, 32 of them 56).
+// that and their sums' traffic: 8 of ring 64 at most (256 x 256 x 16384 14.9, 16 of them 16.9), 16 of
+// the others (weight 256 x 512 x 65536 on ring 128 48, 32 of them 56; unaligned 4 x 640 x 6575 15.1, 8 17.8).
 Plan plan_of(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned) {
     aligned = aligned && K >= kStep && N > 0;   // (a whole step, and columns of B, to load straight into LDS)
     // Few rows, whose weights are read once: one launch with k split inside the workgroups, while these are no
     // more than the CUs (1 x 4096 x 4096 6.6, ring 64 in 4 slices 8.6; 128 x 1024 x 1024 5.0, ring 64 5.8; but
     // 16 x 8192 x 4096 18.9, ring 64 13.9) and k is short (1 x 2048 x 8192 12.0, ring 64 in 8 slices 9.9).
-    // Operands of any alignment, which ring 64 does not take, up to 64 rows and half that k (33 x 4096 x 1001
-    // 9.6, any in 2 slices 11.7; 64 x 4096 x 4001 50, any in 8 slices 15.6; 65 x 4096 x 1001 15.9, any 13.0).
-    if (kind == Linear16Kind::Forward && K > 0 && M <= (aligned ? 128 : 64) && K <= (aligned ? 4096 : 2048)) {
+    // Operands of any alignment, which ring 64 does not take, up to 64 rows and, but for a single row, half that k
+    // (1 x 4096 x 2049 9.7, any in 5 slices 12.0; 33 x 4096 x 1001 9.6, any in 2 11.7; 16 x 4096 x 2049 15.3, any in
+    // 5 12.7; 64 x 4096 x 4001 50, any in 8 15.6; 65 x 4096 x 1001 15.9, any 13.0).
+    if (kind == Linear16Kind::Forward && K > 0 && M <= (aligned ? 128 : 64) && K <= (aligned || M == 1 ? 4096 : 2048)) {
         const int64_t tiles_m = ceil_div(M, (int64_t)16), tiles_n = ceil_div(N, (int64_t)16);
         for (int mt = 1; mt <= (aligned ? 2 : 4); mt *= 2)
             if (ceil_div(tiles_m, (int64_t)mt) * tiles_n <= 256) return direct_plan(M, N, mt);
@@ -129,7 +130,7 @@ Plan plan_of(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned) {
         // 1024 199, 64 x 64 176)
         if (narrow > 64 && (t128 >= 140 || t128 * long_k >= 256))
             return make_plan(Kernel::Any128, M, N, K, 128, t128 >= 200 ? 1 : cut(t128, 512, 1024, 16));
-        return make_plan(Kernel::Any, M, N, K, 64, t64 >= 200 ? 1 : cut(t64, 512, 384, 8));
+        return make_plan(Kernel::Any, M, N, K, 64, t64 >= 200 ? 1 : cut(t64, 512, 384, 16));
     }
     // 256 x 256, for most of the CUs (2560 x 5120 x 1024 35.6, tile 128 38.8; 2560 x 4608 x 1024 37.5, tile 128
     // 34.0), by slices too (weight 1024 x 1024 x 65536 in 16 155, ring 128 in 4 177), where half of a tile does not

@@ -15,7 +15,8 @@ BF16 = 3
     (1, 4096, 4096, True, "direct"), (1, 4096, 4104, True, "ring 64"), (16, 4112, 4096, True, "ring 64"),
     (32, 4096, 2048, True, "direct"), (33, 4096, 2048, True, "ring 64"), (128, 1024, 1024, True, "direct"),
     (129, 1024, 1024, True, "ring 64"), (64, 4096, 63, True, "direct"), (64, 4096, 2048, False, "direct"),
-    (64, 4096, 2049, False, "any"), (64, 4097, 333, False, "any"), (65, 4096, 333, False, "any"),
+    (64, 4096, 2049, False, "any"), (1, 4096, 4001, False, "direct"),
+    (2, 4096, 4001, False, "any"), (64, 4097, 333, False, "any"), (65, 4096, 333, False, "any"),
     (65, 17920, 333, False, "any 128"), (64, 17920, 333, False, "any"), (65, 17792, 333, False, "any"),
     (640, 1664, 8193, False, "any 128"), (640, 1664, 4001, False, "any"), (300, 700, 100001, False, "any 128"),
     (16, 32768, 64, True, "ring 128"), (16, 40000, 64, True, "tile 128"), (1, 128256, 4096, True, "tile 128"),
@@ -37,7 +38,7 @@ def test_forward(M, N, K, aligned, want):
 
 @pytest.mark.parametrize("M,N,K,aligned,slices", [
     (64, 4096, 4096, True, 4), (1024, 1024, 4096, True, 1), (256, 256, 16384, True, 8), (256, 784, 8192, True, 4),
-    (1024, 1024, 65536, True, 16), (512, 512, 65536, True, 16), (256, 784, 8192, False, 8), (1336, 1440, 8026, False, 3), (256, 512, 65536, True, 16),
+    (1024, 1024, 65536, True, 16), (512, 512, 65536, True, 16), (256, 784, 8192, False, 9), (16, 640, 6575, False, 15), (1336, 1440, 8026, False, 3), (256, 512, 65536, True, 16),
     (300, 1000, 200, True, 1),
 ])
 def test_slices(M, N, K, aligned, slices):

@@ -34,9 +34,19 @@ bool no_layer(int64_t M, int64_t N, int64_t K) {
 // A vector's bytes as a row.
 Span vector_span(const void* p, int64_t n, int dtype) { return {p, n, 1, n, dtype}; }
 
+size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
 size_t slope_bytes(int64_t M, int64_t N, int epilogue) {
     if (epilogue == CDX_EPI_NONE) return 0;
-    return ((size_t)M * (size_t)(cdx::ceil_div(N, (int64_t)8) * 8) * 2 + 255) / 256 * 256;
+    return round256((size_t)M * (size_t)(cdx::ceil_div(N, (int64_t)8) * 8) * 2);
+}
+
+// Whether dz is rounded (without an activation, and with ReLU, it is grad_out's own values and zeros): the bias
+// gradient is summed beside the slopes then.
+bool rounds_slope(int epilogue) { return epilogue != CDX_EPI_NONE && epilogue != CDX_EPI_RELU; }
+
+size_t slope_sums_bytes(int64_t M, int64_t N, int epilogue) {
+    return rounds_slope(epilogue) ? round256(cdx::linear16_slope_sums_workspace(M, N)) : 0;
 }
 
 }  // namespace
@@ -91,7 +101,7 @@ size_t cdx_linear16_backward_workspace_size(int64_t M, int64_t N, int64_t K, int
     if (no_layer(M, N, K) || !gemm_epilogue(epilogue)) return 0;
     const size_t dx = cdx::linear16_workspace(Linear16Kind::Input, M, K, N, false);
     const size_t dw = cdx::linear16_workspace(Linear16Kind::Weight, N, K, M, true);
-    return slope_bytes(M, N, epilogue) + (dx > dw ? dx : dw);
+    return slope_bytes(M, N, epilogue) + slope_sums_bytes(M, N, epilogue) + (dx > dw ? dx : dw);
 }
 
 int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out, int64_t ldg,
@@ -128,7 +138,7 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
     const bool dx = grad_x && M > 0 && K > 0;
     const bool dw = N > 0 && ((grad_weight && K > 0) || grad_bias);
     if (!dx && !dw) return CDX_OK;
-    // (a layer without inputs has a bias still: a product of one column that nobody stores)
+    // (a layer without inputs has a bias still: a product of one column that nobody stores, or the slopes' sums)
     if (M == 0) {   // empty sums
         if (grad_weight && K > 0) st = cdx::launch_zero(grad_weight, N * K, param_dtype, stream);
         if (!st && grad_bias) st = cdx::launch_zero(grad_bias, N, param_dtype, stream);
@@ -139,13 +149,23 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
         [&](void* ws) {
             const void* dz = grad_out;
             int64_t lddz = ldg;
+            const bool f32 = param_dtype == CDX_DTYPE_F32;
+            void* bias_sums = grad_bias;   // of the weight product
             uint8_t* part = static_cast<uint8_t*>(ws);
             if (epilogue != CDX_EPI_NONE && N > 0) {
                 lddz = cdx::ceil_div(N, (int64_t)8) * 8;
-                int e = cdx::launch_linear16_slope(grad_out, ldg, z, ldz, ws, lddz, M, N, dtype, epilogue, stream);
+                part += slope_bytes(M, N, epilogue);
+                int e;
+                if (grad_bias && rounds_slope(epilogue)) {
+                    e = cdx::launch_linear16_slope_sums(grad_out, ldg, z, ldz, ws, lddz, M, N, dtype, epilogue, grad_bias,
+                                                        f32, reinterpret_cast<float*>(part), stream);
+                    bias_sums = nullptr;
+                } else {
+                    e = cdx::launch_linear16_slope(grad_out, ldg, z, ldz, ws, lddz, M, N, dtype, epilogue, stream);
+                }
                 if (e) return e;
                 dz = ws;
-                part += slope_bytes(M, N, epilogue);
+                part += slope_sums_bytes(M, N, epilogue);
             }
             if (dx) {
                 cdx::Linear16Product p{M, K, N, dz, lddz, weight, ldw, dtype, {}};
@@ -153,10 +173,10 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
                 int e = cdx::launch_linear16(Linear16Kind::Input, p, false, nullptr, part, stream);
                 if (e) return e;
             }
-            if (!dw) return (int)CDX_OK;
+            if (!dw || (K == 0 && !bias_sums)) return (int)CDX_OK;
             cdx::Linear16Product p{N, K, M, dz, lddz, x, ldx, dtype, {}};
             p.out.y = grad_weight; p.out.ldy = K;
-            return cdx::launch_linear16(Linear16Kind::Weight, p, param_dtype == CDX_DTYPE_F32, grad_bias, part, stream);
+            return cdx::launch_linear16(Linear16Kind::Weight, p, f32, bias_sums, part, stream);
         });
 }
 

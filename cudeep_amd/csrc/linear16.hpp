@@ -42,5 +42,11 @@ const char* linear16_kernel_name(Linear16Kind kind, int64_t M, int64_t N, int64_
 int launch_linear16_slope(const void* grad, int64_t ldg, const void* z, int64_t ldz, void* dz,
                           int64_t lddz, int64_t rows, int64_t cols, int dtype, int act,
                           hipStream_t stream);
+// The same for GELU, SiLU and sigmoid (the others' dz is exact), with `sums`[cols] = sum over rows of dz before its
+// rounding, in 16 bits or fp32; part: the workspace's bytes.
+size_t linear16_slope_sums_workspace(int64_t rows, int64_t cols);
+int launch_linear16_slope_sums(const void* grad, int64_t ldg, const void* z, int64_t ldz, void* dz,
+                               int64_t lddz, int64_t rows, int64_t cols, int dtype, int act, void* sums,
+                               bool sums_f32, float* part, hipStream_t stream);
 
 }  // namespace cdx

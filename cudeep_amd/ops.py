@@ -1068,7 +1068,7 @@ def linear16_backward(grad_out, x, weight, z=None, *, epilogue=L.EPI_NONE, input
                       bias=True, param_dtype=None, workspace=None):
     """(grad of x, of weight, of bias) of linear16 from its output's gradient and, with an activation,
     the z that it kept; the residual's gradient is grad_out itself.  grad_out * epi'(z) is rounded to
-    x's type as the products' operand, sums are float32.  The gradient of x has its type, the
+    x's type as the products' operand, the bias's gradient sums it before that; sums are float32.  The gradient of x has its type, the
     parameters' are of `param_dtype` (x's type or float32).  None for x's without `input`, for both
     parameters' without `params`, for the bias's without `bias`.  `workspace`
     (linear16_backward_workspace_bytes) makes the call allocation-free."""

@@ -629,8 +629,9 @@ int cdx_linear16(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
  * operand (grad_out itself for CDX_EPI_NONE, where z may be NULL),
  *   grad_x[m][k] = sum_n dz[m][n] W[n][k]            (dtype),
  *   grad_weight[n][k] = sum_m dz[m][n] x[m][k]       (param_dtype, dense),
- *   grad_bias[n] = sum_m dz[m][n]                    (param_dtype, dense),
- * overwritten; sums fp32, the same bits every time.  (The residual's gradient is grad_out.)
+ *   grad_bias[n] = sum_m dz[m][n]                    (param_dtype, dense; dz before its rounding),
+ * overwritten; sums fp32, the same bits every time.  (The residual's gradient is grad_out.)  A dz past
+ * float16's largest value is an infinite operand: grad_out below 0.88 of it keeps clear of that.
  * param_dtype: dtype or CDX_DTYPE_F32.  grad_x, grad_weight and grad_bias may be NULL (W and x
  * then too), but grad_bias needs grad_weight.  Results must not overlap anything.
  * workspace as above. */

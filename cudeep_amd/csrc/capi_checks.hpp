@@ -61,6 +61,23 @@ inline int check_in_place(const char* fn, const char* what, const Span& out, con
     return bad(fn, (std::string(what) + " overlap without being the same").c_str());
 }
 
+struct NamedSpan { const char* name; Span at; };
+
+// A call's results must share nothing with each other, nor with what is read while they are written.
+template <size_t W, size_t R>
+inline int check_results(const char* fn, const NamedSpan (&writes)[W], const NamedSpan (&reads)[R]) {
+    auto apart = [&](const NamedSpan& a, const NamedSpan& b) {
+        return overlap(a.at, b.at) ? bad(fn, (std::string(a.name) + " and " + b.name + " overlap").c_str()) : (int)CDX_OK;
+    };
+    for (size_t i = 0; i < W; ++i) {
+        for (const NamedSpan& r : reads)
+            if (const int st = apart(writes[i], r)) return st;
+        for (size_t j = 0; j < i; ++j)
+            if (const int st = apart(writes[i], writes[j])) return st;
+    }
+    return CDX_OK;
+}
+
 // Scratch that holds 16-byte pieces.
 inline int check_workspace(const char* fn, const void* ws) {
     return (uintptr_t)ws % 16 ? bad(fn, "workspace must be 16-byte aligned") : (int)CDX_OK;

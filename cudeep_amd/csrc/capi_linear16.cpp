@@ -121,20 +121,15 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
     if (st) return st;
     if (grad_bias && !grad_weight && N > 0 && K > 0) return bad(fn, "grad_bias needs grad_weight");
     // grad_x is written first: everything that is read later has to be apart from it
-    struct Read { const char* name; Span at; };
-    const Read reads[] = {{"grad_out", {grad_out, ldg, M, N, dtype}},
-                          {"x", {x, ldx, M, grad_weight ? K : 0, dtype}},
-                          {"weight", {weight, ldw, N, grad_x ? K : 0, dtype}},
-                          {"z", {z, ldz, M, epilogue != CDX_EPI_NONE ? N : 0, dtype}}};
-    const Read writes[] = {{"grad_x", {grad_x, ldgx, M, grad_x ? K : 0, dtype}},
-                           {"grad_weight", {grad_weight, K, N, grad_weight ? K : 0, param_dtype}},
-                           {"grad_bias", vector_span(grad_bias, grad_bias ? N : 0, param_dtype)}};
-    for (int i = 0; i < 3; ++i) {
-        for (const Read& r : reads)
-            if (overlap(writes[i].at, r.at)) return bad(fn, (std::string(writes[i].name) + " and " + r.name + " overlap").c_str());
-        for (int j = 0; j < i; ++j)
-            if (overlap(writes[i].at, writes[j].at)) return bad(fn, (std::string(writes[i].name) + " and " + writes[j].name + " overlap").c_str());
-    }
+    const NamedSpan reads[] = {{"grad_out", {grad_out, ldg, M, N, dtype}},
+                               {"x", {x, ldx, M, grad_weight ? K : 0, dtype}},
+                               {"weight", {weight, ldw, N, grad_x ? K : 0, dtype}},
+                               {"z", {z, ldz, M, epilogue != CDX_EPI_NONE ? N : 0, dtype}}};
+    const NamedSpan writes[] = {{"grad_x", {grad_x, ldgx, M, grad_x ? K : 0, dtype}},
+                                {"grad_weight", {grad_weight, K, N, grad_weight ? K : 0, param_dtype}},
+                                {"grad_bias", vector_span(grad_bias, grad_bias ? N : 0, param_dtype)}};
+    st = check_results(fn, writes, reads);
+    if (st) return st;
     const bool dx = grad_x && M > 0 && K > 0;
     const bool dw = N > 0 && ((grad_weight && K > 0) || grad_bias);
     if (!dx && !dw) return CDX_OK;

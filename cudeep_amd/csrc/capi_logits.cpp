@@ -30,6 +30,11 @@ int check_gradient(const char* fn, const void* grad, int64_t ldg, const void* x,
                                     {x, ldx, rows, vocab, dtype});
 }
 
+// n values of `words` 4-byte words each as a row (none where p is NULL).
+Span words_span(const void* p, int64_t n, int64_t words = 1) {
+    return {p, n * words, 1, p ? n * words : 0, CDX_DTYPE_F32};
+}
+
 }  // namespace
 
 extern "C" {
@@ -51,8 +56,16 @@ int cdx_token_logprobs(const void* logits, int64_t ldx, int64_t rows, int64_t vo
     if (rows == 0) return CDX_OK;
     if (!targets || !logprob || !stats) return bad(fn, "targets, logprob or stats is NULL");
     if (top > 0 && (!top_logprob || !top_index)) return bad(fn, "top_logprob or top_index is NULL");
-    cdx::TokenLogprobArgs a{logit_rows(logits, ldx, rows, vocab, dtype, temperature), targets, logprob,
-                            stats, entropy, top, top_logprob, top_index};
+    const cdx::LogitRows r = logit_rows(logits, ldx, rows, vocab, dtype, temperature);
+    st = cdx::token_logprobs_limits(r, top);
+    if (st) return st;
+    const NamedSpan reads[] = {{"logits", {logits, ldx, rows, vocab, dtype}}, {"targets", words_span(targets, rows, 2)}};
+    const NamedSpan writes[] = {{"logprob", words_span(logprob, rows)}, {"stats", words_span(stats, rows, 2)},
+                                {"entropy", words_span(entropy, rows)}, {"top_logprob", words_span(top ? top_logprob : nullptr, rows * top)},
+                                {"top_index", words_span(top ? top_index : nullptr, rows * top, 2)}};
+    st = check_results(fn, writes, reads);
+    if (st) return st;
+    cdx::TokenLogprobArgs a{r, targets, logprob, stats, entropy, top, top_logprob, top_index};
     return with_workspace(fn, cdx_token_logprobs_workspace_size(rows, vocab, top), workspace, workspace_bytes,
                           stream, [&](void* ws) { return cdx::launch_token_logprobs(a, ws, stream); });
 }
@@ -67,6 +80,14 @@ int cdx_token_logprobs_backward(const float* grad_logprob, const void* logits, i
     if (st || rows == 0) return st;
     if (!targets || !stats) return bad(fn, "targets or stats is NULL");
     if (grad_entropy && !entropy) return bad(fn, "grad_entropy needs entropy");
+    // (several workgroups of a row read its values while others write theirs)
+    const NamedSpan reads[] = {{"targets", words_span(targets, rows, 2)}, {"stats", words_span(stats, rows, 2)},
+                               {"grad_logprob", words_span(grad_logprob, rows)},
+                               {"entropy", words_span(grad_entropy ? entropy : nullptr, rows)},
+                               {"grad_entropy", words_span(grad_entropy, rows)}};
+    const NamedSpan writes[] = {{"grad_logits", {grad_logits, ldg, rows, vocab, dtype}}};
+    st = check_results(fn, writes, reads);
+    if (st) return st;
     return cdx::launch_token_logprobs_backward(logit_rows(logits, ldx, rows, vocab, dtype, temperature), targets,
                                                stats, grad_logprob,
                                                entropy, grad_entropy, grad_logits, ldg, stream);
@@ -94,7 +115,19 @@ int cdx_distill_loss(const void* logits, int64_t ldx, int64_t rows, int64_t voca
     if (!st && weight) st = check_gradient(fn, grad_logits, ldg, logits, ldx, rows, vocab, dtype);
     if (st || rows == 0) return st;
     if (!loss) return bad(fn, "loss is NULL");
-    cdx::DistillArgs a{logit_rows(logits, ldx, rows, vocab, dtype, temperature), index, ldi, index_bytes == 8,
+    const cdx::LogitRows r = logit_rows(logits, ldx, rows, vocab, dtype, temperature);
+    st = cdx::distill_limits(r);
+    if (st) return st;
+    // (a row in parts is read by each of its workgroups, of which some write already)
+    const int64_t words = index_bytes / 4;
+    const NamedSpan entries[] = {{"index", {index, ldi * words, rows, count * words, CDX_DTYPE_F32}},
+                                 {"teacher", {teacher, ldt, rows, count, teacher_dtype}}, {"weight", words_span(weight, rows)}};
+    const NamedSpan writes[] = {{"loss", words_span(loss, rows)},
+                                {"grad_logits", {grad_logits, ldg, rows, weight ? vocab : 0, dtype}}};
+    st = check_results(fn, writes, entries);
+    if (!st && overlap(writes[0].at, {logits, ldx, rows, vocab, dtype})) st = bad(fn, "loss and logits overlap");
+    if (st) return st;
+    cdx::DistillArgs a{r, index, ldi, index_bytes == 8,
                        teacher, ldt, teacher_dtype, count, loss, weight, grad_logits, ldg};
     return with_workspace(fn, cdx_distill_loss_workspace_size(rows, vocab, count), workspace, workspace_bytes,
                           stream, [&](void* ws) { return cdx::launch_distill(a, ws, stream); });

@@ -784,7 +784,6 @@ size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 template <class T>
 int run_logprob(const LogprobParams& p, int threads, hipStream_t stream) {
     const int64_t groups = p.r.rows * p.parts;
-    if (!grid_fits(groups, threads)) return set_error(CDX_ERR_UNSUPPORTED, "token_logprobs: too many rows");
     auto go = [&](auto ent, auto top) {
         constexpr bool ENT = decltype(ent)::value, TOP = decltype(top)::value;
         if (threads == 1024)
@@ -834,7 +833,6 @@ int run_distill(const DistillParams& p, const DistillPlan& pl, hipStream_t strea
 
 int launch_distill_plan(const DistillArgs& a, const DistillPlan& pl, void* ws, hipStream_t stream) {
     DistillParams p{a, pl.cut.parts, pl.cut.length, static_cast<Part*>(ws), nullptr};
-    if (!grid_fits(a.r.rows * p.parts, pl.threads)) return set_error(CDX_ERR_UNSUPPORTED, "distill_loss: too many rows");
     if (p.parts > 1)
         p.found = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + round256((size_t)a.r.rows * p.parts * sizeof(Part)));
     return with_dtype(a.r.dtype, [&](auto t) { return run_distill<decltype(t)>(p, pl, stream); });
@@ -859,6 +857,18 @@ size_t token_logprobs_workspace(int64_t rows, int64_t vocab, int top) {
 
 int token_logprobs_parts(int64_t rows, int64_t vocab, int top) {
     return logprob_plan(rows, vocab, top, CDX_DTYPE_F32).cut.parts;
+}
+
+int token_logprobs_limits(const LogitRows& r, int top) {
+    const LogprobPlan pl = logprob_plan(r.rows, r.vocab, top, r.dtype);
+    if (grid_fits(r.rows * pl.cut.parts, pl.threads)) return CDX_OK;
+    return set_error(CDX_ERR_UNSUPPORTED, "token_logprobs: too many rows");
+}
+
+int distill_limits(const LogitRows& r) {
+    const DistillPlan pl = distill_plan(r.rows, r.vocab, r.dtype);
+    if (grid_fits(r.rows * pl.cut.parts, pl.threads)) return CDX_OK;
+    return set_error(CDX_ERR_UNSUPPORTED, "distill_loss: too many rows");
 }
 
 int launch_token_logprobs(const TokenLogprobArgs& a, void* ws, hipStream_t stream) {

@@ -48,6 +48,10 @@ struct DistillArgs {
 size_t distill_workspace(int64_t rows, int64_t vocab, int dtype, int count);
 int launch_distill(const DistillArgs& a, void* ws, hipStream_t stream);
 
+// Whether a launch holds that many rows (the entry points ask before they launch).
+int token_logprobs_limits(const LogitRows& r, int top);
+int distill_limits(const LogitRows& r);
+
 // How many workgroups share a row (for tests that aim at one way or the other).
 int token_logprobs_parts(int64_t rows, int64_t vocab, int top);
 int distill_parts(int64_t rows, int64_t vocab, int dtype);

@@ -655,7 +655,8 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
  *     the lowest index first among equals, with their l.
  * Logits of -infinity have probability 0.  A row of -infinity alone has logprob -infinity, entropy 0 and
  * no gradient.  A NaN or +infinity makes its row's numbers NaN; top_index is then some index in the
- * vocabulary.  workspace: the query's bytes, 16-byte aligned; NULL allocates stream-ordered.
+ * vocabulary.  Results must not overlap each other, logits or targets.
+ * workspace: the query's bytes, 16-byte aligned; NULL allocates stream-ordered.
  * Rows, one workgroup each, are up to 2^24 - 1, and up to 2^22 - 1 of 128 KB and more (else
  * CDX_ERR_UNSUPPORTED).  No counterpart in the reference. */
 size_t cdx_token_logprobs_workspace_size(int64_t rows, int64_t vocab, int top);
@@ -667,7 +668,7 @@ int cdx_token_logprobs(const void* logits, int64_t ldx, int64_t rows, int64_t vo
 /* grad_logits[r][v] = (g ([v = target] - p) - h p (l + entropy[r])) / T, p = exp(l), g = grad_logprob[r]
  * (0 for a negative target), h = grad_entropy[r]; either may be NULL (0), grad_entropy needs entropy.
  * Rows of g = h = 0 become zeros whatever they hold.  grad_logits (dtype) may be the logits' own
- * place (the same pointer and leading dimension). */
+ * place (the same pointer and leading dimension), and must not overlap anything else. */
 int cdx_token_logprobs_backward(const float* grad_logprob, const void* logits, int64_t ldx, int64_t rows,
                                 int64_t vocab, int dtype, double temperature, const int64_t* targets,
                                 const float* stats, const float* entropy, const float* grad_entropy,
@@ -680,8 +681,9 @@ int cdx_token_logprobs_backward(const float* grad_logprob, const void* logits, i
  *   grad_logits[r][v] = weight[r] / T (exp(l_v) - sum of q_k with index_k = v)
  * (0 there, where weight[r] is 0, and in a row of logits that are all -infinity).  weight NULL: the loss alone, and
  * grad_logits is not written.  An index may come more than once; one past the vocabulary makes its
- * row's loss and gradient NaN.  grad_logits (dtype) may be the logits' own place.  Rows and
- * workspace as above. */
+ * row's loss and gradient NaN.  grad_logits (dtype) may be the logits' own place (and is
+ * refused where teacher, index or weight lie in it: workgroups of one row read them while others write);
+ * loss and grad_logits must not overlap anything else.  Rows and workspace as above. */
 size_t cdx_distill_loss_workspace_size(int64_t rows, int64_t vocab, int count);
 int cdx_distill_loss(const void* logits, int64_t ldx, int64_t rows, int64_t vocab, int dtype,
                      double temperature, const void* index, int64_t ldi, int index_bytes,

@@ -74,7 +74,7 @@ void linear16_slope_kernel(const T* __restrict__ grad, int64_t ldg, const T* __r
             load_n<8>(z + r * ldz + c, count, v);
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = act_slope<T, ACT>(g[j], v[j], 0.0f);
+        for (int j = 0; j < 8; ++j) v[j] = layer_slope<T, ACT>(g[j], v[j]);
         store_n<8>(dz + r * lddz + c, count, v);
     }
 }
@@ -101,7 +101,7 @@ void linear16_slope_sums_kernel(const T* __restrict__ grad, int64_t ldg, const T
     auto use = [&](int64_t r, float (&g)[8], float (&v)[8]) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            v[j] = act_slope<T, ACT>(g[j], v[j], 0.0f);
+            v[j] = layer_slope<T, ACT>(g[j], v[j]);
             // (an fp32 value of its own, as in the kernel above: multiplied and rounded to float16 in one instruction it
             // could end in another bit)
             asm("" : "+v"(v[j]));

@@ -188,6 +188,19 @@ template <bool COLS, int EXT, int NT> struct Loader {
     }
 };
 
+// ---- activations -----------------------------------------------------------------------------
+
+// The activation and grad times its slope.  ReLU lets NaN through, as the others do by themselves: a layer that
+// turned NaN shows it.
+template <class T, int ACT> __device__ __forceinline__ float layer_value(float v) {
+    if constexpr (ACT == CDX_EPI_RELU) return v <= 0.0f ? 0.0f : v;
+    else return act_value<T, ACT>(v, 0.0f);
+}
+template <class T, int ACT> __device__ __forceinline__ float layer_slope(float g, float v) {
+    if constexpr (ACT == CDX_EPI_RELU) return v <= 0.0f ? 0.0f : g;
+    else return act_slope<T, ACT>(g, v, 0.0f);
+}
+
 // ---- results ---------------------------------------------------------------------------------
 
 // W sums of row m from column n on (the first `count` exist) through bias, activation and residual.
@@ -200,7 +213,7 @@ __device__ __forceinline__ void finish(const Linear16Out& o, int64_t m, int64_t 
     float r[W] = {};
     if (o.residual) load_n<W>(static_cast<const T*>(o.residual) + m * o.ldr + n, count, r);
 #pragma unroll
-    for (int j = 0; j < W; ++j) v[j] = act_value<T, ACT>(v[j], 0.0f);
+    for (int j = 0; j < W; ++j) v[j] = layer_value<T, ACT>(v[j]);
     if (o.residual) {   // (adding a zero would turn -0 into 0)
 #pragma unroll
         for (int j = 0; j < W; ++j) v[j] += r[j];

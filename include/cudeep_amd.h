@@ -613,7 +613,8 @@ int cdx_linear_weight_grad_e4m3(const void* dz, int64_t lddz, int dtype,
  * and z [M,N], all in dtype (CDX_DTYPE_F16 or _BF16); bias [N] in dtype or CDX_DTYPE_F32.  Sums,
  * bias, activation and residual are fp32, y is rounded once.  bias, residual and z (what the
  * backward pass takes, rounded to dtype; y comes from the unrounded one) may be NULL.  epilogue:
- * CDX_EPI_NONE to _SIGMOID, with the hardware's exponential and reciprocal.  y may be
+ * CDX_EPI_NONE to _SIGMOID, with the hardware's exponential and reciprocal; NaN stays NaN through each
+ * (through ReLU too, whose slope at NaN is 1).  y may be
  * residual itself (the same pointer and leading dimension); y and z must not overlap anything
  * else.  workspace: the query's bytes, 16-byte aligned; NULL allocates stream-ordered.  Products
  * of 2^23 output tiles and more (of 256 x 256, fewer rows or columns 128 x 128 or 64 x 64) are

@@ -109,9 +109,11 @@ SIGNATURES = {
     "cdx_linear_weight_grad_e4m3": (_int, [_vp, _i64, _int, _vp, _i64, _vp, _i64, _vp, _vp, _i64,
                                            _i64, _i64, _vp, _sz, _vp]),
     "cdx_linear16_workspace_size": (_sz, [_i64] * 3),
+    "cdx_linear16_call_workspace_size": (_sz, [_i64, _i64, _i64, _vp, _i64, _vp, _i64]),
     "cdx_linear16": (_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _int, _vp, _i64, _vp, _i64,
                             _vp, _i64, _int, _int, _vp, _sz, _vp]),
     "cdx_linear16_backward_workspace_size": (_sz, [_i64] * 3 + [_int]),
+    "cdx_linear16_backward_call_workspace_size": (_sz, [_i64, _i64, _i64] + [_vp, _i64] * 3 + [_int] * 4),
     "cdx_linear16_backward": (_int, [_i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _int,
                                      _vp, _i64, _vp, _vp, _int, _int, _vp, _sz, _vp]),
     "cdx_token_logprobs_workspace_size": (_sz, [_i64, _i64, _int]),

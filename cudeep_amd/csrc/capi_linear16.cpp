@@ -58,6 +58,13 @@ size_t cdx_linear16_workspace_size(int64_t M, int64_t N, int64_t K) {
     return cdx::linear16_workspace(Linear16Kind::Forward, M, N, K, false);
 }
 
+size_t cdx_linear16_call_workspace_size(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
+                                        const void* weight, int64_t ldw) {
+    if (no_layer(M, N, K)) return 0;
+    return cdx::linear16_workspace(Linear16Kind::Forward, M, N, K,
+                                   cdx::linear16_aligned(Linear16Kind::Forward, M, N, x, ldx, weight, ldw), false);
+}
+
 int cdx_linear16(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, const void* weight,
                  int64_t ldw, const void* bias, int bias_dtype, const void* residual, int64_t ldr,
                  void* y, int64_t ldy, void* z, int64_t ldz, int epilogue, int dtype,
@@ -91,7 +98,7 @@ int cdx_linear16(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx, co
     p.out.residual = residual; p.out.ldr = ldr;
     p.out.bias = bias; p.out.bias_f32 = bias_dtype == CDX_DTYPE_F32;
     p.out.act = epilogue;
-    return with_workspace(fn, cdx_linear16_workspace_size(M, N, K), workspace, workspace_bytes, stream,
+    return with_workspace(fn, cdx_linear16_call_workspace_size(M, N, K, x, ldx, weight, ldw), workspace, workspace_bytes, stream,
                           [&](void* ws) {
                               return cdx::launch_linear16(Linear16Kind::Forward, p, false, nullptr, ws, stream);
                           });
@@ -102,6 +109,26 @@ size_t cdx_linear16_backward_workspace_size(int64_t M, int64_t N, int64_t K, int
     const size_t dx = cdx::linear16_workspace(Linear16Kind::Input, M, K, N, false);
     const size_t dw = cdx::linear16_workspace(Linear16Kind::Weight, N, K, M, true);
     return slope_bytes(M, N, epilogue) + slope_sums_bytes(M, N, epilogue) + (dx > dw ? dx : dw);
+}
+
+size_t cdx_linear16_backward_call_workspace_size(int64_t M, int64_t N, int64_t K, const void* grad_out, int64_t ldg,
+                                                 const void* x, int64_t ldx, const void* weight, int64_t ldw,
+                                                 int epilogue, int input, int params, int bias) {
+    if (no_layer(M, N, K) || !gemm_epilogue(epilogue)) return 0;
+    // (dz in the workspace begins on 16 bytes, in rows of whole 8)
+    const bool own = epilogue != CDX_EPI_NONE;
+    const void* dz = own ? nullptr : grad_out;
+    const int64_t lddz = own ? cdx::ceil_div(N, (int64_t)8) * 8 : ldg;
+    const bool sums = bias && rounds_slope(epilogue);   // beside the slopes
+    size_t dx = 0, dw = 0;
+    if (input)
+        dx = cdx::linear16_workspace(Linear16Kind::Input, M, K, N,
+                                     cdx::linear16_aligned(Linear16Kind::Input, M, K, dz, lddz, weight, ldw), false);
+    if (params)
+        dw = cdx::linear16_workspace(Linear16Kind::Weight, N, K, M,
+                                     cdx::linear16_aligned(Linear16Kind::Weight, N, K, dz, lddz, x, ldx), bias && !sums);
+    if (!input && !params && !bias) return 0;
+    return slope_bytes(M, N, epilogue) + (sums ? slope_sums_bytes(M, N, epilogue) : 0) + (dx > dw ? dx : dw);
 }
 
 int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out, int64_t ldg,
@@ -140,7 +167,10 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
         return st;
     }
     return with_workspace(
-        fn, cdx_linear16_backward_workspace_size(M, N, K, epilogue), workspace, workspace_bytes, stream,
+        fn,
+        cdx_linear16_backward_call_workspace_size(M, N, K, grad_out, ldg, x, ldx, weight, ldw, epilogue, dx,
+                                                  grad_weight && K > 0, dw && grad_bias),
+        workspace, workspace_bytes, stream,
         [&](void* ws) {
             const void* dz = grad_out;
             int64_t lddz = ldg;
@@ -151,16 +181,16 @@ int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out,
                 lddz = cdx::ceil_div(N, (int64_t)8) * 8;
                 part += slope_bytes(M, N, epilogue);
                 int e;
-                if (grad_bias && rounds_slope(epilogue)) {
+                if (grad_bias && rounds_slope(epilogue)) {   // (its parts are the workspace's too)
                     e = cdx::launch_linear16_slope_sums(grad_out, ldg, z, ldz, ws, lddz, M, N, dtype, epilogue, grad_bias,
                                                         f32, reinterpret_cast<float*>(part), stream);
                     bias_sums = nullptr;
+                    part += slope_sums_bytes(M, N, epilogue);
                 } else {
                     e = cdx::launch_linear16_slope(grad_out, ldg, z, ldz, ws, lddz, M, N, dtype, epilogue, stream);
                 }
                 if (e) return e;
                 dz = ws;
-                part += slope_sums_bytes(M, N, epilogue);
             }
             if (dx) {
                 cdx::Linear16Product p{M, K, N, dz, lddz, weight, ldw, dtype, {}};

@@ -296,17 +296,23 @@ int launch_plan(Linear16Kind kind, const Linear16Product& g, const Plan& pl, boo
 
 }  // namespace
 
-size_t linear16_workspace(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool col_sums) {
+size_t linear16_workspace(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned, bool col_sums) {
     if (M == 0 || N == 0) return 0;
-    // (alignment may choose the kernel: the larger of both)
-    size_t most = 0;
-    for (int aligned = 0; aligned < 2; ++aligned) {
-        const Plan pl = plan_of(kind, M, N, K, aligned);
-        const size_t need = pl.slices > 1
-            ? (size_t)pl.slices * ((size_t)M * (size_t)N + (col_sums ? (size_t)M : 0)) * 4 : 0;
-        most = need > most ? need : most;
-    }
-    return most;
+    const Plan pl = plan_of(kind, M, N, K, aligned);
+    if (pl.slices == 1) return 0;
+    return (size_t)pl.slices * ((size_t)M * (size_t)N + (col_sums ? (size_t)M : 0)) * 4;
+}
+
+size_t linear16_workspace(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool col_sums) {
+    const size_t a = linear16_workspace(kind, M, N, K, false, col_sums);
+    const size_t b = linear16_workspace(kind, M, N, K, true, col_sums);
+    return a > b ? a : b;
+}
+
+bool linear16_aligned(Linear16Kind kind, int64_t M, int64_t N, const void* a, int64_t lda, const void* b, int64_t ldb) {
+    const bool ca = kind == Linear16Kind::Weight, cb = kind != Linear16Kind::Forward;
+    return lda % 8 == 0 && ldb % 8 == 0 && ((uintptr_t)a | (uintptr_t)b) % 16 == 0 && lda <= kMaxLd && ldb <= kMaxLd &&
+           (!ca || M % 8 == 0) && (!cb || N % 8 == 0);
 }
 
 const char* linear16_kernel_name(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned,
@@ -319,9 +325,7 @@ const char* linear16_kernel_name(Linear16Kind kind, int64_t M, int64_t N, int64_
 
 int launch_linear16(Linear16Kind kind, const Linear16Product& g, bool out_f32, void* col_y, void* ws,
                     hipStream_t stream) {
-    const bool ca = kind == Linear16Kind::Weight, cb = kind != Linear16Kind::Forward;
-    const bool aligned = g.lda % 8 == 0 && g.ldb % 8 == 0 && ((uintptr_t)g.a | (uintptr_t)g.b) % 16 == 0 &&
-                         g.lda <= kMaxLd && g.ldb <= kMaxLd && (!ca || g.M % 8 == 0) && (!cb || g.N % 8 == 0);
+    const bool aligned = linear16_aligned(kind, g.M, g.N, g.a, g.lda, g.b, g.ldb);
     return launch_plan(kind, g, plan_of(kind, g.M, g.N, g.K, aligned), out_f32, col_y, ws, stream);
 }
 

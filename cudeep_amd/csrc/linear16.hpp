@@ -28,7 +28,11 @@ struct Linear16Product {
 
 enum class Linear16Kind { Forward, Input, Weight };   // both rows; A rows, B columns; both columns
 
-// Bytes of partial sums that a product of this kind needs (0: none).
+// Whether operands allow wide loads, which may choose the kernel.
+bool linear16_aligned(Linear16Kind kind, int64_t M, int64_t N, const void* a, int64_t lda, const void* b, int64_t ldb);
+// Bytes of partial sums that a product of this kind needs (0: none), with such operands or without; the larger of
+// both.
+size_t linear16_workspace(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned, bool col_sums);
 size_t linear16_workspace(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool col_sums);
 // col_y (Weight products; may be null): the column sums sum_k A(m, k).  out_f32: y, dense, and col_y
 // hold fp32 instead of 16-bit values.

@@ -1053,9 +1053,10 @@ def linear16(x, weight, bias=None, *, epilogue=L.EPI_NONE, residual=None, keep=F
     if keep:
         z = x.new_empty(shape)
         zptr = z.data_ptr()
+    xptr, wptr = x.data_ptr(), weight.data_ptr()
     ws_ptr, ws_bytes, _keep = _workspace(
-        workspace, lambda: L.lib().cdx_linear16_workspace_size(M, N, K), x.device)
-    L.call("cdx_linear16", M, N, K, x.data_ptr(), ldx, weight.data_ptr(), ldw, bptr, bcode, rptr, ldr,
+        workspace, lambda: L.lib().cdx_linear16_call_workspace_size(M, N, K, xptr, ldx, wptr, ldw), x.device)
+    L.call("cdx_linear16", M, N, K, xptr, ldx, wptr, ldw, bptr, bcode, rptr, ldr,
            y.data_ptr(), ldy, zptr, N, epilogue, code, ws_ptr, ws_bytes, _stream())
     return (y, z) if keep else y
 
@@ -1095,11 +1096,13 @@ def linear16_backward(grad_out, x, weight, z=None, *, epilogue=L.EPI_NONE, input
         if bias:
             db = x.new_empty((N,), dtype=pdtype)
             bp = db.data_ptr()
+    gptr, xptr, wptr = grad_out.data_ptr(), x.data_ptr(), weight.data_ptr()
     ws_ptr, ws_bytes, _keep = _workspace(
-        workspace, lambda: L.lib().cdx_linear16_backward_workspace_size(M, N, K, epilogue), x.device)
-    L.call("cdx_linear16_backward", M, N, K, grad_out.data_ptr(), ldg, x.data_ptr(), ldx,
-           weight.data_ptr(), ldw, zptr, ldz, epilogue, xp, K, wp, bp, code, _FLOATS[pdtype], ws_ptr,
-           ws_bytes, _stream())
+        workspace, lambda: L.lib().cdx_linear16_backward_call_workspace_size(
+            M, N, K, gptr, ldg, xptr, ldx, wptr, ldw, epilogue, dx is not None, dw is not None, db is not None),
+        x.device)
+    L.call("cdx_linear16_backward", M, N, K, gptr, ldg, xptr, ldx, wptr, ldw, zptr, ldz, epilogue, xp, K, wp, bp, code,
+           _FLOATS[pdtype], ws_ptr, ws_bytes, _stream())
     return dx, dw, db
 
 

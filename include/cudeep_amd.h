@@ -616,10 +616,13 @@ int cdx_linear_weight_grad_e4m3(const void* dz, int64_t lddz, int dtype,
  * CDX_EPI_NONE to _SIGMOID, with the hardware's exponential and reciprocal; NaN stays NaN through each
  * (through ReLU too, whose slope at NaN is 1).  y may be
  * residual itself (the same pointer and leading dimension); y and z must not overlap anything
- * else.  workspace: the query's bytes, 16-byte aligned; NULL allocates stream-ordered.  Products
+ * else.  workspace: a query's bytes, 16-byte aligned (the first answers for operands of any
+ * alignment, the second for these ones, which may need less); NULL allocates stream-ordered.  Products
  * of 2^23 output tiles and more (of 256 x 256, fewer rows or columns 128 x 128 or 64 x 64) are
  * CDX_ERR_UNSUPPORTED.  The same bits every time.  No counterpart in the reference. */
 size_t cdx_linear16_workspace_size(int64_t M, int64_t N, int64_t K);
+size_t cdx_linear16_call_workspace_size(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
+                                        const void* weight, int64_t ldw);
 int cdx_linear16(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
                  const void* weight, int64_t ldw, const void* bias, int bias_dtype,
                  const void* residual, int64_t ldr, void* y, int64_t ldy, void* z, int64_t ldz,
@@ -635,8 +638,12 @@ int cdx_linear16(int64_t M, int64_t N, int64_t K, const void* x, int64_t ldx,
  * float16's largest value is an infinite operand: grad_out below 0.88 of it keeps clear of that.
  * param_dtype: dtype or CDX_DTYPE_F32.  grad_x, grad_weight and grad_bias may be NULL (W and x
  * then too), but grad_bias needs grad_weight.  Results must not overlap anything.
- * workspace as above. */
+ * workspace as above (input, params, bias: which gradients are asked for). */
 size_t cdx_linear16_backward_workspace_size(int64_t M, int64_t N, int64_t K, int epilogue);
+size_t cdx_linear16_backward_call_workspace_size(int64_t M, int64_t N, int64_t K, const void* grad_out,
+                                                 int64_t ldg, const void* x, int64_t ldx,
+                                                 const void* weight, int64_t ldw, int epilogue,
+                                                 int input, int params, int bias);
 int cdx_linear16_backward(int64_t M, int64_t N, int64_t K, const void* grad_out, int64_t ldg,
                           const void* x, int64_t ldx, const void* weight, int64_t ldw,
                           const void* z, int64_t ldz, int epilogue, void* grad_x, int64_t ldgx,

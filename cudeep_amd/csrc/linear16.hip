@@ -81,7 +81,9 @@ void linear16_slope_kernel(const T* __restrict__ grad, int64_t ldg, const T* __r
 
 // The same with the column sums of dz, which no matrix instruction needs in 16 bits: they are of the slopes'
 // fp32 values, before dz is rounded.  A workgroup has 256 columns of `chunk` rows, a thread eight columns of every
-// eighth row; its sums go to part[chunk's number], which the next kernel adds in their order.  8192 x 4096 with GELU
+// eighth row; its sums go to part[chunk's number], which the next kernel adds in their order.  Up to 32 rows are one part,
+// the result itself (`whole`, or part in fp32; a backward pass of 16 x 4096 x 4096 31.2 us, with a second launch 32.9; but
+// of 64 x 4096 x 1024 24.4 in one part, 23.3 in two).  8192 x 4096 with GELU
 // in bf16 38.9 us and 1.4 for the parts (34.3 without sums), 8192 x 256 6.1 and 2.4 (5.5), 32768 x 512 19.6 and 4.6
 // (19.3); a float32 bias gradient of 8192 rows is off by 1.5e-7 of its norm, by 1.7e-3 from the rounded dz.
 constexpr int kSlopeCols = 256;
@@ -90,7 +92,7 @@ template <class T, int ACT, bool PAST>
 __global__ __launch_bounds__(256)
 void linear16_slope_sums_kernel(const T* __restrict__ grad, int64_t ldg, const T* __restrict__ z, int64_t ldz,
                                 T* __restrict__ dz, int64_t lddz, int64_t rows, int64_t cols, int64_t chunk,
-                                float* __restrict__ part) {
+                                float* __restrict__ part, T* __restrict__ whole) {
     constexpr int U = 4, LANES = kSlopeCols / 8, STEP = 256 / LANES;
     __shared__ float red[STEP][kSlopeCols];
     const int lane = threadIdx.x % LANES, r0 = threadIdx.x / LANES;
@@ -149,7 +151,8 @@ void linear16_slope_sums_kernel(const T* __restrict__ grad, int64_t ldg, const T
     float v = red[0][threadIdx.x];
 #pragma unroll
     for (int i = 1; i < STEP; ++i) v += red[i][threadIdx.x];
-    part[(int64_t)blockIdx.y * cols + n] = v;
+    if (whole) whole[n] = (T)v;
+    else part[(int64_t)blockIdx.y * cols + n] = v;
 }
 
 // The parts' sums, in their order: 16 columns a workgroup, 16 threads a column.
@@ -350,7 +353,8 @@ int launch_linear16_slope(const void* grad, int64_t ldg, const void* z, int64_t 
 
 size_t linear16_slope_sums_workspace(int64_t rows, int64_t cols) {
     if (rows == 0 || cols == 0) return 0;
-    return (size_t)slope_parts(rows, cols).parts * (size_t)cols * sizeof(float);
+    const int parts = slope_parts(rows, cols).parts;
+    return parts > 1 ? (size_t)parts * (size_t)cols * sizeof(float) : 0;
 }
 
 int launch_linear16_slope_sums(const void* grad, int64_t ldg, const void* z, int64_t ldz, void* dz,
@@ -360,13 +364,15 @@ int launch_linear16_slope_sums(const void* grad, int64_t ldg, const void* z, int
     const int64_t strips = ceil_div(cols, (int64_t)kSlopeCols), joins = ceil_div(cols, (int64_t)16);
     if (!grid_fits(strips * sp.parts, 256) || !grid_fits(joins, 256))
         return set_error(CDX_ERR_UNSUPPORTED, "linear16: too many columns");
+    if (sp.parts == 1 && sums_f32) part = static_cast<float*>(sums);
     return with_16(dtype, [&](auto t) {
         using T = decltype(t);
+        T* whole = sp.parts == 1 && !sums_f32 ? static_cast<T*>(sums) : nullptr;
         const dim3 grid((unsigned)strips, (unsigned)sp.parts);
         auto run = [&](auto a, auto past) {
             hipLaunchKernelGGL((linear16_slope_sums_kernel<T, decltype(a)::value, decltype(past)::value>), grid,
                                dim3(256), 0, stream, static_cast<const T*>(grad), ldg, static_cast<const T*>(z),
-                               ldz, static_cast<T*>(dz), lddz, rows, cols, sp.chunk, part);
+                               ldz, static_cast<T*>(dz), lddz, rows, cols, sp.chunk, part, whole);
         };
         const bool past = past_caches(rows, cols, dtype);
         auto go = [&](auto a) { past ? run(a, std::true_type{}) : run(a, std::false_type{}); };
@@ -374,7 +380,7 @@ int launch_linear16_slope_sums(const void* grad, int64_t ldg, const void* z, int
         else if (act == CDX_EPI_SILU) go(std::integral_constant<int, CDX_EPI_SILU>{});
         else go(std::integral_constant<int, CDX_EPI_SIGMOID>{});
         const int st = hip_error(hipGetLastError(), "linear16_slope_sums_kernel launch");
-        if (st) return st;
+        if (st || sp.parts == 1) return st;
         if (sums_f32)
             hipLaunchKernelGGL(linear16_slope_join_kernel<float>, dim3((unsigned)joins), dim3(256), 0, stream, part,
                                sp.parts, cols, static_cast<float*>(sums));

@@ -259,6 +259,17 @@ Plan plan_of(Linear16Kind kind, int64_t M, int64_t N, int64_t K, bool aligned) {
     return make_plan(Kernel::Ring64, M, N, K, 64, cut(t64, 256, 1024, 8));
 }
 
+// Calls f with an activation's code as a constant: those whose dz is rounded, and ReLU with them.
+template <class F> int with_smooth_act(int act, F f) {
+    using std::integral_constant;
+    if (act == CDX_EPI_GELU) return f(integral_constant<int, CDX_EPI_GELU>{});
+    if (act == CDX_EPI_SILU) return f(integral_constant<int, CDX_EPI_SILU>{});
+    return f(integral_constant<int, CDX_EPI_SIGMOID>{});
+}
+template <class F> int with_layer_act(int act, F f) {
+    return act == CDX_EPI_RELU ? f(std::integral_constant<int, CDX_EPI_RELU>{}) : with_smooth_act(act, f);
+}
+
 unsigned wide_grid(int64_t threads) {
     const int64_t g = ceil_div(threads, (int64_t)256);
     return (unsigned)(g < 65536 ? g : 65536);
@@ -337,7 +348,7 @@ int launch_linear16_slope(const void* grad, int64_t ldg, const void* z, int64_t 
                           hipStream_t stream) {
     return with_16(dtype, [&](auto t) {
         using T = decltype(t);
-        return with_act(act, [&](auto a) {
+        return with_layer_act(act, [&](auto a) {
             const dim3 grid(wide_grid(rows * ceil_div(cols, (int64_t)8)));
             auto go = [&](auto past) {
                 hipLaunchKernelGGL((linear16_slope_kernel<T, decltype(a)::value, decltype(past)::value>), grid,
@@ -375,10 +386,10 @@ int launch_linear16_slope_sums(const void* grad, int64_t ldg, const void* z, int
                                ldz, static_cast<T*>(dz), lddz, rows, cols, sp.chunk, part, whole);
         };
         const bool past = past_caches(rows, cols, dtype);
-        auto go = [&](auto a) { past ? run(a, std::true_type{}) : run(a, std::false_type{}); };
-        if (act == CDX_EPI_GELU) go(std::integral_constant<int, CDX_EPI_GELU>{});
-        else if (act == CDX_EPI_SILU) go(std::integral_constant<int, CDX_EPI_SILU>{});
-        else go(std::integral_constant<int, CDX_EPI_SIGMOID>{});
+        with_smooth_act(act, [&](auto a) {
+            past ? run(a, std::true_type{}) : run(a, std::false_type{});
+            return 0;
+        });
         const int st = hip_error(hipGetLastError(), "linear16_slope_sums_kernel launch");
         if (st || sp.parts == 1) return st;
         if (sums_f32)

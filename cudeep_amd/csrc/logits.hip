@@ -786,12 +786,14 @@ int run_logprob(const LogprobParams& p, int threads, hipStream_t stream) {
     const int64_t groups = p.r.rows * p.parts;
     auto go = [&](auto ent, auto top) {
         constexpr bool ENT = decltype(ent)::value, TOP = decltype(top)::value;
-        if (threads == 1024)
-            hipLaunchKernelGGL((logprob_kernel<T, 1024, ENT, TOP>), dim3((unsigned)groups), dim3(1024), 0, stream, p);
-        else if (threads == 512)
-            hipLaunchKernelGGL((logprob_kernel<T, 512, ENT, TOP>), dim3((unsigned)groups), dim3(512), 0, stream, p);
-        else
-            hipLaunchKernelGGL((logprob_kernel<T, 256, ENT, TOP>), dim3((unsigned)groups), dim3(256), 0, stream, p);
+        auto run = [&](auto nt) {
+            constexpr int NT = decltype(nt)::value;
+            hipLaunchKernelGGL((logprob_kernel<T, NT, ENT, TOP>), dim3((unsigned)groups), dim3(NT), 0, stream, p);
+        };
+        constexpr int MOST = TOP ? 512 : 1024;   // (logprob_plan)
+        if (threads == 256) run(std::integral_constant<int, 256>{});
+        else if (threads == 512) run(std::integral_constant<int, 512>{});
+        else run(std::integral_constant<int, MOST>{});
         int st = hip_error(hipGetLastError(), "logprob_kernel launch");
         if (st || p.parts == 1) return st;
         hipLaunchKernelGGL((logprob_join_kernel<T, ENT, TOP>), dim3((unsigned)p.r.rows), dim3(kJoinThreads), 0, stream, p);

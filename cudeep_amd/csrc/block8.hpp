@@ -130,9 +130,10 @@ __device__ __forceinline__ void store_n(T* p, int n, const float (&v)[N]) {
 
 // 16 bytes that are read for the last time, or written and not read soon, with PAST: they pass the caches by, and
 // what those hold for others stays there.  It pays from about a quarter of the 256 MB cache on, with
-// operands that change from call to call: loss and gradient of 513 x 50001 logits (103 MB) in fp32 48.8 us,
-// 66.1 with ordinary loads and stores; gradient of 1021 x 50001 with the forward pass before it 98 and
-// 120; 4096 x 65536 in bf16 226 and 247.
+// operands that change from call to call: the slopes of a Linear layer in 16 bits, with the products that read
+// them, of 8192 x 6144 (101 MB, 1024 inputs) 262 us, 288 with ordinary loads, and with a reading of grad as the
+// residual's gradient behind them 295 and 321; of 67 MB 186 and 187 (207 and 224), of 59 MB 171.5 and 170.0 (190.7 and
+// 187.0), of 403 MB 994 and 985 (1121 and 1121).  Gradients of logits: logits.hip.
 typedef u32x4 __attribute__((aligned(1))) u32x4_any;
 template <bool PAST> __device__ __forceinline__ u32x4 load16_as(const void* p) {
     if constexpr (PAST) return __builtin_nontemporal_load(static_cast<const u32x4_any*>(p));

@@ -140,3 +140,8 @@ extern "C" int cdxi_logits_parts(int op, int64_t rows, int64_t vocab, int top) {
     return op ? cdx::distill_parts(rows, vocab, CDX_DTYPE_F32)
               : cdx::token_logprobs_parts(rows, vocab, top);
 }
+
+// Internal: what of a gradient of that size passes the caches by (0 nothing, 1 its logits, 2 both).
+extern "C" int cdxi_logits_past_caches(int64_t rows, int64_t vocab, int dtype) {
+    return cdx::gradient_past_caches(rows, vocab, dtype);
+}

@@ -47,9 +47,9 @@ void linear16_sum_kernel(Params p, const float* __restrict__ part, const float* 
 }
 
 // dz = grad act'(z), eight columns a thread, one pass that memory bounds (8192 x 4096 in bf16 36 us, 5.6 TB/s:
-// some of z is in the caches).  PAST: grad and z, which nobody reads again, pass the caches by
+// some of z is in the caches).  PAST: grad and z pass the caches by
 // (block8.hpp), so that dz is there for the products: a training step of 8192 x 4096 x 4096 727 us, 741
-// without.
+// without.  (grad, as the residual's gradient, may be read once more behind them: no slower for it.)
 template <class T, int ACT, bool PAST>
 __global__ __launch_bounds__(256)
 void linear16_slope_kernel(const T* __restrict__ grad, int64_t ldg, const T* __restrict__ z, int64_t ldz,

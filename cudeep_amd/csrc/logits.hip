@@ -12,7 +12,8 @@
 // logits (-infinity, or a type's lowest value) never meet infinity - infinity; a row of -infinity
 // alone has S = 0, and L = -infinity says so.
 //
-// Gradients of 64 MB and more are written, and their logits read for the last time, past the caches: what
+// Of gradients of 64 MB and more the logits are read for the last time past the caches, and those that the caches
+// would not hold until the next product reads them are written past them too (enum Past): what
 // those hold of rows that are read again stays there.
 #include "logits.hpp"
 
@@ -436,10 +437,34 @@ void logprob_join_kernel(LogprobParams p) {
 // The gradient, element by element: a workgroup takes kBackward elements of a row.  Memory bounds it, 1021 x
 // 50001 in fp32 61.9 us, 6.6 TB/s read and written (62.1 with the rows in reverse, which begins with those
 // that were read last).
+// What of a gradient passes the caches: nothing; its logits, read for the last time; both.  Measured with what reads
+// the gradient next, a bf16 product of 50304 or 32000 logits with 1024 columns, us, nothing / logits / both:
+//   bf16   48 MB 229.9 226.4 226.5 (in place 226.6 226.2 227.6)    64 MB 280.7 274.7 277.8 (270.5 270.2 272.4)
+//         100 MB 448.8 440.5 478.6 (432.9 443.6 463.5)            160 MB 590.0 576.3 572.7 (554.1 570.0 572.3)
+//         200 MB 766.4 759.8 750.0 (712.3 734.1 744.7)            400 MB 1422 1428 1398 (1416 1423 1400)
+//   fp32, rounded to bf16 in between
+//          63 MB 282.0 279.4 280.5 (277.7 279.5 276.3)            100 MB 353.2 348.4 355.0 (347.4 350.3 349.3)
+//         129 MB 437.7 429.2 423.9 (424.8 426.7 423.2)            259 MB 793.6 789.9 763.2 (775.3 784.5 754.4)
+// So both for fp32 from 64 MB on and for 16 bits from 200 MB on; below that, from 64 MB on, the logits alone (by itself, loss and gradient of 100 MB in bf16 57.5 54.5 52.2, of 513 x 50001 in fp32 66.1 with
+// nothing, 48.8 with both).
+enum class Past { None, Logits, Both };
+Past gradient_past(const LogitRows& r) {
+    if (!past_caches(r.rows, r.vocab, r.dtype)) return Past::None;
+    return r.dtype == CDX_DTYPE_F32 || (double)r.rows * (double)r.vocab * 2 >= 200e6 ? Past::Both : Past::Logits;
+}
+// Calls f with it as a constant (Logits alone: 16 bits).
+template <class T, class F> void with_past(Past past, F f) {
+    using std::integral_constant;
+    if (past == Past::Both) return f(integral_constant<Past, Past::Both>{});
+    if constexpr (sizeof(T) == 2)
+        if (past == Past::Logits) return f(integral_constant<Past, Past::Logits>{});
+    f(integral_constant<Past, Past::None>{});
+}
+
 constexpr int kBackwardThreads = 256;
 template <class T> constexpr int kBackward = kBackwardThreads * kUnroll * kVec<T>;
 
-template <class T, bool STREAM>
+template <class T, Past PAST>
 __global__ __launch_bounds__(kBackwardThreads)
 void logprob_backward_kernel(LogitRows r, const int64_t* __restrict__ targets, const float* __restrict__ stats,
                              const float* __restrict__ g_lp, const float* __restrict__ entropy,
@@ -481,7 +506,7 @@ void logprob_backward_kernel(LogitRows r, const int64_t* __restrict__ targets, c
         u32x4 u[kUnroll];
         if (!none) {   // (a row without a gradient is not read)
 #pragma unroll
-            for (int i = 0; i < kUnroll; ++i) u[i] = load16_as<STREAM>(x + at0 + i * STRIDE);
+            for (int i = 0; i < kUnroll; ++i) u[i] = load16_as<PAST != Past::None>(x + at0 + i * STRIDE);
         }
 #pragma unroll
         for (int i = 0; i < kUnroll; ++i) {
@@ -491,7 +516,7 @@ void logprob_backward_kernel(LogitRows r, const int64_t* __restrict__ targets, c
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = (float)e[j];
             gradient(v, at0 + i * STRIDE);
-            store16_as<STREAM, T>(out + at0 + i * STRIDE, v);
+            store16_as<PAST == Past::Both, T>(out + at0 + i * STRIDE, v);
         }
         return;
     }
@@ -609,7 +634,7 @@ __device__ __forceinline__ void grad_entries(const DistillArgs& a, T* out, int b
 
 // The gradient of elements begin .. end - 1, which are read again; all threads call it, with the row's entries
 // in LDS.
-template <class T, int NT, bool STREAM>
+template <class T, int NT, Past PAST>
 __device__ __forceinline__ void distill_grad(const DistillArgs& a, int64_t row, int begin, int end, const GradRow& g, const Entries& e) {
     constexpr int V = kVec<T>, U = kUnroll;
     const T* x = static_cast<const T*>(a.r.x) + row * a.r.ldx;
@@ -618,7 +643,7 @@ __device__ __forceinline__ void distill_grad(const DistillArgs& a, int64_t row, 
     for (; at + ((U - 1) * NT + 1) * V <= end; at += U * NT * V) {
         u32x4 u[U];
 #pragma unroll
-        for (int i = 0; i < U; ++i) u[i] = load16_as<STREAM>(x + at + i * NT * V);
+        for (int i = 0; i < U; ++i) u[i] = load16_as<PAST != Past::None>(x + at + i * NT * V);
 #pragma unroll
         for (int i = 0; i < U; ++i) {
             T t[V];
@@ -627,7 +652,7 @@ __device__ __forceinline__ void distill_grad(const DistillArgs& a, int64_t row, 
 #pragma unroll
             for (int j = 0; j < V; ++j) v[j] = (float)t[j];
             grad_values(g, v);
-            store16_as<STREAM, T>(out + at + i * NT * V, v);
+            store16_as<PAST == Past::Both, T>(out + at + i * NT * V, v);
         }
     }
     for (; at < end; at += NT * V) {
@@ -653,7 +678,7 @@ __device__ __forceinline__ void load_entries(const DistillArgs& a, int64_t row, 
 // A workgroup a row: sums, entries, and the gradient, for which the row is read again.  Memory bounds it:
 // 4096 x 65536 in bf16 with 64 entries 232 us, in which 0.86 GB are read (0.54 are the logits) and 0.54
 // written.  Rows kept in registers for the second reading do not fit (spills, 875 us against 247).
-template <class T, int NT, bool GRAD, bool STREAM>
+template <class T, int NT, bool GRAD, Past PAST>
 __global__ __launch_bounds__(NT)
 void distill_kernel(DistillArgs a) {
     __shared__ Part red[NT / 64];
@@ -672,7 +697,7 @@ void distill_kernel(DistillArgs a) {
     if (threadIdx.x == 0) a.loss[row] = loss;
     if constexpr (GRAD) {
         __syncthreads();
-        distill_grad<T, NT, STREAM>(a, row, 0, (int)a.r.vocab, grad_row(a, row, st, some, loss), e);
+        distill_grad<T, NT, PAST>(a, row, 0, (int)a.r.vocab, grad_row(a, row, st, some, loss), e);
     }
 }
 
@@ -729,7 +754,7 @@ void distill_join_kernel(DistillParams p) {
         const int begin = part * p.length;
         const int end = a.r.vocab - begin < p.length ? (int)a.r.vocab : begin + p.length;
         __syncthreads();
-        distill_grad<T, NT, false>(a, row, begin, end, grad_row(a, row, st, some, loss), e);
+        distill_grad<T, NT, Past::None>(a, row, begin, end, grad_row(a, row, st, some, loss), e);
     }
 }
 
@@ -810,15 +835,15 @@ int run_distill(const DistillParams& p, const DistillPlan& pl, hipStream_t strea
     const DistillArgs& a = p.a;
     const dim3 rows((unsigned)a.r.rows), all((unsigned)(a.r.rows * p.parts)), threads(kDistillThreads);
     if (p.parts == 1) {
-        auto go = [&](auto threads, auto grad, auto stream_past) {
-            constexpr int NT = decltype(threads)::value;
-            hipLaunchKernelGGL((distill_kernel<T, NT, decltype(grad)::value, decltype(stream_past)::value>), rows, dim3(NT), 0, stream, a);
-        };
-        const bool past = past_caches(a.r.rows, a.r.vocab, a.r.dtype);
         auto kind = [&](auto threads) {
-            if (!a.weight) go(threads, std::false_type{}, std::false_type{});
-            else if (past) go(threads, std::true_type{}, std::true_type{});
-            else go(threads, std::true_type{}, std::false_type{});
+            constexpr int NT = decltype(threads)::value;
+            if (!a.weight) {
+                hipLaunchKernelGGL((distill_kernel<T, NT, false, Past::None>), rows, dim3(NT), 0, stream, a);
+                return;
+            }
+            with_past<T>(gradient_past(a.r), [&](auto past) {
+                hipLaunchKernelGGL((distill_kernel<T, NT, true, decltype(past)::value>), rows, dim3(NT), 0, stream, a);
+            });
         };
         if (pl.threads == 1024) kind(std::integral_constant<int, 1024>{});
         else if (pl.threads == 512) kind(std::integral_constant<int, 512>{});
@@ -886,12 +911,10 @@ int launch_token_logprobs_backward(const LogitRows& r, const int64_t* targets, c
         if (!grid_fits(r.rows * parts, kBackwardThreads))
             return set_error(CDX_ERR_UNSUPPORTED, "token_logprobs_backward: too many elements");
         const dim3 grid((unsigned)(r.rows * parts)), threads(kBackwardThreads);
-        if (past_caches(r.rows, r.vocab, r.dtype))
-            hipLaunchKernelGGL((logprob_backward_kernel<T, true>), grid, threads, 0, stream, r, targets, stats, g,
-                               entropy, gh, static_cast<T*>(grad), ldg, (int)parts);
-        else
-            hipLaunchKernelGGL((logprob_backward_kernel<T, false>), grid, threads, 0, stream, r, targets, stats, g,
-                               entropy, gh, static_cast<T*>(grad), ldg, (int)parts);
+        with_past<T>(gradient_past(r), [&](auto past) {
+            hipLaunchKernelGGL((logprob_backward_kernel<T, decltype(past)::value>), grid, threads, 0, stream, r, targets,
+                               stats, g, entropy, gh, static_cast<T*>(grad), ldg, (int)parts);
+        });
         return hip_error(hipGetLastError(), "logprob_backward_kernel launch");
     });
 }
@@ -905,6 +928,10 @@ size_t distill_workspace(int64_t rows, int64_t vocab, int dtype, int count) {
 
 int distill_parts(int64_t rows, int64_t vocab, int dtype) {
     return distill_plan(rows, vocab, dtype).cut.parts;
+}
+
+int gradient_past_caches(int64_t rows, int64_t vocab, int dtype) {
+    return (int)gradient_past({nullptr, vocab, rows, vocab, dtype, 1.0f});
 }
 
 int launch_distill(const DistillArgs& a, void* ws, hipStream_t stream) {

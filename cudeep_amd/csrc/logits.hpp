@@ -55,5 +55,7 @@ int distill_limits(const LogitRows& r);
 // How many workgroups share a row (for tests that aim at one way or the other).
 int token_logprobs_parts(int64_t rows, int64_t vocab, int top);
 int distill_parts(int64_t rows, int64_t vocab, int dtype);
+// What of a gradient passes the caches by: 0 nothing, 1 its logits, 2 both.
+int gradient_past_caches(int64_t rows, int64_t vocab, int dtype);
 
 }  // namespace cdx

@@ -410,7 +410,7 @@ struct Slice {
 
 // Operands of any alignment: every step through registers into the LDS buffer that is not being read, the
 // step after it on its way meanwhile; one barrier a step.  The loads' checks and the way through registers
-// bound it: 4096 x 4096 x 4001 in 128 x 128 tiles of eight waves 183 us, 734 TFLOP/s (aligned operands
+// bound it: 4096 x 4096 x 4001 in 128 x 128 tiles of eight waves 183 to 203 us from card to card, 734 to 660 TFLOP/s (aligned operands
 // of 4096, turns: 127).
 template <class T, bool CA, bool CB, int BM, int BN, int WM, int WN>
 __global__ __launch_bounds__(64 * WM * WN)
@@ -559,8 +559,9 @@ void linear16_tile_kernel(Params p) {
 //
 // 256 x 256 is the widest tile whose sums (128 registers a lane) and operands stay in registers: a step's LDS
 // reads are half of a 128 x 128 tile's for the same products.  Measured, bf16, 8192 x 4096 x 4096, from card
-// to card: forward 207 to 219 us (1330 to 1260 TFLOP/s), input gradient 204 to 222, weight gradient with bias
-// sums 212 to 224; 4096 x 4096 x 4096 119.  The matrix units' power bounds it: operands of zeros take 163 us (1690 TFLOP/s), and the clock is 2.4 GHz then,
+// to card: forward 207 to 234 us (1330 to 1175 TFLOP/s; a library product 174 to 198; with bias, residual, GELU and z 262),
+// input gradient 204 to 222, weight gradient with bias sums 212 to 224; 4096 x 4096 x 4096 110 to 119.  The energy of LDS
+// reads and matrix units bounds it: operands of zeros take 163 us (1690 TFLOP/s), and the clock is 2.4 GHz then,
 // 1.9 to 2.2 with random ones, of whose cycles matrix instructions take 50 to 57 %.
 template <class T, bool CA, bool CB>
 __global__ __launch_bounds__(512, 2)
